@@ -234,6 +234,100 @@ sdm_status sdm_tied_project(const void* h, const void* emb, int64_t N, int d, in
 sdm_status sdm_embed(const int32_t* ids, const void* emb, int64_t N, int d, int V, int dtype, void* out, int* bad,
                      void* stream);
 
+/* ------------------------------------------------------------------------------------- rules on logits, choice
+ * The rules a serving loop puts on a row of logits before it picks a token.  For row s and token v, in float32:
+ *   x = logits[s, v]
+ *   v occurs in history[s, 0 .. history_len[s])                      x > 0 ? x / repetition : x * repetition
+ *   v occurs g times in history[s, prompt_len[s] .. history_len[s])  x - frequency * g, then x - presence if g > 0
+ *   v has bias entries                                               x + their sum, taken in the entries' order
+ *   v's bit in the row's mask is 0                                   -infinity, whatever x was (NaN included)
+ * Every array is optional (NULL).  Without history nothing is penalised; without history_len a row's history is all
+ * history_n entries, without prompt_len all of it counts as generated; lengths are clamped to [0, history_n].  Ids
+ * outside [0, V) in history and bias_ids (padding, -1) are skipped.  repetition, frequency and presence are per row
+ * (S) where the pointer is given, else the value beside it.  mask holds mask_rows rows of ceil(V / 32) words, token
+ * v's bit at (word v / 32, bit v % 32), 1 = allowed; row s uses mask row mask_row[s] (outside [0, mask_rows): no
+ * mask), or row s (row 0 where mask_rows is 1) without mask_row. */
+typedef struct {
+  const int32_t* history;      /* (S, history_n), row stride history_ld */
+  int64_t history_ld;
+  int history_n;
+  const int32_t* history_len;  /* (S) */
+  const int32_t* prompt_len;   /* (S) */
+  const float* repetition;     /* (S) */
+  const float* frequency;      /* (S) */
+  const float* presence;       /* (S) */
+  float repetition_all, frequency_all, presence_all;
+  const int32_t* bias_ids;     /* (S, bias_n) */
+  const float* bias_values;    /* (S, bias_n) */
+  int bias_n;                  /* at most 1024 */
+  const int32_t* mask;         /* (mask_rows, ceil(V / 32)) */
+  int mask_rows;
+  const int32_t* mask_row;     /* (S) */
+} sdm_logit_rules;
+
+/* out (S, V) = the rules on logits (S, V), both in dtype, rounded once; row strides ld, ld_out in elements.  out may
+ * be logits itself (same stride), and may not overlap it otherwise.  V at most 2^30; rules may be NULL. */
+sdm_status sdm_logits_process(const sdm_logit_rules* rules, const void* logits, int64_t ld, int64_t S, int V,
+                              int dtype, void* out, int64_t ld_out, void* stream);
+
+/* One token per row from the processed logits y (which are not written).  NaN counts as -infinity.  With m the
+ * row's largest y, t = (y - m) / T (0 where y equals m), and the token's mass is the whole number
+ * rint(exp(t) * 2^40), so that sums of masses do not depend on their order.  Tokens are taken in the order (y
+ * descending, index ascending): the first top_k are kept (top_k <= 0: all), of them the ones whose preceding mass is
+ * below max(1, ceil(top_p * kept mass)) (top_p >= 1: all); the token is the first one in index order whose running
+ * kept mass exceeds min(floor(u * K), K - 1), K the kept mass.  ids (S) int32, logprob (S) float32 or NULL:
+ * t - log(K / 2^40), the log-probability under the distribution drawn from.  T = 0 takes the largest y (lowest index)
+ * with its logprob at T = 1 over all tokens; a negative or NaN T is taken as 0.  A row with no y above -infinity gets id -1 and logprob -infinity.
+ * temperature, top_p, u (S) float32 and top_k (S) int32, per row where the pointer is given, else the value beside
+ * it; u (in [0, 1)) may be NULL only where temperature is NULL and temperature_all is 0.  V at most 2^18. */
+typedef struct {
+  const float* temperature;
+  const int32_t* top_k;
+  const float* top_p;
+  const float* u;
+  float temperature_all, top_p_all;
+  int top_k_all;
+} sdm_choice_params;
+sdm_status sdm_logits_choose(const sdm_logit_rules* rules, const sdm_choice_params* choice, const void* logits,
+                             int64_t ld, int64_t S, int V, int dtype, int32_t* ids, float* logprob, void* stream);
+
+/* ---------------------------------------------------------------------------------------------- distillation loss
+ * Loss of a student's logits (N, V) (dtype, row stride ld) against a teacher's k top logits per row, and optionally
+ * its gradient, in one pass over the logits.  teacher_ids (N, k) int32, teacher_logits (N, k) float32; an entry whose
+ * id is outside [0, V) or whose logit is -infinity is skipped.  T = temperature, q = softmax(logits / T) over V.
+ *   p_i = softmax(teacher_logits / T) over the row's entries, or exp(teacher_logits / T - teacher_lse) where
+ *         teacher_lse (N) float32, the teacher's log-sum-exp at T over its whole vocabulary, is given
+ *   soft = T^2 sum_i p_i (log p_i - log q_i), and with teacher_lse also p_r (log p_r - log q_r), the mass of the
+ *          tokens that are not listed taken as one event: p_r = max(0, 1 - sum p), q_r = sum of their q
+ *   hard = -log softmax(logits)[targets]       (targets (N) int32 or NULL; outside [0, V): the row has no hard term)
+ *   loss = row_weight (alpha soft + (1 - alpha) hard)    (row_weight (N) float32 or NULL = 1)
+ * loss (N) float32.  dlogits (N, V) in dtype, row stride ld_grad, or NULL: grad_scale * d loss / d logits, rounded
+ * once; may be logits itself (same stride), and may not overlap it otherwise.  A row whose weight is 0 is not read:
+ * its loss and gradient are 0.  An id listed twice counts twice in p and once in q.  1 <= k <= 512, V <= 2^18. */
+sdm_status sdm_distill(const void* logits, int64_t ld, int64_t N, int V, int dtype, const int32_t* teacher_ids,
+                       const float* teacher_logits, int k, const float* teacher_lse, const int32_t* targets,
+                       const float* row_weight, float temperature, float alpha, float grad_scale, float* loss,
+                       void* dlogits, int64_t ld_grad, void* stream);
+/* x (N, V) *= g[row] in place (g_stride 1) or *= g[0] (g_stride 0), in dtype, row stride ld: the chain rule's factor
+ * on a gradient that sdm_distill wrote.  A row whose factor is 1 is left alone, unread. */
+sdm_status sdm_scale_rows(void* x, int64_t ld, int64_t N, int V, int dtype, const float* g, int g_stride,
+                          void* stream);
+
+/* ------------------------------------------------------------------------- scaled token lookup and its gradient
+ * sdm_embed_scaled: out (N, d) = scale * emb[ids], rounded once.  An id outside [0, V) gives a zero row and sets *bad
+ * (device int, may be NULL) to 1.
+ * sdm_embed_grad: grad (V, d) = scale * sum of dout's rows over the positions of each id (plus the old grad where
+ * accumulate is 1), dout (N, d) in dtype with row stride ld, grad in grad_dtype; ids outside [0, V) and padding_id
+ * (-1: none) are skipped.  Positions are grouped by id, and each sum runs over them in order (long ones in fixed
+ * pieces joined in order) in float32, so the result does not depend on timing.  N at most 2^30, d
+ * at most 2^20, V at most 2^24. */
+sdm_status sdm_embed_scaled(const int32_t* ids, const void* emb, int64_t N, int d, int V, float scale, int dtype,
+                            void* out, int* bad, void* stream);
+size_t sdm_embed_grad_workspace_size(int64_t N, int d, int V);
+sdm_status sdm_embed_grad(const int32_t* ids, const void* dout, int64_t ld, int64_t N, int d, int V, float scale,
+                          int padding_id, int dtype, int grad_dtype, int accumulate, void* grad, void* workspace,
+                          size_t workspace_bytes, void* stream);
+
 /* Plain GEMM used by the modules above, exposed for tests: y (rows, n) = x (rows, kdim) @ w (n, kdim)^T in
  * float32 accumulation; x, w in dtype, y float32.  In SDM_BF16 mode this runs on the tcgen05 tensor cores. */
 sdm_status sdm_gemm(const void* x, const void* w, int64_t rows, int kdim, int n, int dtype, float* y, void* stream);

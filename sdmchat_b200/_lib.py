@@ -13,7 +13,7 @@ PKG = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(PKG, "libsdm_b200.so")
 
 SDM_F32, SDM_BF16 = 0, 1
-ABI_VERSION = 3
+ABI_VERSION = 4
 
 c_int, c_int64, c_float, c_size_t, c_void_p, c_double = (ctypes.c_int, ctypes.c_int64, ctypes.c_float, ctypes.c_size_t,
                                                           ctypes.c_void_p, ctypes.c_double)
@@ -35,6 +35,21 @@ class TsParams(ctypes.Structure):
                 ("norm_eps", c_float), ("dtype", c_int),
                 ("norm_w", c_void_p), ("wq", c_void_p), ("keys1", c_void_p), ("keys2", c_void_p),
                 ("values", c_void_p), ("log_scale", c_void_p), ("wo", c_void_p)]
+
+
+class LogitRules(ctypes.Structure):
+    """sdm_logit_rules (include/sdm_b200.h)."""
+    _fields_ = [("history", c_void_p), ("history_ld", c_int64), ("history_n", c_int), ("history_len", c_void_p),
+                ("prompt_len", c_void_p), ("repetition", c_void_p), ("frequency", c_void_p), ("presence", c_void_p),
+                ("repetition_all", c_float), ("frequency_all", c_float), ("presence_all", c_float),
+                ("bias_ids", c_void_p), ("bias_values", c_void_p), ("bias_n", c_int), ("mask", c_void_p),
+                ("mask_rows", c_int), ("mask_row", c_void_p)]
+
+
+class ChoiceParams(ctypes.Structure):
+    """sdm_choice_params (include/sdm_b200.h)."""
+    _fields_ = [("temperature", c_void_p), ("top_k", c_void_p), ("top_p", c_void_p), ("u", c_void_p),
+                ("temperature_all", c_float), ("top_p_all", c_float), ("top_k_all", c_int)]
 
 
 P = c_void_p
@@ -76,6 +91,16 @@ _SIGS = {
     "sdm_tied_argmax": (c_int, [P, P, P, c_int64, c_int, c_int, c_float, c_int, P, P, c_size_t, P]),
     "sdm_tied_project": (c_int, [P, P, c_int64, c_int, c_int, c_int, P, P]),
     "sdm_embed": (c_int, [P, P, c_int64, c_int, c_int, c_int, P, P, P]),
+    "sdm_logits_process": (c_int, [ctypes.POINTER(LogitRules), P, c_int64, c_int64, c_int, c_int, P, c_int64, P]),
+    "sdm_logits_choose": (c_int, [ctypes.POINTER(LogitRules), ctypes.POINTER(ChoiceParams), P, c_int64, c_int64, c_int,
+                                  c_int, P, P, P]),
+    "sdm_distill": (c_int, [P, c_int64, c_int64, c_int, c_int, P, P, c_int, P, P, P, c_float, c_float, c_float, P, P,
+                            c_int64, P]),
+    "sdm_scale_rows": (c_int, [P, c_int64, c_int64, c_int, c_int, P, c_int, P]),
+    "sdm_embed_scaled": (c_int, [P, P, c_int64, c_int, c_int, c_float, c_int, P, P, P]),
+    "sdm_embed_grad_workspace_size": (c_size_t, [c_int64, c_int, c_int]),
+    "sdm_embed_grad": (c_int, [P, P, c_int64, c_int64, c_int, c_int, c_float, c_int, c_int, c_int, c_int, P, P,
+                               c_size_t, P]),
     "sdm_gemm": (c_int, [P, P, c_int64, c_int, c_int, c_int, P, P]),
 }
 

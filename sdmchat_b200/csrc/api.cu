@@ -404,7 +404,7 @@ sdm_status head_t(int mode, const void* xv, const void* nf_w, const void* emb, c
 
 extern "C" {
 
-int sdm_abi_version(void) { return 3; }
+int sdm_abi_version(void) { return 4; }
 
 sdm_status sdm_device_status(void* stream) {
   int gemm = 0, scan = 0;
