@@ -46,7 +46,7 @@ sdm_status sdm_logits_process(const sdm_logit_rules* rules, const void* logits, 
   const sdm_logit_rules& r = rules ? *rules : kNoRules;
   const sdm_status s = check_rules(r, rows);
   if (s != SDM_OK) return s;
-  if (ceil_div((int64_t)V + 7, 16384) > 0x7fffffff / (rows > 0 ? rows : 1)) return SDM_ERR_SHAPE;
+  if (ceil_div((int64_t)V + 7, 1024) > 0x7fffffff / (rows > 0 ? rows : 1)) return SDM_ERR_SHAPE;
   return to_status(launch_logits_process(r, logits, ld, rows, V, dtype, out, ld_out, S(stream)));
 }
 

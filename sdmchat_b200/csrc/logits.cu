@@ -97,40 +97,54 @@ __device__ __forceinline__ uint32_t mask_bits(const uint32_t* mask, int v, int V
 }
 
 // ------------------------------------------------------------------------------------------------------- process
-// Block (slice, row): positions [slice * tile, +tile) of the row.
-template <typename T>
-__global__ void __launch_bounds__(256) process_kernel(sdm_logit_rules r, const T* logits, int64_t ld,
-                                                      int V, int tile, int slices, T* out, int64_t ld_out) {
+constexpr int kProcessThreads = 256;
+
+// Block (slice, row): 256 x E x U positions of the row, U chunks per thread.  The loads are issued first, so that they
+// are on their way while the history is marked.
+template <typename T, int U>
+__global__ void __launch_bounds__(kProcessThreads) process_kernel(sdm_logit_rules r, const T* logits, int64_t ld,
+                                                                  int V, int slices, T* out, int64_t ld_out) {
   pdl_enter();
-  constexpr int E = Chunk<T>::E;
-  extern __shared__ uint32_t word[];
+  constexpr int E = Chunk<T>::E, tile = kProcessThreads * E * U;
+  extern __shared__ __align__(16) uint32_t word[];
   const int64_t row = blockIdx.x / slices;
   const int slice = blockIdx.x % slices;
   const T* x = logits + row * ld;
   T* y = out + row * ld_out;
   const int off = row_offset(x);
   const bool aligned_out = row_offset(y) == off;
-  const int p0 = slice * tile;
+  const int64_t p0 = (int64_t)slice * tile;
+  const int v0 = (int)(p0 - off);  // the token of word[0]
+  uint4 raw[U];
+#pragma unroll
+  for (int k = 0; k < U; ++k) {
+    const int64_t v = (int64_t)v0 + (k * kProcessThreads + (int)threadIdx.x) * E;
+    raw[k] = make_uint4(0, 0, 0, 0);
+    if (v >= 0 && v + E <= V) raw[k] = *reinterpret_cast<const uint4*>(x + v);
+  }
   const RowRules q = row_rules(r, row, V);
-  if (q.marks) mark_tokens(r, q, row, p0 - off, tile, V, word);
-  const int p1 = min(p0 + tile, V + off);
-  for (int p = p0 + (int)threadIdx.x * E; p < p1; p += blockDim.x * E) {
-    const int v = p - off;
-    if (v >= 0 && v + E <= V && aligned_out) {
+  if (q.marks) mark_tokens(r, q, row, v0, tile, V, word);
+#pragma unroll
+  for (int k = 0; k < U; ++k) {
+    const int i = (k * kProcessThreads + (int)threadIdx.x) * E;
+    const int64_t v = (int64_t)v0 + i;
+    if (v >= V) break;
+    const bool whole = v >= 0 && v + E <= V;
+    if (whole && aligned_out) {
       float f[E];
-      Chunk<T>::unpack(*reinterpret_cast<const uint4*>(x + v), f);
+      Chunk<T>::unpack(raw[k], f);
       if (q.marks) {
 #pragma unroll
         for (int e = 0; e < E; e += 4) {
-          const uint4 w = *reinterpret_cast<const uint4*>(word + (p - p0) + e);
-          if (w.x) f[e] = ruled(f[e], w.x, q, v + e);
-          if (w.y) f[e + 1] = ruled(f[e + 1], w.y, q, v + e + 1);
-          if (w.z) f[e + 2] = ruled(f[e + 2], w.z, q, v + e + 2);
-          if (w.w) f[e + 3] = ruled(f[e + 3], w.w, q, v + e + 3);
+          const uint4 w = *reinterpret_cast<const uint4*>(word + i + e);
+          if (w.x) f[e] = ruled(f[e], w.x, q, (int)v + e);
+          if (w.y) f[e + 1] = ruled(f[e + 1], w.y, q, (int)v + e + 1);
+          if (w.z) f[e + 2] = ruled(f[e + 2], w.z, q, (int)v + e + 2);
+          if (w.w) f[e + 3] = ruled(f[e + 3], w.w, q, (int)v + e + 3);
         }
       }
       if (q.mask) {
-        const uint32_t b = mask_bits<E>(q.mask, v, V);
+        const uint32_t b = mask_bits<E>(q.mask, (int)v, V);
 #pragma unroll
         for (int e = 0; e < E; ++e)
           if (!((b >> e) & 1)) f[e] = -CUDART_INF_F;
@@ -138,10 +152,10 @@ __global__ void __launch_bounds__(256) process_kernel(sdm_logit_rules r, const T
       *reinterpret_cast<uint4*>(y + v) = Chunk<T>::pack(f);
     } else {
       for (int e = 0; e < E; ++e) {
-        const int u = v + e;
+        const int64_t u = v + e;
         if (u < 0 || u >= V) continue;
         float f = to_f32(x[u]);
-        if (q.marks && word[p - p0 + e]) f = ruled(f, word[p - p0 + e], q, u);
+        if (q.marks && word[i + e]) f = ruled(f, word[i + e], q, (int)u);
         if (q.mask && !((q.mask[u >> 5] >> (u & 31)) & 1)) f = -CUDART_INF_F;
         y[u] = from_f32<T>(f);
       }
@@ -150,7 +164,11 @@ __global__ void __launch_bounds__(256) process_kernel(sdm_logit_rules r, const T
 }
 
 // -------------------------------------------------------------------------------------------------------- choose
-constexpr int kThreads = 512, kWarps = kThreads / 32, kBins = 256;
+constexpr int kThreads = 512, kWarps = kThreads / 32;
+constexpr int kBins = kThreads;    // one per thread when they are scanned
+constexpr int kSplit = 256;        // parts of a key range
+constexpr int kList = 1024;        // candidates that one block ranks
+constexpr int kListK = 256;        // a top_k up to this is found among candidates
 
 // float -> unsigned in the same order (-0 has been made +0, NaN -infinity).
 __device__ __forceinline__ uint32_t order_key(float y) {
@@ -166,115 +184,264 @@ __device__ __forceinline__ float key_value(uint32_t k) {
 __device__ __forceinline__ float scaled_gap(float y, float m, float T) {
   return y == m ? 0.f : __fdiv_rn(__fsub_rn(y, m), T);
 }
-__device__ __forceinline__ u64 mass_of(float y, float m, float T) {
-  return __float2ull_rn(__fmul_rn(expf(scaled_gap(y, m, T)), 1099511627776.f));
-}
+
+// The same mass, many tokens over one T: hi * 2^20 + lo with 0 <= hi <= 2^20 and |lo| <= 2^19, by adding and taking
+// off powers of two whose last place is 1 (no conversions).  The quotient is div_rn_by's, correctly rounded as
+// __fdiv_rn's while T and 1 / T are normal; other temperatures divide.  At 29 T below the largest a mass is 0.
+struct Masses {
+  float m, T, inv, floor_;
+  bool plain;
+  __device__ Masses(float m_, float T_) {
+    m = m_;
+    T = T_;
+    inv = __frcp_rn(T_);
+    floor_ = -29.f * T_;
+    plain = !(T_ > 1e-30f && T_ < 1e30f);
+  }
+  __device__ __forceinline__ void get(float y, uint32_t& hi, int& lo) const {
+    const float x = y == m ? 0.f : __fsub_rn(y, m);
+    float e = 0.f;
+    if (x > floor_ || plain) e = expf(plain ? __fdiv_rn(x, T) : div_rn_by(x, T, inv));
+    const float h = __fmaf_rn(e, 1048576.f, 8388608.f);              // 2^23 + rint(e 2^20)
+    const float r = __fmaf_rn(e, 1048576.f, -__fsub_rn(h, 8388608.f));  // exact, in [-1/2, 1/2]
+    const float l = __fmaf_rn(r, 1048576.f, 12582912.f);             // 2^23 + 2^22 + rint(r 2^20)
+    hi = __float_as_uint(h) - 0x4b000000u;
+    lo = (int)(__float_as_uint(l) - 0x4b400000u);
+  }
+  __device__ __forceinline__ u64 operator()(float y) const {
+    uint32_t hi;
+    int lo;
+    get(y, hi, lo);
+    return ((u64)hi << 20) + (u64)(long long)lo;
+  }
+};
 
 __device__ __forceinline__ u64 warp_sum64(u64 v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
-
-struct ChooseShared {
-  u64 best[kMaxCluster], total[kMaxCluster];
-  uint32_t ties[kMaxCluster];
-  uint32_t lo[2][kMaxCluster], hi[2][kMaxCluster];
-  u64 mass[2][kBins];        // this block's histogram, two buffers in turn
-  uint32_t count[2][kBins];
-  u64 mass_before[kBins + 1];       // over the cluster: of the bins above each bin
-  uint32_t count_before[kBins + 1];
-  u64 first_mass[kBins + 1];        // the first histogram's, kept for the second search
-  uint32_t first_count[kBins + 1];
-  u64 warp64[kWarps];
-  uint32_t warp32[kWarps];
-  int bin;
-  uint32_t klo, khi;
-};
+__device__ __forceinline__ u64 warp_scan64(u64 v, int lane) {
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const u64 up = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += up;
+  }
+  return v;
+}
 
 // kept: key > cut, and of the tokens with key == cut the first `ties` in index order
 struct Cut {
   uint32_t key;
-  uint32_t ties, tie_count;  // kept and all tokens of that key (tie_count 0: key is below every kept token)
-  u64 mass;                  // all kept tokens'
+  uint32_t ties, tie_count;  // kept and all tokens of that key (tie_count 0: no token has it)
+  u64 mass;                  // the kept tokens' (of a search by mass, or where masses were counted)
 };
 
-// Sums this block's histogram `buf` over the cluster, and writes its sums over the bins before each bin.
-template <typename Cluster>
-__device__ void join_bins(Cluster& cluster, ChooseShared& s, int buf, u64* mass_before, uint32_t* count_before) {
+struct ChooseShared {
+  u64 best[kMaxCluster], total[kMaxCluster];
+  float low[kMaxCluster];
+  uint32_t ties[kMaxCluster], listed[kMaxCluster];
+  union {
+    // this block's histogram: tokens, and masses in three limbs of 14 bits (a slice's 2^15 tokens cannot overflow one)
+    struct {
+      uint32_t count[kBins], limb[3][kBins];
+    };
+    u64 sorted[kList];              // block 0's list in order, once the histogram is done with
+  };
+  u64 mass_before[kBins + 1];       // over the cluster: of the bins above each bin
+  uint32_t count_before[kBins + 1];
+  u64 split_mass[kSplit + 1];       // the same of a split key range
+  uint32_t split_count[kSplit + 1];
+  u64 warp64[kWarps];
+  uint32_t warp32[kWarps];
+  uint32_t list_n;
+  int bin;
+  uint32_t klo, khi;
+  uint32_t lo[2][kMaxCluster], hi[2][kMaxCluster];
+  Cut cut;
+  u64 list[kList];                  // candidates: key << 32 | ~token
+};
+
+template <int N>
+__device__ __forceinline__ void clear_bins(ChooseShared& s) {
+  for (int b = threadIdx.x; b < N; b += kThreads) s.count[b] = s.limb[0][b] = s.limb[1][b] = s.limb[2][b] = 0;
+}
+__device__ __forceinline__ void add_mass(ChooseShared& s, int b, u64 w) {
+  const uint32_t w0 = (uint32_t)w & 0x3fffu, w1 = (uint32_t)(w >> 14) & 0x3fffu, w2 = (uint32_t)(w >> 28);
+  if (w0) atomicAdd(&s.limb[0][b], w0);
+  if (w1) atomicAdd(&s.limb[1][b], w1);
+  if (w2) atomicAdd(&s.limb[2][b], w2);
+}
+
+// Sums the blocks' histograms over the cluster, and writes the sums over the bins before each bin.
+template <int N, typename Cluster>
+__device__ void join_bins(Cluster& cluster, ChooseShared& s, bool masses, u64* mass_before, uint32_t* count_before) {
   cluster.sync();
   const int b = threadIdx.x, lane = b & 31, warp = b >> 5;
-  u64 m = 0;
-  uint32_t c = 0;
-  if (b < kBins) {
+  u64 m = 0, im = 0;
+  uint32_t c = 0, ic = 0;
+  if (b < N) {
     for (unsigned r = 0; r < cluster.num_blocks(); ++r) {
-      m += *cluster.map_shared_rank(&s.mass[buf][b], r);
-      c += *cluster.map_shared_rank(&s.count[buf][b], r);
+      c += *cluster.map_shared_rank(&s.count[b], r);
+      if (masses)
+        m += (u64)*cluster.map_shared_rank(&s.limb[0][b], r) + ((u64)*cluster.map_shared_rank(&s.limb[1][b], r) << 14) +
+             ((u64)*cluster.map_shared_rank(&s.limb[2][b], r) << 28);
     }
-    u64 im = m;
-    uint32_t ic = c;
+    ic = c;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const u64 um = __shfl_up_sync(0xffffffffu, im, o);
-      const uint32_t uc = __shfl_up_sync(0xffffffffu, ic, o);
-      if (lane >= o) {
-        im += um;
-        ic += uc;
-      }
+      const uint32_t up = __shfl_up_sync(0xffffffffu, ic, o);
+      if (lane >= o) ic += up;
     }
+    im = warp_scan64(m, lane);
     if (lane == 31) {
       s.warp64[warp] = im;
       s.warp32[warp] = ic;
     }
-    m = im - m;
-    c = ic - c;
   }
   __syncthreads();
-  if (b < kBins) {
+  if (b < N) {
     for (int w = 0; w < warp; ++w) {
-      m += s.warp64[w];
-      c += s.warp32[w];
+      im += s.warp64[w];
+      ic += s.warp32[w];
     }
-    mass_before[b] = m;
-    count_before[b] = c;
-    if (b == kBins - 1) {
-      u64 tm = 0;
-      uint32_t tc = 0;
-      for (int w = 0; w < kBins / 32; ++w) {
-        tm += s.warp64[w];
-        tc += s.warp32[w];
-      }
-      mass_before[kBins] = tm;
-      count_before[kBins] = tc;
+    if (b == 0) {
+      mass_before[0] = 0;
+      count_before[0] = 0;
     }
+    mass_before[b + 1] = im;
+    count_before[b + 1] = ic;
   }
   __syncthreads();
 }
 
-// The bin in which the running count (by_count) or mass reaches `target`.
+// The first of N bins through which the running count (by_count) or mass reaches `target`; N - 1 if none does.
+template <int N>
 __device__ __forceinline__ int find_bin(ChooseShared& s, const u64* mass_before, const uint32_t* count_before,
                                         bool by_count, u64 target) {
   const int b = threadIdx.x;
-  if (b < kBins) {
+  if (b == 0) s.bin = N - 1;
+  __syncthreads();
+  if (b < N) {
     const u64 before = by_count ? (u64)count_before[b] : mass_before[b];
     const u64 through = by_count ? (u64)count_before[b + 1] : mass_before[b + 1];
     if (before < target && target <= through) s.bin = b;
   }
   __syncthreads();
-  const int bin = s.bin;
-  __syncthreads();
-  return bin;
+  return s.bin;
 }
 
-// Where a row's running count or mass, largest logit first, reaches `target` (1 <= target <= the row's whole).  The
-// first histogram is linear in m - y; below it the bin's key range is split in 256 until one key, or one token, is
-// left: masses are exact whole numbers, so every step is.
+// Bin of a logit: linear in its distance from the largest, so that bins hold comparable numbers of tokens.
+__device__ __forceinline__ int gap_bin(float v, float m, float scale) {
+  return v == m ? 0 : min(kBins - 1, (int)((m - v) * scale));
+}
+
+// Lists this block's tokens of bins first .. last above -infinity, and tells the cluster how many they are.  Returns
+// the cluster's number (lists are cut at kList).
 template <typename Cluster>
-__device__ Cut search(Cluster& cluster, ChooseShared& s, const float* y, int lo, int hi, float m, float T, float inv,
-                      bool by_count, u64 target, int which, int& buf) {
-  const int B = find_bin(s, s.first_mass, s.first_count, by_count, target);
-  u64 above_mass = s.first_mass[B], in_mass = s.first_mass[B + 1] - above_mass;
-  uint32_t above = s.first_count[B], in = s.first_count[B + 1] - above;
+__device__ uint32_t list_bins(Cluster& cluster, ChooseShared& s, const float* y, int lo, int hi, int v0, float m,
+                              float scale, int first, int last) {
+  if (threadIdx.x == 0) s.list_n = 0;
+  __syncthreads();
+  for (int i = lo + threadIdx.x; i < hi; i += kThreads) {
+    const float v = y[i];
+    const int b = gap_bin(v, m, scale);
+    if (b >= first && b <= last && v > -CUDART_INF_F) {
+      const uint32_t at = atomicAdd(&s.list_n, 1u);
+      if (at < kList) s.list[at] = (u64)order_key(v) << 32 | (0xffffffffu - (uint32_t)(v0 + i));
+    }
+  }
+  __syncthreads();
+  if (threadIdx.x < cluster.num_blocks()) *cluster.map_shared_rank(&s.listed[cluster.block_rank()], threadIdx.x) = s.list_n;
+  cluster.sync();
+  uint32_t n = 0;
+  for (unsigned r = 0; r < cluster.num_blocks(); ++r) n += s.listed[r];
+  return n;
+}
+
+// Block 0: brings the cluster's lists (n tokens, n <= kList) together in s.sorted, largest first.  All keys differ,
+// so the order does not depend on how the lists were filled.
+template <typename Cluster>
+__device__ void sort_lists(Cluster& cluster, ChooseShared& s, uint32_t n) {
+  uint32_t at = s.listed[0];
+  for (unsigned r = 1; r < cluster.num_blocks(); ++r) {
+    const uint32_t k = s.listed[r];
+    const u64* from = cluster.map_shared_rank(&s.list[0], r);
+    for (uint32_t i = threadIdx.x; i < k; i += kThreads) s.list[at + i] = from[i];
+    at += k;
+  }
+  __syncthreads();
+  for (uint32_t i = threadIdx.x; i < n; i += kThreads) {
+    const u64 mine = s.list[i];
+    uint32_t rank = 0;
+#pragma unroll 4
+    for (uint32_t j = 0; j < n; ++j) rank += s.list[j] > mine;
+    s.sorted[rank] = mine;
+  }
+  __syncthreads();
+}
+
+// Masses of the block's two tokens sorted[2 tid], sorted[2 tid + 1] (0 from `n` on): their sum over all tokens before
+// is returned, `all` is the sum over all.
+__device__ u64 scan_sorted(ChooseShared& s, const Masses& M, uint32_t n, u64& w0, u64& w1, u64& all) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const uint32_t i = 2 * threadIdx.x;
+  w0 = i < n ? M(key_value((uint32_t)(s.sorted[i] >> 32))) : 0;
+  w1 = i + 1 < n ? M(key_value((uint32_t)(s.sorted[i + 1] >> 32))) : 0;
+  const u64 run = warp_scan64(w0 + w1, lane);
+  if (lane == 31) s.warp64[warp] = run;
+  __syncthreads();
+  u64 before = run - w0 - w1;
+  all = 0;
+  for (int w = 0; w < kWarps; ++w) {
+    if (w < warp) before += s.warp64[w];
+    all += s.warp64[w];
+  }
+  __syncthreads();
+  return before;
+}
+
+// Where a row's running count or mass, largest logit first, reaches `target` (1 <= target <= the row's whole), from
+// the joined histogram: the bin's tokens are listed and ranked by one block.  A bin of more than kList tokens (ties, or
+// a row that is almost level) has its key range split in kSplit until one key is left.
+template <typename Cluster>
+__device__ Cut search(Cluster& cluster, ChooseShared& s, const float* y, int lo, int hi, int v0, const Masses& M,
+                      float scale, bool by_count, bool masses, u64 target, int which) {
+  const int B = find_bin<kBins>(s, s.mass_before, s.count_before, by_count, target);
+  u64 above_mass = s.mass_before[B];
+  uint32_t above = s.count_before[B];
+  const uint32_t n = list_bins(cluster, s, y, lo, hi, v0, M.m, scale, B, B);
+  // -infinity is not listed: where the count runs into it, all that is listed is kept
+  const bool short_ = by_count && target - above > n;
+  if (short_) {
+    cluster.sync();  // s.listed is read before it is written again
+    return {order_key(-CUDART_INF_F), 0, 0, masses ? s.mass_before[kBins] : 0};
+  }
+  if (n <= kList) {
+    if (cluster.block_rank() == 0) {
+      sort_lists(cluster, s, n);
+      u64 w0, w1, all;
+      u64 before = above_mass + scan_sorted(s, M, masses ? n : 0, w0, w1, all);
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const uint32_t i = 2 * threadIdx.x + e;
+        const u64 w = e ? w1 : w0;
+        const bool here = i < n && (by_count ? above + i + 1 == target : before < target && target - before <= w);
+        if (here) {
+          const uint32_t key = (uint32_t)(s.sorted[i] >> 32);
+          uint32_t first = i, end = i + 1;
+          while (first > 0 && (uint32_t)(s.sorted[first - 1] >> 32) == key) --first;
+          while (end < n && (uint32_t)(s.sorted[end] >> 32) == key) ++end;
+          s.cut = {key, i + 1 - first, end - first, before + w};
+        }
+        before += w;
+      }
+      __syncthreads();
+      if (threadIdx.x > 0 && threadIdx.x < cluster.num_blocks()) *cluster.map_shared_rank(&s.cut, threadIdx.x) = s.cut;
+    }
+    cluster.sync();
+    return s.cut;
+  }
   // the bin's range of keys
   if (threadIdx.x == 0) {
     s.klo = 0xffffffffu;
@@ -284,8 +451,7 @@ __device__ Cut search(Cluster& cluster, ChooseShared& s, const float* y, int lo,
   uint32_t kl = 0xffffffffu, kh = 0;
   for (int i = lo + threadIdx.x; i < hi; i += kThreads) {
     const float v = y[i];
-    const int b = v == m ? 0 : min(kBins - 1, (int)((m - v) * inv));
-    if (b == B) {
+    if (gap_bin(v, M.m, scale) == B) {
       const uint32_t k = order_key(v);
       kl = min(kl, k);
       kh = max(kh, k);
@@ -309,50 +475,51 @@ __device__ Cut search(Cluster& cluster, ChooseShared& s, const float* y, int lo,
     kl = min(kl, s.lo[which][r]);
     kh = max(kh, s.hi[which][r]);
   }
-  // keys kl .. kh hold `in` tokens of in_mass; `above` tokens of above_mass are larger
-  for (int step = 0; step < 6; ++step) {  // 32-bit keys are down to one after four
-    if (by_count ? target - above == in : in == 1) return {kl - 1, 0, 0, above_mass + in_mass};
-    if (kl == kh) {
-      const u64 w = mass_of(key_value(kl), m, T);
-      const uint32_t ties = by_count ? (uint32_t)(target - above) : (uint32_t)((target - above_mass + w - 1) / w);
-      return {kl, ties, in, above_mass + ties * w};
-    }
+  uint32_t in = n;
+  for (int step = 0; step < 5 && kl != kh; ++step) {  // 32-bit keys are down to one after four
     const int shift = max(0, 24 - __clz(kh - kl));
-    for (int b = threadIdx.x; b < kBins; b += kThreads) {
-      s.mass[buf][b] = 0;
-      s.count[buf][b] = 0;
-    }
+    cluster.sync();  // the histogram's last readers are done
+    clear_bins<kSplit>(s);
     __syncthreads();
     for (int i = lo + threadIdx.x; i < hi; i += kThreads) {
       const float v = y[i];
       const uint32_t k = order_key(v);
       if (k >= kl && k <= kh) {
         const int b = (kh - k) >> shift;
-        atomicAdd(&s.count[buf][b], 1u);
-        atomicAdd(&s.mass[buf][b], mass_of(v, m, T));
+        atomicAdd(&s.count[b], 1u);
+        if (masses) add_mass(s, b, M(v));
       }
     }
-    join_bins(cluster, s, buf, s.mass_before, s.count_before);
-    buf ^= 1;
-    const int b = find_bin(s, s.mass_before, s.count_before, by_count, by_count ? target - above : target - above_mass);
-    in = s.count_before[b + 1] - s.count_before[b];
-    in_mass = s.mass_before[b + 1] - s.mass_before[b];
-    above += s.count_before[b];
-    above_mass += s.mass_before[b];
+    join_bins<kSplit>(cluster, s, masses, s.split_mass, s.split_count);
+    const int b = find_bin<kSplit>(s, s.split_mass, s.split_count, by_count, by_count ? target - above : target - above_mass);
+    in = s.split_count[b + 1] - s.split_count[b];
+    above += s.split_count[b];
+    above_mass += s.split_mass[b];
     kh -= (uint32_t)b << shift;
     kl = max(kl, kh - min(kh, (1u << shift) - 1));
     __syncthreads();
   }
-  return {kl - 1, 0, 0, above_mass + in_mass};
+  const u64 w = M(key_value(kl));
+  const uint32_t ties = by_count ? (uint32_t)(target - above) : (uint32_t)((target - above_mass + w - 1) / max(w, (u64)1));
+  return {kl, ties, in, above_mass + ties * w};
 }
+
+__device__ __forceinline__ u64 draw_target(float u, u64 K) {
+  const double t = floor((double)u * (double)K);
+  return min(t > 0.0 ? (u64)t : (u64)0, K - 1);  // NaN and negative: 0
+}
+__device__ __forceinline__ u64 share_of(float top_p, u64 W) {
+  return top_p > 0.f ? max((u64)ceil((double)top_p * (double)W), (u64)1) : (u64)1;
+}
+__device__ __forceinline__ float log_mass(u64 K) { return logf((float)K * 9.094947017729282e-13f); }  // K / 2^40
 
 // A cluster of blocks per row, each with a slice of the row's processed logits in shared memory.
 template <typename T>
-__global__ void __launch_bounds__(kThreads) choose_kernel(sdm_logit_rules r, sdm_choice_params c,
+__global__ void __launch_bounds__(kThreads, 2) choose_kernel(sdm_logit_rules r, sdm_choice_params c,
                                                           const T* __restrict__ logits, int64_t ld, int V, int slice,
                                                           int32_t* __restrict__ ids, float* __restrict__ logprob) {
   pdl_enter();
-  constexpr int E = Chunk<T>::E;
+  constexpr int E = Chunk<T>::E, U = 4;
   extern __shared__ __align__(16) uint32_t word[];  // slice words: the marks, then in their place the logits
   __shared__ ChooseShared s;
   float* y = reinterpret_cast<float*>(word);
@@ -363,60 +530,116 @@ __global__ void __launch_bounds__(kThreads) choose_kernel(sdm_logit_rules r, sdm
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const T* x = logits + row * ld;
   const int off = row_offset(x);
-  const int p0 = (int)rank * slice;
+  const int p0 = (int)rank * slice, v0 = p0 - off;  // v0: the token of y[0]
+  const int lo = max(0, -v0), hi = max(lo, min(slice, V - v0));  // this block's tokens: v0 + [lo, hi)
+
+  // the first loads are on their way while the marks are made
+  uint4 raw[U];
+  auto load = [&](int i) {
+    uint4 q = make_uint4(0, 0, 0, 0);
+    if (i >= lo && i + E <= hi) q = *reinterpret_cast<const uint4*>(x + v0 + i);
+    return q;
+  };
+#pragma unroll
+  for (int k = 0; k < U; ++k) raw[k] = load((k * kThreads + tid) * E);
+
   const RowRules q = row_rules(r, row, V);
   const float T0 = c.temperature ? c.temperature[row] : c.temperature_all;
   const bool greedy = !(T0 > 0.f);
   const float Tr = greedy ? 1.f : T0;
   const int top_k = c.top_k ? c.top_k[row] : c.top_k_all;
   const float top_p = c.top_p ? c.top_p[row] : c.top_p_all;
-  const int lo = max(0, off - p0), hi = max(lo, min(slice, V + off - p0));  // this block's tokens: p0 - off + [lo, hi)
-
-  if (q.marks) mark_tokens(r, q, row, p0 - off, slice, V, word);
+  const float u = c.u ? c.u[row] : 0.f;
+  if (q.marks) mark_tokens(r, q, row, v0, slice, V, word);
   u64 best = 0;
-  for (int i = tid * E; i < hi; i += kThreads * E) {
-    const int v = p0 + i - off;
-    float f[E];
-    const bool whole = v >= 0 && v + E <= V;
-    if (whole) {
-      Chunk<T>::unpack(*reinterpret_cast<const uint4*>(x + v), f);
-    } else {
+  for (int i0 = 0; i0 < hi; i0 += U * kThreads * E) {
+    if (i0 > 0) {
 #pragma unroll
-      for (int e = 0; e < E; ++e) f[e] = v + e >= 0 && v + e < V ? to_f32(x[v + e]) : -CUDART_INF_F;
+      for (int k = 0; k < U; ++k) raw[k] = load(i0 + (k * kThreads + tid) * E);
     }
-    uint32_t bits = 0xffffffffu;
-    if (q.mask) {
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      const int i = i0 + (k * kThreads + tid) * E, v = v0 + i;
+      if (i >= hi) break;
+      float f[E];
+      const bool whole = i >= lo && i + E <= hi;
       if (whole) {
-        bits = mask_bits<E>(q.mask, v, V);
+        Chunk<T>::unpack(raw[k], f);
       } else {
 #pragma unroll
-        for (int e = 0; e < E; ++e)
-          if (v + e >= 0 && v + e < V && !((q.mask[(v + e) >> 5] >> ((v + e) & 31)) & 1)) bits &= ~(1u << e);
+        for (int e = 0; e < E; ++e) f[e] = i + e >= lo && i + e < hi ? to_f32(x[v + e]) : -CUDART_INF_F;
+      }
+      uint32_t bits = 0xffffffffu;
+      if (q.mask) {
+        if (whole) {
+          bits = mask_bits<E>(q.mask, v, V);
+        } else {
+#pragma unroll
+          for (int e = 0; e < E; ++e)
+            if (i + e >= lo && i + e < hi && !((q.mask[(v + e) >> 5] >> ((v + e) & 31)) & 1)) bits &= ~(1u << e);
+        }
+      }
+      float top = -CUDART_INF_F;
+      if (q.marks) {
+#pragma unroll
+        for (int e = 0; e < E; e += 4) {
+          const uint4 w = *reinterpret_cast<const uint4*>(word + i + e);
+          if (w.x) f[e] = ruled(f[e], w.x, q, v + e);
+          if (w.y) f[e + 1] = ruled(f[e + 1], w.y, q, v + e + 1);
+          if (w.z) f[e + 2] = ruled(f[e + 2], w.z, q, v + e + 2);
+          if (w.w) f[e + 3] = ruled(f[e + 3], w.w, q, v + e + 3);
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        if (!((bits >> e) & 1)) f[e] = -CUDART_INF_F;
+        f[e] = __fadd_rn(fmaxf(f[e], -CUDART_INF_F), 0.f);  // NaN is -infinity; -0 and +0 are one value in the order
+        top = fmaxf(top, f[e]);
+      }
+#pragma unroll
+      for (int e = 0; e < E; e += 4)
+        *reinterpret_cast<float4*>(y + i + e) = make_float4(f[e], f[e + 1], f[e + 2], f[e + 3]);
+      const uint32_t tk = order_key(top);
+      if (tk > (uint32_t)(best >> 32)) {  // this thread's tokens come in index order: the first largest stays
+        int at = E - 1;
+#pragma unroll
+        for (int e = E - 1; e >= 0; --e)
+          if (f[e] == top) at = e;
+        at = max(at, lo - i);  // all -infinity: any of the row's own
+        best = (u64)tk << 32 | (0xffffffffu - (uint32_t)(v + at));
       }
     }
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      if (q.marks && word[i + e]) f[e] = ruled(f[e], word[i + e], q, v + e);
-      if (!((bits >> e) & 1) || isnan(f[e])) f[e] = -CUDART_INF_F;
-      f[e] = __fadd_rn(f[e], 0.f);  // -0 and +0 are one value in the order
-      if (v + e >= 0 && v + e < V) best = max(best, (u64)order_key(f[e]) << 32 | (0xffffffffu - (uint32_t)(v + e)));
-    }
-#pragma unroll
-    for (int e = 0; e < E; e += 4) *reinterpret_cast<float4*>(y + i + e) = make_float4(f[e], f[e + 1], f[e + 2], f[e + 3]);
   }
+  const float group_top = best ? key_value((uint32_t)(best >> 32)) : -CUDART_INF_F;
+  float low = group_top > -CUDART_INF_F ? group_top : CUDART_INF_F;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
-  if (lane == 0) s.warp64[warp] = best;
+  for (int o = 16; o > 0; o >>= 1) {
+    best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
+    low = fminf(low, __shfl_xor_sync(0xffffffffu, low, o));
+  }
+  if (lane == 0) {
+    s.warp64[warp] = best;
+    s.warp32[warp] = __float_as_uint(low);
+  }
   __syncthreads();
   cluster.barrier_wait(std::move(started));
   if (tid < (int)C) {
     u64 b = 0;
-    for (int w = 0; w < kWarps; ++w) b = max(b, s.warp64[w]);
+    float l = CUDART_INF_F;
+    for (int w = 0; w < kWarps; ++w) {
+      b = max(b, s.warp64[w]);
+      l = fminf(l, __uint_as_float(s.warp32[w]));
+    }
     *cluster.map_shared_rank(&s.best[rank], tid) = b;
+    *cluster.map_shared_rank(&s.low[rank], tid) = l;
   }
   cluster.sync();
   best = 0;
-  for (unsigned k = 0; k < C; ++k) best = max(best, s.best[k]);
+  low = CUDART_INF_F;
+  for (unsigned k = 0; k < C; ++k) {
+    best = max(best, s.best[k]);
+    low = fminf(low, s.low[k]);
+  }
   const float m = key_value((uint32_t)(best >> 32));
   if (m == -CUDART_INF_F) {  // nothing is allowed: the same in every block of the cluster
     if (rank == 0 && tid == 0) {
@@ -425,50 +648,95 @@ __global__ void __launch_bounds__(kThreads) choose_kernel(sdm_logit_rules r, sdm
     }
     return;
   }
+  const Masses M(m, Tr);
+  const bool by_k = !greedy && top_k > 0 && top_k < V, by_p = !greedy && top_p < 1.f;
+
+  // A small top_k.  A thread's largest logits are as many tokens of the row, so the top_k-th largest of them is at or
+  // below the row's: tokens above it (a few more than top_k) are listed, and one block does the rest on the list.
+  if (by_k && top_k <= kListK) {
+    const float scale = (float)(kBins - 1) / (m - low);
+    clear_bins<kBins>(s);
+    __syncthreads();
+    if (group_top > -CUDART_INF_F) atomicAdd(&s.count[gap_bin(group_top, m, scale)], 1u);
+    join_bins<kBins>(cluster, s, false, s.mass_before, s.count_before);
+    const int last = find_bin<kBins>(s, s.mass_before, s.count_before, true, (u64)top_k);
+    const uint32_t n = list_bins(cluster, s, y, lo, hi, v0, m, scale, 0, last);
+    if (n <= kList) {
+      if (rank == 0) {
+        sort_lists(cluster, s, n);
+        const uint32_t kept = min(n, (uint32_t)top_k);
+        u64 w[2], W, K;
+        u64 before = scan_sorted(s, M, kept, w[0], w[1], W);
+        const u64 share = by_p ? share_of(top_p, W) : W;
+        uint32_t mine = 0;  // kept ones of this thread's two
+        if (2 * tid < kept && before < share) mine = 2 * tid + 1 < kept && before + w[0] < share ? 2 : 1;
+        const uint32_t stay = __syncthreads_count(mine >= 1) + __syncthreads_count(mine == 2);
+        scan_sorted(s, M, stay, w[0], w[1], K);
+        const u64 target = draw_target(u, K);
+        u64* mass = s.list;  // the kept tokens' masses, by rank
+        if (2 * tid < kList) {
+          mass[2 * tid] = w[0];
+          mass[2 * tid + 1] = w[1];
+        }
+        __syncthreads();
+        for (uint32_t i = tid; i < stay; i += kThreads) {  // the mass of the kept tokens of lower index
+          const uint32_t token = 0xffffffffu - (uint32_t)s.sorted[i];
+          u64 run = 0;
+          for (uint32_t j = 0; j < stay; ++j)
+            if (0xffffffffu - (uint32_t)s.sorted[j] < token) run += mass[j];
+          if (run <= target && target - run < mass[i]) {
+            ids[row] = (int32_t)token;
+            if (logprob) logprob[row] = scaled_gap(key_value((uint32_t)(s.sorted[i] >> 32)), m, Tr) - log_mass(K);
+          }
+        }
+      }
+      cluster.sync();  // the lists were read by block 0
+      return;
+    }
+    cluster.sync();  // the histogram is made anew
+  }
 
   // what is kept
   Cut cut = {0, 0, 0, 0};  // all: every key is above 0
-  const bool by_k = !greedy && top_k > 0 && top_k < V, by_p = !greedy && top_p < 1.f;
   if (by_k || by_p) {
-    const float inv = (float)kBins / (28.1f * Tr);  // beyond exp(-28.1) a mass is 0
-    for (int b = tid; b < kBins; b += kThreads) {
-      s.mass[0][b] = 0;
-      s.count[0][b] = 0;
-    }
+    const float scale = (float)kBins / (28.5f * Tr);  // beyond exp(-28.5) a mass is 0
+    clear_bins<kBins>(s);
     __syncthreads();
     for (int i = lo + tid; i < hi; i += kThreads) {
       const float v = y[i];
-      const int b = v == m ? 0 : min(kBins - 1, (int)((m - v) * inv));
-      atomicAdd(&s.count[0][b], 1u);
-      const u64 w = mass_of(v, m, Tr);
-      if (w) atomicAdd(&s.mass[0][b], w);
+      const int b = gap_bin(v, m, scale);
+      if (by_k) atomicAdd(&s.count[b], 1u);
+      if (by_p) add_mass(s, b, M(v));
     }
-    join_bins(cluster, s, 0, s.first_mass, s.first_count);
-    int buf = 1;
-    u64 kept = s.first_mass[kBins];
+    join_bins<kBins>(cluster, s, by_p, s.mass_before, s.count_before);
+    u64 kept = s.mass_before[kBins];
     if (by_k) {
-      cut = search(cluster, s, y, lo, hi, m, Tr, inv, true, (u64)top_k, 0, buf);
+      cut = search(cluster, s, y, lo, hi, v0, M, scale, true, by_p, (u64)top_k, 0);
       kept = cut.mass;
     }
-    if (by_p) {
-      const u64 share = (u64)ceil((double)top_p * (double)kept);  // a negative or NaN top_p keeps one token
-      cut = search(cluster, s, y, lo, hi, m, Tr, inv, false, top_p > 0.f ? max(share, (u64)1) : (u64)1, 1, buf);
-    }
+    if (by_p) cut = search(cluster, s, y, lo, hi, v0, M, scale, false, true, share_of(top_p, kept), 1);
   }
 
   // each warp's kept mass over its own stretch of the slice
   const int seg = slice / kWarps, s0 = max(lo, warp * seg), s1 = min(hi, (warp + 1) * seg);
   const bool partial = cut.ties < cut.tie_count;
-  const u64 tie_mass = cut.tie_count ? mass_of(key_value(cut.key), m, Tr) : 0;
-  u64 sum = 0;
-  uint32_t tied = 0;
+  const u64 tie_mass = cut.tie_count ? M(key_value(cut.key)) : 0;
+  uint32_t sum_hi = 0, tied = 0;
+  int sum_lo = 0;
   for (int i = s0 + lane; i < s1; i += 32) {
     const float v = y[i];
     const uint32_t k = order_key(v);
-    if (k > cut.key) sum += mass_of(v, m, Tr);
-    else if (k == cut.key) ++tied;
+    if (k > cut.key) {
+      uint32_t h;
+      int l;
+      M.get(v, h, l);
+      sum_hi += h;
+      sum_lo += l;
+    } else if (k == cut.key) {
+      ++tied;
+    }
   }
-  sum = warp_sum64(sum);
+  u64 sum = warp_sum64(((u64)sum_hi << 20) + (u64)(long long)sum_lo);
   tied = __reduce_add_sync(0xffffffffu, tied);
   uint32_t tie_before = 0;
   if (partial) {  // ties are kept from the lowest index on: count the ones before this warp
@@ -498,7 +766,7 @@ __global__ void __launch_bounds__(kThreads) choose_kernel(sdm_logit_rules r, sdm
     if (k < rank) before += s.total[k];
     K += s.total[k];
   }
-  const float log_k = logf((float)K * 9.094947017729282e-13f);  // K / 2^40
+  const float log_k = log_mass(K);
   if (greedy) {
     if (rank == 0 && tid == 0) {
       ids[row] = (int32_t)(0xffffffffu - (uint32_t)best);
@@ -506,10 +774,7 @@ __global__ void __launch_bounds__(kThreads) choose_kernel(sdm_logit_rules r, sdm
     }
     return;
   }
-  const float u = c.u ? c.u[row] : 0.f;
-  const double ur = floor((double)u * (double)K);
-  u64 target = ur > 0.0 ? (u64)ur : 0;  // NaN and negative: 0
-  target = min(target, K - 1);
+  const u64 target = draw_target(u, K);
   for (int w = 0; w < warp; ++w) before += s.warp64[w];
   if (target < before || target - before >= sum) return;  // another warp's
   u64 left = target - before;  // the first token whose running mass in this stretch exceeds `left`
@@ -524,19 +789,14 @@ __global__ void __launch_bounds__(kThreads) choose_kernel(sdm_logit_rules r, sdm
     const bool tie = i < s1 && cut.tie_count && k == cut.key;
     const uint32_t tie_lanes = __ballot_sync(0xffffffffu, tie);
     u64 w = 0;
-    if (i < s1 && k > cut.key) w = mass_of(v, m, Tr);
+    if (i < s1 && k > cut.key) w = M(v);
     if (tie && (!partial || tie_before + __popc(tie_lanes & ((1u << lane) - 1)) < cut.ties)) w = tie_mass;
     tie_before += __popc(tie_lanes);
-    u64 run = w;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const u64 up = __shfl_up_sync(0xffffffffu, run, o);
-      if (lane >= o) run += up;
-    }
+    const u64 run = warp_scan64(w, lane);
     const uint32_t over = __ballot_sync(0xffffffffu, run > left);
     if (over) {
       if (lane == __ffs(over) - 1) {
-        ids[row] = p0 + i - off;
+        ids[row] = v0 + i;
         if (logprob) logprob[row] = scaled_gap(v, m, Tr) - log_k;
       }
       return;
@@ -545,20 +805,26 @@ __global__ void __launch_bounds__(kThreads) choose_kernel(sdm_logit_rules r, sdm
   }
 }
 
+template <typename T, int U>
+cudaError_t process_u(const sdm_logit_rules& r, const T* x, int64_t ld, int64_t S, int V, T* out, int64_t ld_out,
+                      cudaStream_t st) {
+  constexpr int E = Chunk<T>::E, tile = kProcessThreads * E * U;
+  const int64_t slices = ceil_div((int64_t)V + E - 1, tile);
+  if (slices * S > 0x7fffffff) return cudaErrorInvalidValue;
+  const bool marks = (r.history && r.history_n > 0) || (r.bias_ids && r.bias_n > 0);
+  LaunchScope scope_("logits_process", st);
+  return launch_k(process_kernel<T, U>, dim3((unsigned)(slices * S)), dim3(kProcessThreads),
+                  marks ? (size_t)tile * 4 : 0, st, r, x, ld, V, (int)slices, out, ld_out);
+}
+
 template <typename T>
 cudaError_t process_t(const sdm_logit_rules& r, const T* x, int64_t ld, int64_t S, int V, T* out, int64_t ld_out,
                       cudaStream_t st) {
-  // the largest slice (so that a row's history is read by few blocks) that still gives every SM two blocks
-  int tile = 16384;
-  while (tile > 1024 && ceil_div((int64_t)V + 7, tile) * S < 2 * kSMs) tile /= 2;
-  const int64_t slices = ceil_div((int64_t)V + 7, tile);
-  if (slices * S > 0x7fffffff) return cudaErrorInvalidValue;
-  const size_t smem = (size_t)tile * 4;
-  cudaError_t e = cudaFuncSetAttribute(process_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, 16384 * 4);
-  if (e != cudaSuccess) return e;
-  LaunchScope scope_("logits_process", st);
-  return launch_k(process_kernel<T>, dim3((unsigned)(slices * S)), dim3(256), smem, st, r, x, ld, V, tile, (int)slices,
-                  out, ld_out);
+  // four chunks per thread (few blocks read a row's history, many bytes are in flight) where that fills the SMs twice
+  constexpr int E = Chunk<T>::E;
+  if (S * ceil_div((int64_t)V + E - 1, kProcessThreads * E * 4) >= 2 * kSMs)
+    return process_u<T, 4>(r, x, ld, S, V, out, ld_out, st);
+  return process_u<T, 1>(r, x, ld, S, V, out, ld_out, st);
 }
 
 template <typename T>

@@ -5,64 +5,94 @@ Tensors are on a CUDA device, in float32 or bfloat16 (ids int32; other integer t
 on the current stream of its tensors' device.  `distill_loss` and `embed_tokens` record autograd; the other functions
 are forward only.  There is no CPU or PyTorch fallback.
 """
+import contextlib
 import dataclasses
+import struct
 from typing import Optional, Union
 
 import torch
 
 from . import _lib as L_
-from ._lib import check, lib, ptr, stream_ptr, workspace, dtype_code
+from ._lib import check, lib, workspace, dtype_code
 
 Per = Union[float, torch.Tensor]  # one value for all rows, or one per row
+I32, F32 = torch.int32, torch.float32
+_NOTHING = contextlib.nullcontext()
+# sdm_logit_rules and sdm_choice_params as C lays them out (a call at one stream is bound by the host: packing a struct
+# this way takes a fifth of setting its fields one by one)
+_RULES = struct.Struct("@PqiPPPPPfffPPiPiP")
+_CHOICE = struct.Struct("@PPPPffi0P")
 
 
-def _device(t, name):
-    if not t.is_cuda:
+def _ix(t, name):
+    """Device index of a CUDA tensor."""
+    ix = t.get_device()
+    if ix < 0:
         raise ValueError(f"{name}: libsdm_b200 takes device tensors only")
-    return t.device
+    return ix
 
 
-def _on(t, dev, name, dtype, shape):
-    """t as a contiguous tensor of dtype on dev with the given shape (None: any size)."""
+def _stream(ix):
+    return torch._C._cuda_getCurrentRawStream(ix)
+
+
+def _guard(ix):
+    """Makes device ix current for a launch."""
+    return _NOTHING if torch.cuda.current_device() == ix else torch.cuda.device(ix)
+
+
+def _at(t, ix, name, dtype, shape, keep):
+    """Pointer of t (None: 0) as a contiguous tensor of dtype on device ix with the given shape (None: any size).  A
+    converted copy goes into `keep`, which lives until the launch."""
     if t is None:
-        return None
-    if t.device != dev:
-        raise ValueError(f"{name} is on {t.device}, the logits or ids on {dev}")
+        return 0
+    if t.dtype is dtype and t.get_device() == ix and t.shape == shape and t.is_contiguous():
+        return t.data_ptr()
+    if t.get_device() != ix:
+        raise ValueError(f"{name} is on {t.device}, the logits or ids are on device {ix}")
     if t.dim() != len(shape) or any(w is not None and n != w for n, w in zip(t.shape, shape)):
         raise ValueError(f"{name} has shape {tuple(t.shape)}, wanted {tuple('any' if w is None else w for w in shape)}")
-    if dtype == torch.int32 and (t.dtype.is_floating_point or t.dtype.is_complex):
+    if dtype is I32 and (t.dtype.is_floating_point or t.dtype.is_complex):
         raise TypeError(f"{name} holds whole numbers, not {t.dtype}")
-    return t.detach().to(dtype).contiguous()
+    t = t.detach().to(dtype).contiguous()
+    keep.append(t)
+    return t.data_ptr()
+
+
+def _per(v, ix, name, dtype, S, keep):
+    """(pointer, value for all rows) of a per-row parameter."""
+    if isinstance(v, torch.Tensor):
+        return _at(v, ix, name, dtype, (S,), keep), 0
+    return 0, v
 
 
 def _rows(t, name):
     """t (N, V) with contiguous rows, and its row stride."""
     if t.dim() != 2:
         raise ValueError(f"{name} is 2-D (rows, vocabulary), not {t.dim()}-D")
-    dtype_code(t.dtype)
-    if t.shape[1] > 1 and t.stride(1) != 1 or t.shape[0] > 1 and t.stride(0) < t.shape[1]:
-        t = t.contiguous()
-    return t, (t.stride(0) if t.shape[0] > 1 else t.shape[1])
+    N, V = t.shape
+    if t.is_contiguous():
+        return t, V
+    if V > 1 and t.stride(1) != 1 or N > 1 and t.stride(0) < V:
+        return t.contiguous(), V
+    return t, (t.stride(0) if N > 1 else V)
 
 
 def _out_rows(out, like, name):
+    """Row stride of an output for `like`'s rows."""
     if out.shape != like.shape or out.dtype != like.dtype or out.device != like.device:
         raise ValueError(f"{name} has the shape, dtype and device of the logits")
-    if out.shape[1] > 1 and out.stride(1) != 1 or out.shape[0] > 1 and out.stride(0) < out.shape[1]:
+    N, V = out.shape
+    if V > 1 and out.stride(1) != 1 or N > 1 and out.stride(0) < V:
         raise ValueError(f"{name} needs contiguous rows that do not overlap")
-    if out.data_ptr() != like.data_ptr() and out.untyped_storage().data_ptr() == like.untyped_storage().data_ptr():
-        span = lambda t: (t.data_ptr(), t.data_ptr() + ((t.shape[0] - 1) * t.stride(0) + t.shape[1]) * t.element_size())  # noqa: E731
-        (a0, a1), (b0, b1) = span(out), span(like)
-        if a0 < b1 and b0 < a1:
-            raise ValueError(f"{name} overlaps the logits without being them")
-    return out
 
+    def span(t):
+        return t.data_ptr(), t.data_ptr() + ((N - 1) * t.stride(0) + (V - 1) * t.stride(1) + 1) * t.element_size()
 
-def _per(v, dev, name, dtype, S):
-    """(tensor or None, value for all rows) of a per-row parameter."""
-    if isinstance(v, torch.Tensor):
-        return _on(v, dev, name, dtype, (S,)), 0
-    return None, v
+    (a0, a1), (b0, b1) = span(out), span(like)
+    if a0 < b1 and b0 < a1 and (a0 != b0 or out.stride() != like.stride()) and N * V > 0:
+        raise ValueError(f"{name} overlaps the logits without being them")
+    return out.stride(0) if N > 1 else V
 
 
 @dataclasses.dataclass
@@ -86,51 +116,57 @@ class LogitRules:
     mask: Optional[torch.Tensor] = None
     mask_row: Optional[torch.Tensor] = None
 
-    def _struct(self, S, V, dev):
-        """(sdm_logit_rules, the tensors it points to)."""
-        i32, f32 = torch.int32, torch.float32
-        hist = _on(self.history, dev, "history", i32, (S, None))
-        hl = _on(self.history_len, dev, "history_len", i32, (S,))
-        pl = _on(self.prompt_len, dev, "prompt_len", i32, (S,))
-        if hist is None and (hl is not None or pl is not None):
+    def _struct(self, S, V, ix, keep):
+        """sdm_logit_rules for S rows over V tokens on device ix."""
+        hist, bi, bv, mask = self.history, self.bias_ids, self.bias_values, self.mask
+        L = nb = G = 0
+        hp = hlp = plp = bip = bvp = mp = 0
+        if hist is not None:
+            L = hist.shape[-1]
+            hp = _at(hist, ix, "history", I32, (S, L), keep)
+            hlp = _at(self.history_len, ix, "history_len", I32, (S,), keep)
+            plp = _at(self.prompt_len, ix, "prompt_len", I32, (S,), keep)
+            if L == 0:
+                hp = hlp = plp = 0
+        elif self.history_len is not None or self.prompt_len is not None:
             raise ValueError("history_len and prompt_len need a history")
-        if hist is not None and hist.shape[1] == 0:
-            hist = hl = pl = None
-        if (self.bias_ids is None) != (self.bias_values is None):
+        if bi is not None and bv is not None:
+            nb = bi.shape[-1]
+            bip = _at(bi, ix, "bias_ids", I32, (S, nb), keep)
+            bvp = _at(bv, ix, "bias_values", F32, (S, nb), keep)
+        elif bi is not None or bv is not None:
             raise ValueError("bias_ids and bias_values come together")
-        bi = _on(self.bias_ids, dev, "bias_ids", i32, (S, None))
-        bv = _on(self.bias_values, dev, "bias_values", f32, (S, None if bi is None else bi.shape[1]))
-        mask = _on(self.mask, dev, "mask", i32, (None, -(-V // 32)))
-        mr = _on(self.mask_row, dev, "mask_row", i32, (S,))
-        if mask is None and mr is not None:
+        mrp = _at(self.mask_row, ix, "mask_row", I32, (S,), keep)
+        if mask is not None:
+            G = mask.shape[0]
+            mp = _at(mask, ix, "mask", I32, (G, -(-V // 32)), keep)
+            if not mrp and G != 1 and G != S:
+                raise ValueError(f"{G} masks for {S} rows need mask_row")
+        elif mrp:
             raise ValueError("mask_row needs a mask")
-        if mask is not None and mr is None and mask.shape[0] not in (1, S):
-            raise ValueError(f"{mask.shape[0]} masks for {S} rows need mask_row")
-        rep, rep_all = _per(self.repetition, dev, "repetition", f32, S)
-        frq, frq_all = _per(self.frequency, dev, "frequency", f32, S)
-        prs, prs_all = _per(self.presence, dev, "presence", f32, S)
-        keep = (hist, hl, pl, rep, frq, prs, bi, bv, mask, mr)
-        r = L_.LogitRules(
-            history=ptr(hist), history_ld=0 if hist is None else hist.shape[1],
-            history_n=0 if hist is None else hist.shape[1], history_len=ptr(hl), prompt_len=ptr(pl),
-            repetition=ptr(rep), frequency=ptr(frq), presence=ptr(prs), repetition_all=rep_all,
-            frequency_all=frq_all, presence_all=prs_all, bias_ids=ptr(bi), bias_values=ptr(bv),
-            bias_n=0 if bi is None else bi.shape[1], mask=ptr(mask), mask_rows=0 if mask is None else mask.shape[0],
-            mask_row=ptr(mr))
-        return r, keep
+        rp, ra = _per(self.repetition, ix, "repetition", F32, S, keep)
+        fp, fa = _per(self.frequency, ix, "frequency", F32, S, keep)
+        pp, pa = _per(self.presence, ix, "presence", F32, S, keep)
+        return L_.LogitRules.from_buffer_copy(
+            _RULES.pack(hp, L, L, hlp, plp, rp, fp, pp, ra, fa, pa, bip, bvp, nb, mp, G, mrp))
 
 
 def process_logits(logits, rules=None, out=None):
     """The rules on logits (S, V), in their dtype (rounded once): penalties, biases, then the mask (sdm_logits_process).
     out: where to write (the logits themselves are allowed), else a new tensor."""
-    dev = _device(logits, "logits")
-    x, ld = _rows(logits.detach(), "logits")
+    ix = _ix(logits, "logits")
+    code = dtype_code(logits.dtype)
+    x, ld = _rows(logits, "logits")
     S, V = x.shape
-    out = torch.empty(S, V, dtype=x.dtype, device=dev) if out is None else _out_rows(out, logits, "out")
-    r, keep = (rules or LogitRules())._struct(S, V, dev)
-    with torch.cuda.device(dev):
-        check(lib().sdm_logits_process(r, ptr(x), ld, S, V, dtype_code(x.dtype), ptr(out),
-                                       out.stride(0) if S > 1 else V, stream_ptr(dev)), "sdm_logits_process")
+    if out is None:
+        out, ld_out = torch.empty(S, V, dtype=x.dtype, device=x.device), V
+    else:
+        ld_out = _out_rows(out, logits, "out")
+    keep = []
+    r = None if rules is None else rules._struct(S, V, ix, keep)
+    with _guard(ix):
+        check(lib().sdm_logits_process(r, x.data_ptr(), ld, S, V, code, out.data_ptr(), ld_out, _stream(ix)),
+              "sdm_logits_process")
     return out
 
 
@@ -140,46 +176,52 @@ def sample_logits(logits, rules=None, u=None, temperature: Per = 1.0, top_k: Uni
     distribution drawn from (sdm_logits_choose).  u (S,) in [0, 1) picks the token: with the kept tokens in index
     order, the first whose running probability exceeds it.  temperature 0 takes the largest logit (u may be None if
     that is so for all rows).  A row that allows no token gives -1 and -infinity."""
-    dev = _device(logits, "logits")
-    x, ld = _rows(logits.detach(), "logits")
+    ix = _ix(logits, "logits")
+    code = dtype_code(logits.dtype)
+    x, ld = _rows(logits, "logits")
     S, V = x.shape
-    r, keep = (rules or LogitRules())._struct(S, V, dev)
-    f32 = torch.float32
-    tt, t_all = _per(temperature, dev, "temperature", f32, S)
-    tk, k_all = _per(top_k, dev, "top_k", torch.int32, S)
-    tp, p_all = _per(top_p, dev, "top_p", f32, S)
-    u = _on(u, dev, "u", f32, (S,))
-    if u is None and (tt is not None or t_all != 0):
+    keep = []
+    r = None if rules is None else rules._struct(S, V, ix, keep)
+    tp, ta = _per(temperature, ix, "temperature", F32, S, keep)
+    kp, ka = _per(top_k, ix, "top_k", I32, S, keep)
+    pp, pa = _per(top_p, ix, "top_p", F32, S, keep)
+    if u is None and (tp or ta != 0):
         raise ValueError("sampling needs u, one number in [0, 1) per row")
-    c = L_.ChoiceParams(temperature=ptr(tt), top_k=ptr(tk), top_p=ptr(tp), u=ptr(u), temperature_all=t_all,
-                        top_p_all=p_all, top_k_all=k_all)
-    ids = torch.empty(S, dtype=torch.int32, device=dev)
-    lp = torch.empty(S, dtype=f32, device=dev)
-    with torch.cuda.device(dev):
-        check(lib().sdm_logits_choose(r, c, ptr(x), ld, S, V, dtype_code(x.dtype), ptr(ids), ptr(lp),
-                                      stream_ptr(dev)), "sdm_logits_choose")
+    up = _at(u, ix, "u", F32, (S,), keep)
+    c = L_.ChoiceParams.from_buffer_copy(_CHOICE.pack(tp, kp, pp, up, ta, pa, ka))
+    ids = torch.empty(S, dtype=I32, device=x.device)
+    lp = torch.empty(S, dtype=F32, device=x.device)
+    with _guard(ix):
+        check(lib().sdm_logits_choose(r, c, x.data_ptr(), ld, S, V, code, ids.data_ptr(), lp.data_ptr(), _stream(ix)),
+              "sdm_logits_choose")
     return ids, lp
 
 
 # -------------------------------------------------------------------------------------------------- distillation
 def _distill(logits, teacher_ids, teacher_logits, targets, temperature, alpha, row_weight, teacher_lse, grad_scale,
              want_grad, out=None):
-    dev = _device(logits, "logits")
-    x, ld = _rows(logits.detach(), "logits")
+    ix = _ix(logits, "logits")
+    code = dtype_code(logits.dtype)
+    x, ld = _rows(logits, "logits")
     N, V = x.shape
-    ids = _on(teacher_ids, dev, "teacher_ids", torch.int32, (N, None))
-    tl = _on(teacher_logits, dev, "teacher_logits", torch.float32, (N, ids.shape[1]))
-    tg = _on(targets, dev, "targets", torch.int32, (N,))
-    w = _on(row_weight, dev, "row_weight", torch.float32, (N,))
-    lse = _on(teacher_lse, dev, "teacher_lse", torch.float32, (N,))
-    loss = torch.empty(N, dtype=torch.float32, device=dev)
-    grad = None
+    k = teacher_ids.shape[-1]
+    keep = []
+    idp = _at(teacher_ids, ix, "teacher_ids", I32, (N, k), keep)
+    tlp = _at(teacher_logits, ix, "teacher_logits", F32, (N, k), keep)
+    tgp = _at(targets, ix, "targets", I32, (N,), keep)
+    wp = _at(row_weight, ix, "row_weight", F32, (N,), keep)
+    lsep = _at(teacher_lse, ix, "teacher_lse", F32, (N,), keep)
+    loss = torch.empty(N, dtype=F32, device=x.device)
+    grad, gp, ldg = None, 0, 0
     if want_grad:
-        grad = torch.empty(N, V, dtype=x.dtype, device=dev) if out is None else _out_rows(out, logits, "out")
-    with torch.cuda.device(dev):
-        check(lib().sdm_distill(ptr(x), ld, N, V, dtype_code(x.dtype), ptr(ids), ptr(tl), ids.shape[1], ptr(lse),
-                                ptr(tg), ptr(w), temperature, alpha, grad_scale, ptr(loss), ptr(grad),
-                                0 if grad is None else (grad.stride(0) if N > 1 else V), stream_ptr(dev)), "sdm_distill")
+        if out is None:
+            grad, ldg = torch.empty(N, V, dtype=x.dtype, device=x.device), V
+        else:
+            grad, ldg = out, _out_rows(out, logits, "out")
+        gp = grad.data_ptr()
+    with _guard(ix):
+        check(lib().sdm_distill(x.data_ptr(), ld, N, V, code, idp, tlp, k, lsep, tgp, wp, temperature, alpha,
+                                grad_scale, loss.data_ptr(), gp, ldg, _stream(ix)), "sdm_distill")
     return loss, grad
 
 
@@ -210,9 +252,10 @@ class _DistillLoss(torch.autograd.Function):
             if getattr(ctx, "used", False):
                 raise RuntimeError("the gradient was formed with the loss and handed out by the first backward pass")
             ctx.used = True
-            with torch.cuda.device(grad.device):
-                check(lib().sdm_scale_rows(ptr(grad), V, N, V, dtype_code(grad.dtype), ptr(g), 0 if one else 1,
-                                           stream_ptr(grad.device)), "sdm_scale_rows")
+            ix = grad.get_device()
+            with _guard(ix):
+                check(lib().sdm_scale_rows(grad.data_ptr(), V, N, V, dtype_code(grad.dtype), g.data_ptr(),
+                                           0 if one else 1, _stream(ix)), "sdm_scale_rows")
         return grad, None, None
 
 
@@ -258,43 +301,53 @@ class _ScaledSum(torch.autograd.Function):
 
 # ------------------------------------------------------------------------------------------------- token table
 def _ids32(ids):
-    _device(ids, "ids")
-    if ids.dtype.is_floating_point or ids.dtype.is_complex or ids.dtype == torch.bool:
+    if ids.dtype is I32 and ids.is_contiguous():
+        return ids
+    if ids.dtype.is_floating_point or ids.dtype.is_complex or ids.dtype is torch.bool:
         raise TypeError(f"ids are whole numbers, not {ids.dtype}")
-    return ids.detach().to(torch.int32).contiguous()
+    return ids.detach().to(I32).contiguous()
 
 
 def embed_grad(ids, dout, num_rows, scale=1.0, padding_id=None, dtype=torch.float32, out=None):
     """The token table's gradient (num_rows, d): scale times the sum of dout (..., d) over the positions of each id
     (sdm_embed_grad).  ids outside the table and padding_id are skipped.  out: a gradient (num_rows, d), float32 or
     bfloat16, to add to; else a new one of `dtype`.  The same inputs give the same bits."""
+    ix = _ix(ids, "ids")
     i32 = _ids32(ids)
-    dev = i32.device
-    if dout.device != dev or dout.shape[:-1] != ids.shape:
-        raise ValueError(f"dout {tuple(dout.shape)} on {dout.device} does not go with ids {tuple(ids.shape)} on {dev}")
+    if dout.get_device() != ix or dout.shape[:-1] != ids.shape:
+        raise ValueError(f"dout {tuple(dout.shape)} on {dout.device} does not go with ids {tuple(ids.shape)} on {ids.device}")
     d = dout.shape[-1]
     N = i32.numel()
-    g = dout.detach()
-    if g.dim() != 2 or g.stride(1) != 1 or g.stride(0) < d:
-        g = g.reshape(N, d).contiguous()
-    if out is not None and (out.shape != (num_rows, d) or not out.is_contiguous() or out.device != dev):
-        raise ValueError(f"out is a contiguous ({num_rows}, {d}) tensor on {dev}")
-    grad = torch.empty(num_rows, d, dtype=dtype, device=dev) if out is None else out
-    ws = workspace(lib().sdm_embed_grad_workspace_size(N, d, num_rows), dev)
-    with torch.cuda.device(dev):
-        check(lib().sdm_embed_grad(ptr(i32), ptr(g), g.stride(0) if N > 1 else d, N, d, num_rows, scale,
-                                   -1 if padding_id is None else padding_id, dtype_code(g.dtype),
-                                   dtype_code(grad.dtype), int(out is not None), ptr(grad), ptr(ws), ws.numel(),
-                                   stream_ptr(dev)), "sdm_embed_grad")
+    if dout.is_contiguous():
+        ld = d
+    elif dout.dim() == 2 and dout.stride(1) == 1 and dout.stride(0) >= d:
+        ld = dout.stride(0) if N > 1 else d
+    else:
+        dout, ld = dout.contiguous(), d
+    if out is None:
+        grad = torch.empty(num_rows, d, dtype=dtype, device=i32.device)
+    else:
+        if out.shape != (num_rows, d) or not out.is_contiguous() or out.get_device() != ix:
+            raise ValueError(f"out is a contiguous ({num_rows}, {d}) tensor on {ids.device}")
+        grad = out
+    nbytes = lib().sdm_embed_grad_workspace_size(N, d, num_rows)
+    ws = workspace(nbytes, i32.device)
+    with _guard(ix):
+        check(lib().sdm_embed_grad(i32.data_ptr(), dout.data_ptr(), ld, N, d, num_rows, scale,
+                                   -1 if padding_id is None else padding_id, dtype_code(dout.dtype),
+                                   dtype_code(grad.dtype), int(out is not None), grad.data_ptr(), ws.data_ptr(),
+                                   nbytes, _stream(ix)), "sdm_embed_grad")
     return grad
 
 
 def _embed(i32, table, scale, bad):
     V, d = table.shape
+    ix = i32.get_device()
     out = torch.empty(*i32.shape, d, dtype=table.dtype, device=table.device)
-    with torch.cuda.device(table.device):
-        check(lib().sdm_embed_scaled(ptr(i32), ptr(table), i32.numel(), d, V, scale, dtype_code(table.dtype), ptr(out),
-                                     ptr(bad), stream_ptr(table.device)), "sdm_embed_scaled")
+    with _guard(ix):
+        check(lib().sdm_embed_scaled(i32.data_ptr(), table.data_ptr(), i32.numel(), d, V, scale,
+                                     dtype_code(table.dtype), out.data_ptr(), 0 if bad is None else bad.data_ptr(),
+                                     _stream(ix)), "sdm_embed_scaled")
     return out
 
 
@@ -316,13 +369,14 @@ class _EmbedTokens(torch.autograd.Function):
 def embed_tokens(ids, table, scale=1.0, padding_id=None, bad=None):
     """scale * table[ids] in the table's dtype (sdm_embed_scaled), differentiable by the table (padding_id's row gets
     no gradient).  An id outside the table gives a zero row and sets bad (a device int32 tensor of one element)."""
+    ix = _ix(ids, "ids")
     i32 = _ids32(ids)
     if table.dim() != 2:
         raise ValueError(f"the table is 2-D (tokens, d), not {table.dim()}-D")
-    if table.device != i32.device:
-        raise ValueError(f"ids are on {i32.device}, the table on {table.device}")
-    if bad is not None and (bad.dtype != torch.int32 or bad.device != i32.device):
+    if table.get_device() != ix:
+        raise ValueError(f"ids are on {ids.device}, the table is on {table.device}")
+    if bad is not None and (bad.dtype is not I32 or bad.get_device() != ix):
         raise ValueError("bad is an int32 tensor on the ids' device")
-    if torch.is_grad_enabled() and table.requires_grad:
+    if table.requires_grad and torch.is_grad_enabled():
         return _EmbedTokens.apply(table, i32, scale, padding_id, bad)
-    return _embed(i32, table.detach().contiguous(), scale, bad)
+    return _embed(i32, table if table.is_contiguous() else table.contiguous(), scale, bad)

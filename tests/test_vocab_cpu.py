@@ -102,13 +102,22 @@ def test_python_checks_need_device_tensors():
         S.distill_loss(x, i, torch.zeros(2, 3), reduction="max")
 
 
+def test_packed_structs_are_the_declared_ones():
+    from sdmchat_b200 import vocab as W
+    assert W._RULES.size == ctypes.sizeof(_lib.LogitRules) and W._CHOICE.size == ctypes.sizeof(_lib.ChoiceParams)
+    vals = list(range(1, 18))
+    r = _lib.LogitRules.from_buffer_copy(W._RULES.pack(*vals))
+    assert [getattr(r, n) for n, _ in r._fields_] == vals
+    c = _lib.ChoiceParams.from_buffer_copy(W._CHOICE.pack(*vals[:7]))
+    assert [getattr(c, n) for n, _ in c._fields_] == vals[:7]
+
+
 def test_python_checks_of_rules():
     """Shapes, types and pairs are looked at before any pointer is taken (host tensors stand in)."""
-    cpu = torch.device("cpu")
     i, f = torch.zeros(3, 4, dtype=torch.int32), torch.zeros(3)
     for kw in (dict(history=i[:2]), dict(history=i.float()), dict(history_len=i[:, 0]), dict(prompt_len=i[:, 0]),
                dict(bias_ids=i), dict(bias_values=torch.zeros(3, 4)), dict(bias_ids=i, bias_values=torch.zeros(3, 5)),
                dict(mask=torch.zeros(1, 3, dtype=torch.int32)), dict(mask=torch.zeros(2, 4, dtype=torch.int32)),
                dict(mask_row=i[:, 0]), dict(repetition=f[:2]), dict(frequency=i)):
         with pytest.raises((ValueError, TypeError)):
-            S.LogitRules(**kw)._struct(3, 100, cpu)
+            S.LogitRules(**kw)._struct(3, 100, -1, [])
