@@ -5,9 +5,10 @@
 // event, q_r = sum of q over the tokens that are not listed, the loss gains T^2 p_r (log p_r - log q_r) and a token
 // that is not listed T p_r (q - q / q_r).  The hard loss's gradient is softmax(logits) - [target].
 //
-// A row (64 KB at 32,768 bfloat16 logits) is read from memory once, into the shared memory of a block, or of a
-// cluster of blocks that exchange their maxima and sums; the gradient is formed from that copy.
+// With the gradient, a row (64 KB at 32,768 bfloat16 logits) is read from memory once, into the shared memory of a
+// block, or of a cluster of blocks that exchange their maxima and sums; the gradient is formed from that copy.
 #include <math_constants.h>
+#include <type_traits>
 #include "vocab.cuh"
 
 namespace sdm {
@@ -15,272 +16,541 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kThreads = 512, kWarps = kThreads / 32;
+constexpr int kThreads = 256, kWarps = kThreads / 32;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 struct DistillShared {
-  float warp[3][kWarps];
-  float part[4][kMaxCluster];  // max, soft sum, hard sum by block
-  int id[kMaxTeacher];
+  float warp[4][kWarps];
+  float part[4][kMaxCluster];     // by block: max, sums
+  int id[kMaxTeacher];            // the row's entries, -1 where unused
   float logp[kMaxTeacher], val[kMaxTeacher];
-  float target_val;
-  float p_sum, lse;
+  float target_val, p_sum;
+  int repeated;                   // some id of this block's slice is listed twice
 };
 
-__device__ __forceinline__ float block_max(float v, float* warp) {
-  v = warp_max(v);
-  if ((threadIdx.x & 31) == 0) warp[threadIdx.x >> 5] = v;
-  __syncthreads();
-  float r = warp[0];
-#pragma unroll
-  for (int w = 1; w < kWarps; ++w) r = fmaxf(r, warp[w]);
+// Exponentials are 2^(v c - B), c = log2(e) / T and B = c max rounded to float32: the one rounding of B cancels in
+// every quotient and logarithm, which take the same B.
+__device__ __forceinline__ float ex2(float t) {
+  float e;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
+  return e;
+}
+
+// Two floats in one 64-bit register, for the paired instructions.
+typedef unsigned long long pair_t;
+__device__ __forceinline__ pair_t pair(float a, float b) {
+  pair_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
   return r;
 }
-__device__ __forceinline__ float block_sum(float v, float* warp) {
-  v = warp_sum(v);
-  if ((threadIdx.x & 31) == 0) warp[threadIdx.x >> 5] = v;
-  __syncthreads();
-  float r = 0.f;
-#pragma unroll
-  for (int w = 0; w < kWarps; ++w) r += warp[w];
+__device__ __forceinline__ float2 both(pair_t p) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(p));
   return r;
 }
+__device__ __forceinline__ pair_t fma_pair(pair_t a, pair_t b, pair_t c) {
+  pair_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ pair_t add_pair(pair_t a, pair_t b) {
+  pair_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+// 2^t on the FMA pipe, for a kernel that would wait on the exponential unit (16 a clock and SM against 128 FMAs):
+// t = n + f with n = rint(t) (Cody and Waite's reduction), a polynomial in f in [-1/2, 1/2] fitted by Remez's exchange
+// to the least relative error (7.5e-8; 2.2e-7 in float32), and n added to the exponent.  Below -126 it stays at 2^-126.
+__device__ __forceinline__ pair_t exp2_pair(pair_t t) {
+  float2 v = both(t);
+  t = pair(fmaxf(v.x, -126.f), fmaxf(v.y, -126.f));
+  const pair_t z = add_pair(t, pair(12582912.f, 12582912.f));  // 2^23 + 2^22 + n
+  const pair_t n = add_pair(z, pair(-12582912.f, -12582912.f));
+  const pair_t f = fma_pair(n, pair(-1.f, -1.f), t);
+  constexpr float kExp2[6] = {1.0000001192092896f, 0.6931469440460205f, 0.24022120237350464f,
+                              0.05550713092088699f, 0.009675540961325169f, 0.0013276472454890609f};
+  pair_t p = pair(kExp2[5], kExp2[5]);
+#pragma unroll
+  for (int i = 4; i >= 0; --i) p = fma_pair(p, f, pair(kExp2[i], kExp2[i]));
+  const float2 pv = both(p), zv = both(z);
+  return pair(__int_as_float(__float_as_int(pv.x) + (__float_as_int(zv.x) << 23)),
+              __int_as_float(__float_as_int(pv.y) + (__float_as_int(zv.y) << 23)));
+}
+
+// Largest of a chunk's elements (NaN is passed over).
+template <typename T>
+__device__ __forceinline__ float chunk_max(uint4 u);
+template <>
+__device__ __forceinline__ float chunk_max<float>(uint4 u) {
+  return fmaxf(fmaxf(__uint_as_float(u.x), __uint_as_float(u.y)), fmaxf(__uint_as_float(u.z), __uint_as_float(u.w)));
+}
+template <>
+__device__ __forceinline__ float chunk_max<bf16_t>(uint4 u) {
+  const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&u);
+  const __nv_bfloat162 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+  return fmaxf(__low2float(m), __high2float(m));
+}
+
+// Sum of up to three values over the block, each in the same order in every thread.
+__device__ __forceinline__ void block_sum3(DistillShared& s, float& a, float& b, float& c) {
+  a = warp_sum(a);
+  b = warp_sum(b);
+  c = warp_sum(c);
+  if ((threadIdx.x & 31) == 0) {
+    s.warp[1][threadIdx.x >> 5] = a;
+    s.warp[2][threadIdx.x >> 5] = b;
+    s.warp[3][threadIdx.x >> 5] = c;
+  }
+  __syncthreads();
+  a = b = c = 0.f;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    a += s.warp[1][w];
+    b += s.warp[2][w];
+    c += s.warp[3][w];
+  }
+}
+
+// What a block needs to know of its row.
+struct Row {
+  int64_t row;
+  int V, k, tgt;
+  float w, inv_t;
+  bool hard;
+  int C, rank, v0, lo, hi;  // the block's tokens are v0 + [lo, hi), at positions [lo, hi) of its slice
+};
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads) distill_kernel(DistillArgs a, int slice) {
-  pdl_enter();
-  constexpr int E = Chunk<T>::E;
-  extern __shared__ uint4 buf4[];  // this block's slice of the row, by 16-byte chunk
-  T* buf = reinterpret_cast<T*>(buf4);
-  __shared__ DistillShared s;
-  auto cluster = cg::this_cluster();
-  const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
-  if (C > 1) cluster.sync();
-  const int64_t row = blockIdx.x / C;
-  const int tid = threadIdx.x;
-  const int V = a.V, k = a.k;
-  const T* x = static_cast<const T*>(a.logits) + row * a.ld;
-  T* g = a.dlogits ? static_cast<T*>(a.dlogits) + row * a.ld_grad : nullptr;
-  const float w = a.row_weight ? a.row_weight[row] : 1.f;
-  const int tgt = a.targets ? a.targets[row] : -1;
-  const bool hard = tgt >= 0 && tgt < V;
-  const int off = row_offset(x);
-  const int p0 = rank * slice;
-  const int v0 = p0 - off;  // the token of buf[0]
-  const int lo = max(0, -v0), hi = max(lo, min(slice, V - v0));
-  const bool vec_out = g && row_offset(g) == off;
+__device__ __forceinline__ Row row_of(const DistillArgs& a, int slice, int C, int rank, const T*& x) {
+  Row q;
+  q.C = C;
+  q.rank = rank;
+  q.row = blockIdx.x / C;
+  x = static_cast<const T*>(a.logits) + q.row * a.ld;
+  q.V = a.V;
+  q.k = a.k;
+  q.w = a.row_weight ? a.row_weight[q.row] : 1.f;
+  q.tgt = a.targets ? a.targets[q.row] : -1;
+  q.hard = q.tgt >= 0 && q.tgt < q.V;
+  q.inv_t = 1.f / a.temperature;
+  q.v0 = rank * slice - row_offset(x);
+  q.lo = max(0, -q.v0);
+  q.hi = max(q.lo, min(slice, q.V - q.v0));
+  return q;
+}
 
-  if (w == 0.f) {
-    if (rank == 0 && tid == 0) a.loss[row] = 0.f;
-    if (g) {
-      const uint4 zero = make_uint4(0, 0, 0, 0);
-      for (int i = tid * E; i < hi; i += kThreads * E) {
-        if (vec_out && i >= lo && i + E <= hi) {
-          *reinterpret_cast<uint4*>(g + v0 + i) = zero;
-        } else {
-          for (int e = max(i, lo); e < min(i + E, hi); ++e) g[v0 + e] = from_f32<T>(0.f);
-        }
-      }
-    }
-    return;
-  }
-
-  // the row into shared memory; the tail of the last chunk and the head of the first are filled with -infinity
-  float mx = -CUDART_INF_F;
-  for (int i = tid * E; i < hi; i += kThreads * E) {
-    uint4 u;
-    float f[E];
-    if (i >= lo && i + E <= hi) {
-      u = *reinterpret_cast<const uint4*>(x + v0 + i);
-      Chunk<T>::unpack(u, f);
-    } else {
-#pragma unroll
-      for (int e = 0; e < E; ++e) f[e] = i + e >= lo && i + e < hi ? to_f32(x[v0 + i + e]) : -CUDART_INF_F;
-      u = Chunk<T>::pack(f);
-    }
-    buf4[i / E] = u;
-#pragma unroll
-    for (int e = 0; e < E; ++e) mx = fmaxf(mx, f[e]);
-  }
-
-  // the teacher's distribution (every block of the cluster computes it)
-  const float inv_t = 1.f / a.temperature;
-  for (int j = tid; j < k; j += kThreads) {
-    int id = a.t_ids[row * k + j];
-    const float t = a.t_logits[row * k + j];
-    if (id < 0 || id >= V || t == -CUDART_INF_F) id = -1;
+// The row's entries and the logits they point at (every block of a cluster takes all of them).
+template <typename T>
+__device__ __forceinline__ void load_teacher(const DistillArgs& a, const Row& q, const T* x, DistillShared& s) {
+  for (int j = threadIdx.x; j < q.k; j += kThreads) {
+    int id = a.t_ids[q.row * q.k + j];
+    const float t = a.t_logits[q.row * q.k + j];
+    if (id < 0 || id >= q.V || t == -CUDART_INF_F) id = -1;
     s.id[j] = id;
     s.logp[j] = id >= 0 ? __fdiv_rn(t, a.temperature) : -CUDART_INF_F;
     s.val[j] = id >= 0 ? to_f32(x[id]) : 0.f;
   }
-  if (hard && tid == 0) s.target_val = to_f32(x[tgt]);
-  mx = block_max(mx, s.warp[0]);
-  if (tid < 32) {
-    float tm = -CUDART_INF_F;
-    for (int j = tid; j < k; j += 32) tm = fmaxf(tm, s.logp[j]);
+  if (threadIdx.x == kThreads - 1) s.target_val = q.hard ? to_f32(x[q.tgt]) : 0.f;
+}
+
+// One warp: log p of each entry, and their sum (-1: the row has no entry).
+__device__ __forceinline__ void teacher_softmax(const DistillArgs& a, const Row& q, DistillShared& s) {
+  const int lane = threadIdx.x & 31;
+  float lse, tm = -CUDART_INF_F;
+  bool any = false;
+  for (int j = lane; j < q.k; j += 32) {
+    tm = fmaxf(tm, s.logp[j]);
+    any |= s.id[j] >= 0;
+  }
+  any = __any_sync(0xffffffffu, any);
+  if (a.t_lse) {
+    lse = a.t_lse[q.row];
+  } else {
     tm = warp_max(tm);
-    const bool some = tm > -CUDART_INF_F || tm != tm;
-    float lse = 0.f;
-    if (a.t_lse) {
-      lse = a.t_lse[row];
-    } else if (some) {
-      float sum = 0.f;
-      for (int j = tid; j < k; j += 32) sum += s.id[j] >= 0 ? expf(s.logp[j] - tm) : 0.f;
-      lse = tm + logf(warp_sum(sum));
-    }
-    float ps = 0.f;
-    for (int j = tid; j < k; j += 32) {
-      s.logp[j] -= lse;
-      if (s.id[j] >= 0) ps += expf(s.logp[j]);
-    }
-    ps = warp_sum(ps);
-    bool any = false;
-    for (int j = tid; j < k; j += 32) any |= s.id[j] >= 0;
-    any = __any_sync(0xffffffffu, any);
-    if (tid == 0) {
-      s.p_sum = any ? ps : -1.f;
-    }
+    float sum = 0.f;
+    for (int j = lane; j < q.k; j += 32) sum += s.id[j] >= 0 ? expf(s.logp[j] - tm) : 0.f;
+    lse = tm + logf(warp_sum(sum));
   }
+  float ps = 0.f;
+  for (int j = lane; j < q.k; j += 32) {
+    s.logp[j] -= lse;
+    if (a.t_lse && s.id[j] >= 0) ps += expf(s.logp[j]);
+  }
+  if (a.t_lse) ps = warp_sum(ps);
+  if (lane == 0) s.p_sum = !any ? -1.f : a.t_lse ? ps : lse != lse ? lse : 1.f;  // a softmax's sum is 1
+}
+
+// Whether entry j is the first with its id; ids are looked through only where one is repeated.
+__device__ __forceinline__ bool is_first(const DistillShared& s, int j) {
+  if (s.repeated)
+    for (int i = 0; i < j; ++i)
+      if (s.id[i] == s.id[j]) return false;
+  return true;
+}
+
+// The row's loss from its sums (one warp): st, s1 over all tokens at T and at 1, rest over the unlisted ones at T.
+__device__ __forceinline__ float row_loss(const DistillArgs& a, const Row& q, const DistillShared& s, float ct,
+                                          float Bt, float B1, float st, float s1, float rest) {
+  const int lane = threadIdx.x & 31;
+  float loss = 0.f;
+  if (s.p_sum != -1.f) {
+    const float lst = log2f(st);
+    float sum = 0.f;
+    for (int j = lane; j < q.k; j += 32) {
+      if (s.id[j] < 0) continue;
+      const float lp = s.logp[j], p = expf(lp);
+      if (p > 0.f || p != p) sum += p * (lp - kLn2 * (fmaf(s.val[j], ct, -Bt) - lst));
+    }
+    sum = warp_sum(sum);
+    const float pr = a.t_lse ? fmaxf(0.f, 1.f - s.p_sum) : 0.f;
+    if (pr > 0.f) sum += pr * (logf(pr) - kLn2 * (log2f(rest) - lst));
+    loss = a.alpha * sum * (a.temperature * a.temperature);
+  }
+  if (q.hard) loss += (1.f - a.alpha) * kLn2 * (log2f(s1) - fmaf(s.target_val, kLog2e, -B1));
+  return q.w * loss;
+}
+
+// A block's slice in 16-byte chunks: whole ones [c0, c1), and up to 2 E tokens of its first and last chunk that other
+// blocks or rows share (edge(t), t < 2 E; a position or -1).
+struct Chunks {
+  int c0, c1, lo, hi, E;
+  __device__ Chunks(const Row& q, int e) {
+    E = e;
+    lo = q.lo;
+    hi = q.hi;
+    c0 = (lo + E - 1) / E;
+    c1 = max(c0, hi / E);
+  }
+  __device__ int edge(int t) const {
+    if (t < E) return lo + t < min(c0 * E, hi) ? lo + t : -1;
+    const int i = c1 * E + t - E;
+    return t < 2 * E && i >= lo && i < hi ? i : -1;
+  }
+};
+
+// Loss and gradient.  NEXP 2: the exponentials at T and at 1 differ and both are wanted; 1: one serves.
+template <typename T, int NEXP>
+__global__ void __launch_bounds__(kThreads, 3) distill_grad_kernel(DistillArgs a, int slice) {
+  pdl_enter();
+  constexpr int E = Chunk<T>::E;
+  typedef typename std::conditional<sizeof(T) == 2, uint16_t, uint32_t>::type Tag;
+  extern __shared__ uint4 buf4[];  // this block's slice of the row, by 16-byte chunk
+  T* buf = reinterpret_cast<T*>(buf4);
+  __shared__ DistillShared s;
+  auto cluster = cg::this_cluster();
+  const int C = (int)cluster.num_blocks(), tid = threadIdx.x;
+  if (C > 1) cluster.sync();
+  const T* x;
+  const Row q = row_of<T>(a, slice, C, (int)cluster.block_rank(), x);
+  T* g = static_cast<T*>(a.dlogits) + q.row * a.ld_grad;
+  const int lo = q.lo, hi = q.hi, v0 = q.v0, k = q.k;
+  const bool vec_out = row_offset(g) == row_offset(x);
+  const Chunks ch(q, E);
+  const int edge = ch.edge(tid);  // at most one token of the ragged chunks per thread
+
+  // the row into shared memory, all of it on its way at once
+  for (int c = ch.c0 + tid; c < ch.c1; c += kThreads)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(buf4 + c)),
+                 "l"(x + v0 + c * E)
+                 : "memory");
+  if (q.w == 0.f) {
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    if (q.rank == 0 && tid == 0) a.loss[q.row] = 0.f;
+    const uint4 zero = make_uint4(0, 0, 0, 0);
+    for (int c = ch.c0 + tid; c < ch.c1; c += kThreads) {
+      if (vec_out) {
+        *reinterpret_cast<uint4*>(g + v0 + c * E) = zero;
+      } else {
+        for (int e = 0; e < E; ++e) g[v0 + c * E + e] = from_f32<T>(0.f);
+      }
+    }
+    if (edge >= 0) g[v0 + edge] = from_f32<T>(0.f);
+    return;
+  }
+
+  load_teacher(a, q, x, s);
+  float mx = -CUDART_INF_F;
+  if (edge >= 0) {
+    const T v = x[v0 + edge];
+    buf[edge] = v;
+    mx = to_f32(v);
+    if (mx != mx) mx = -CUDART_INF_F;
+  }
+  asm volatile("cp.async.wait_all;" ::: "memory");
+  for (int c = ch.c0 + tid; c < ch.c1; c += kThreads) mx = fmaxf(mx, chunk_max<T>(buf4[c]));  // its own copies
+  mx = warp_max(mx);
+  if ((tid & 31) == 0) s.warp[0][tid >> 5] = mx;
+  if (tid == 0) s.repeated = 0;
   __syncthreads();
-  if (C > 1) {
-    if (tid < C) *cluster.map_shared_rank(&s.part[0][rank], tid) = mx;
-    cluster.sync();
-    for (int r = 0; r < C; ++r) mx = fmaxf(mx, s.part[0][r]);
-  }
-  const bool soft = s.p_sum >= 0.f || s.p_sum != s.p_sum;
-  const float P = soft ? s.p_sum : 0.f;
-  const bool tail = a.t_lse != nullptr && soft;
-  // listed tokens leave the sums below; their terms are added once each, so that the mass of the others is a sum of
-  // its own and no difference
+  // The listed tokens of this block leave the sums below; their terms are added once each, so that the mass of the
+  // others is a sum of its own and no difference.  Each entry first writes its number in its token's place: one that
+  // does not find it again is not alone.
+  Tag* tag = reinterpret_cast<Tag*>(buf);
   for (int j = tid; j < k; j += kThreads) {
     const int i = s.id[j] - v0;
-    if (s.id[j] >= 0 && i >= lo && i < hi) buf[i] = from_f32<T>(-CUDART_INF_F);
+    if (s.id[j] >= 0 && i >= lo && i < hi) tag[i] = (Tag)j;
   }
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, s.warp[0][w]);
+  if (tid >= kThreads - 32) teacher_softmax(a, q, s);
   __syncthreads();
+  for (int j = tid; j < k; j += kThreads) {
+    const int i = s.id[j] - v0;
+    if (s.id[j] < 0 || i < lo || i >= hi) continue;
+    if (tag[i] != (Tag)j) s.repeated = 1;
+    buf[i] = from_f32<T>(-CUDART_INF_F);
+  }
+  if (C > 1) {
+    if (tid < C) *cluster.map_shared_rank(&s.part[0][q.rank], tid) = mx;
+    cluster.sync();
+    for (int r = 0; r < C; ++r) mx = fmaxf(mx, s.part[0][r]);
+  } else {
+    __syncthreads();
+  }
 
-  // sums of exp over the row, at T and (for the hard loss) at 1
-  const float ct = inv_t * 1.4426950408889634f, c1 = 1.4426950408889634f;
-  float st = 0.f, s1 = 0.f;
-  for (int i = tid * E; i < hi; i += kThreads * E) {
+  // sums of exp over the row, at T and at 1
+  const float ct = q.inv_t * kLog2e, c1 = kLog2e, nBt = -(mx * ct), nB1 = -(mx * c1);
+  float st = 0.f, s1 = 0.f, listed = 0.f;
+  // Four exponentials per bfloat16 logit would take the exponential unit longer than memory takes for the logit and
+  // its gradient: one of the four goes to the FMA pipe.
+  constexpr bool kMix = NEXP == 2 && sizeof(T) == 2;
+  pair_t s1p = pair(0.f, 0.f);
+#pragma unroll 2
+  for (int c = ch.c0 + tid; c < ch.c1; c += kThreads) {
     float f[E];
-    Chunk<T>::unpack(buf4[i / E], f);
+    Chunk<T>::unpack(buf4[c], f);
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      const float d = f[e] - mx;
-      if (soft) st += exp2f(d * ct);
-      if (hard) s1 += exp2f(d * c1);
+      st += ex2(fmaf(f[e], ct, nBt));
+      if (NEXP == 2 && !kMix) s1 += ex2(fmaf(f[e], c1, nB1));
+    }
+    if (kMix) {
+#pragma unroll
+      for (int e = 0; e < E; e += 2)
+        s1p = add_pair(s1p, exp2_pair(fma_pair(pair(f[e], f[e + 1]), pair(c1, c1), pair(nB1, nB1))));
     }
   }
-  st = block_sum(st, s.warp[1]);
-  s1 = block_sum(s1, s.warp[2]);
+  if (kMix) s1 = both(s1p).x + both(s1p).y;
+  if (edge >= 0) {
+    const float f = to_f32(buf[edge]);
+    st += ex2(fmaf(f, ct, nBt));
+    if (NEXP == 2) s1 += ex2(fmaf(f, c1, nB1));
+  }
+  for (int j = tid; j < k; j += kThreads) {
+    const int i = s.id[j] - v0;
+    if (s.id[j] < 0 || i < lo || i >= hi || !is_first(s, j)) continue;
+    listed += ex2(fmaf(s.val[j], ct, nBt));
+    if (NEXP == 2) s1 += ex2(fmaf(s.val[j], c1, nB1));
+  }
+  block_sum3(s, st, s1, listed);
   if (C > 1) {
     if (tid < C) {
-      *cluster.map_shared_rank(&s.part[1][rank], tid) = st;
-      *cluster.map_shared_rank(&s.part[2][rank], tid) = s1;
+      *cluster.map_shared_rank(&s.part[1][q.rank], tid) = st;
+      *cluster.map_shared_rank(&s.part[2][q.rank], tid) = s1;
+      *cluster.map_shared_rank(&s.part[3][q.rank], tid) = listed;
     }
     cluster.sync();
-    st = s1 = 0.f;
+    st = s1 = listed = 0.f;
     for (int r = 0; r < C; ++r) {
       st += s.part[1][r];
       s1 += s.part[2][r];
+      listed += s.part[3][r];
     }
   }
-  // the listed tokens' terms, each distinct one once: warp 0 of every block
-  __shared__ float listed[2];
-  if (tid < 32) {
-    float lt = 0.f, l1 = 0.f;
-    for (int j = tid; j < k; j += 32) {
-      const int id = s.id[j];
-      bool first = id >= 0;
-      for (int i = 0; i < j && first; ++i) first = s.id[i] != id;
-      if (first) {
-        const float d = s.val[j] - mx;
-        lt += exp2f(d * ct);
-        l1 += exp2f(d * c1);
-      }
-    }
-    lt = warp_sum(lt);
-    l1 = warp_sum(l1);
-    if (tid == 0) {
-      listed[0] = lt;
-      listed[1] = l1;
-    }
-  }
-  __syncthreads();
   const float rest = st;
-  st += listed[0];
-  s1 += listed[1];
-  const float pr = tail ? fmaxf(0.f, 1.f - P) : 0.f;
-  const float lst = logf(st);
+  st += listed;
+  if (NEXP == 1 || st != st) s1 = st;  // a NaN or an infinity shows in st
+  const float P = s.p_sum;
+  const bool soft = P != -1.f;
+  const float pr = soft && a.t_lse ? fmaxf(0.f, 1.f - P) : 0.f;
 
-  if (rank == 0 && tid < 32) {
-    float sum = 0.f;
-    if (soft) {
-      for (int j = tid; j < k; j += 32) {
-        if (s.id[j] < 0) continue;
-        const float lp = s.logp[j], p = expf(lp);
-        if (p > 0.f || p != p) sum += p * (lp - ((s.val[j] - mx) * inv_t - lst));
-      }
-      sum = warp_sum(sum);
-      if (pr > 0.f) sum += pr * (logf(pr) - (logf(rest) - lst));
+  // the gradient: a token that is not listed has qr exp(logit / T) + q1 exp(logit), each over its sum
+  const float scale = q.w * a.grad_scale;
+  const float ks = soft ? scale * a.alpha * a.temperature : 0.f, kh = q.hard ? scale * (1.f - a.alpha) : 0.f;
+  const float qt = soft ? ks * (P + pr) / st : 0.f;          // listed
+  const float qr = pr > 0.f ? qt - ks * pr / rest : qt;      // not listed
+  const float q1 = q.hard ? kh / s1 : 0.f;
+  const float qm = NEXP == 1 ? qr + q1 : qr;
+  auto value = [&](float f) {
+    float r = qm * ex2(fmaf(f, ct, nBt));
+    if (NEXP == 2) r = fmaf(q1, ex2(fmaf(f, c1, nB1)), r);
+    return r;
+  };
+  if (vec_out) {
+#pragma unroll 2
+    for (int c = ch.c0 + tid; c < ch.c1; c += kThreads) {
+      float f[E];
+      Chunk<T>::unpack(buf4[c], f);
+#pragma unroll
+      for (int e = 0; e < E; ++e) f[e] = value(f[e]);
+      *reinterpret_cast<uint4*>(g + v0 + c * E) = Chunk<T>::pack(f);
     }
-    if (tid == 0) {
-      float loss = a.alpha * sum * (a.temperature * a.temperature);
-      if (hard) loss += (1.f - a.alpha) * (logf(s1) - (s.target_val - mx));
-      a.loss[row] = w * loss;
-    }
+  } else {
+    for (int i = ch.c0 * E + tid; i < ch.c1 * E; i += kThreads) g[v0 + i] = from_f32<T>(value(to_f32(buf[i])));
   }
-  if (!g) return;
-
-  // the gradient: a token that is not listed has ct_rest exp(z) + c1_all exp(logit), both over their sums
-  const float scale = w * a.grad_scale;
-  const float ks = soft ? scale * a.alpha * a.temperature : 0.f, kh = hard ? scale * (1.f - a.alpha) : 0.f;
-  const float qt = ks * (P + pr) / st;                         // listed
-  const float qr = pr > 0.f ? qt - ks * pr / rest : qt;        // not listed
-  const float q1 = hard ? kh / s1 : 0.f;
-  for (int i = tid * E; i < hi; i += kThreads * E) {
-    float f[E];
-    Chunk<T>::unpack(buf4[i / E], f);
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const float d = f[e] - mx;
-      float r = 0.f;
-      if (soft) r = qr * exp2f(d * ct);
-      if (hard) r = fmaf(q1, exp2f(d * c1), r);
-      f[e] = r;
-    }
-    if (vec_out && i >= lo && i + E <= hi) {
-      *reinterpret_cast<uint4*>(g + v0 + i) = Chunk<T>::pack(f);
-    } else {
-#pragma unroll
-      for (int e = 0; e < E; ++e)
-        if (i + e >= lo && i + e < hi) g[v0 + i + e] = from_f32<T>(f[e]);
-    }
+  if (edge >= 0) g[v0 + edge] = from_f32<T>(value(to_f32(buf[edge])));
+  if (q.rank == 0 && tid >= kThreads - 32) {
+    const float loss = row_loss(a, q, s, ct, -nBt, -nB1, st, s1, rest);
+    if (tid == kThreads - 1) a.loss[q.row] = loss;
   }
   __syncthreads();  // the tokens with a term of their own are written over the pass above
   for (int j = tid; j < k; j += kThreads) {
     const int id = s.id[j];
-    if (id < 0 || id - v0 < lo || id - v0 >= hi) continue;
-    bool first = true;
-    for (int i = 0; i < j && first; ++i) first = s.id[i] != id;
-    if (!first) continue;
-    float p = 0.f;
-    for (int i = j; i < k; ++i)
-      if (s.id[i] == id) p += expf(s.logp[i]);
-    const float d = s.val[j] - mx;
-    float r = qt * exp2f(d * ct) - ks * p;
-    if (hard) {
-      r += q1 * exp2f(d * c1);
-      if (id == tgt) r -= kh;
+    if (id < 0 || id - v0 < lo || id - v0 >= hi || !is_first(s, j)) continue;
+    float p = expf(s.logp[j]);
+    if (s.repeated)
+      for (int i = j + 1; i < k; ++i)
+        if (s.id[i] == id) p += expf(s.logp[i]);
+    float r = qt * ex2(fmaf(s.val[j], ct, nBt)) - ks * p;
+    if (q.hard) {
+      r += q1 * ex2(fmaf(s.val[j], c1, nB1));
+      if (id == q.tgt) r -= kh;
     }
     g[id] = from_f32<T>(r);
   }
-  if (hard && tid == 0 && tgt - v0 >= lo && tgt - v0 < hi) {
-    bool own = true;
-    for (int j = 0; j < k && own; ++j) own = s.id[j] != tgt;
-    if (own) {
-      const float d = s.target_val - mx;
-      g[tgt] = from_f32<T>((soft ? qr * exp2f(d * ct) : 0.f) + q1 * exp2f(d * c1) - kh);
+  if (q.hard && tid < 32 && q.tgt - v0 >= lo && q.tgt - v0 < hi) {
+    bool listed_too = false;
+    for (int j = tid; j < k; j += 32) listed_too |= s.id[j] == q.tgt;
+    if (!__any_sync(0xffffffffu, listed_too) && tid == 0)
+      g[q.tgt] = from_f32<T>(qr * ex2(fmaf(s.target_val, ct, nBt)) + q1 * ex2(fmaf(s.target_val, c1, nB1)) - kh);
+  }
+}
+
+// The loss alone: the row streams through registers, each thread keeping the largest logit it has seen and its sums
+// relative to that.  Where the teacher's remaining mass counts, a bit per token tells which are listed.
+template <typename T, int NEXP>
+__global__ void __launch_bounds__(kThreads, 6) distill_loss_kernel(DistillArgs a, int slice) {
+  pdl_enter();
+  constexpr int E = Chunk<T>::E, U = 4;
+  extern __shared__ uint32_t is_listed[];
+  __shared__ DistillShared s;
+  auto cluster = cg::this_cluster();
+  const int C = (int)cluster.num_blocks(), tid = threadIdx.x;
+  if (C > 1) cluster.sync();
+  const T* x;
+  const Row q = row_of<T>(a, slice, C, (int)cluster.block_rank(), x);
+  const int lo = q.lo, hi = q.hi, v0 = q.v0, k = q.k;
+  if (q.w == 0.f) {
+    if (q.rank == 0 && tid == 0) a.loss[q.row] = 0.f;
+    return;
+  }
+  const bool tail = a.t_lse != nullptr;
+  load_teacher(a, q, x, s);
+  if (tail) {
+    for (int i = tid; i < (slice + 31) / 32; i += kThreads) is_listed[i] = 0;
+    if (tid == 0) s.repeated = 0;
+    __syncthreads();
+    for (int j = tid; j < k; j += kThreads) {
+      const int i = s.id[j] - v0;
+      if (s.id[j] < 0 || i < lo || i >= hi) continue;
+      const uint32_t bit = 1u << (i & 31);
+      if (atomicOr(&is_listed[i >> 5], bit) & bit) s.repeated = 1;
     }
+    __syncthreads();
+  }
+  const float ct = q.inv_t * kLog2e, c1 = kLog2e;
+  const Chunks ch(q, E);
+  float mt = -CUDART_INF_F, nBt = 0.f, nB1 = 0.f, st = 0.f, s1 = 0.f;
+  auto raise = [&](float cm) {  // the largest logit so far
+    if (cm > mt) {
+      const float nt = -(cm * ct), n1 = -(cm * c1);
+      if (mt > -CUDART_INF_F) {
+        st *= ex2(nt - nBt);
+        if (NEXP == 2) s1 *= ex2(n1 - nB1);
+      }
+      mt = cm;
+      nBt = nt;
+      nB1 = n1;
+    }
+  };
+  auto add = [&](uint4 u, int c) {
+    float f[E];
+    Chunk<T>::unpack(u, f);
+    if (NEXP == 2) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) s1 += ex2(fmaf(f[e], c1, nB1));
+    }
+    if (tail) {
+      const uint32_t bits = (is_listed[c * E >> 5] >> (c * E & 31)) & ((1u << E) - 1);
+      if (bits) {
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+          if ((bits >> e) & 1) f[e] = -CUDART_INF_F;
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e) st += ex2(fmaf(f[e], ct, nBt));
+  };
+  const uint4* x4 = reinterpret_cast<const uint4*>(x + v0);  // chunk c, for c in [c0, c1)
+  int c = ch.c0 + tid;
+  for (; c + (U - 1) * kThreads < ch.c1; c += U * kThreads) {
+    uint4 u[U];
+#pragma unroll
+    for (int j = 0; j < U; ++j) u[j] = __ldg(x4 + c + j * kThreads);
+    float cm = chunk_max<T>(u[0]);
+#pragma unroll
+    for (int j = 1; j < U; ++j) cm = fmaxf(cm, chunk_max<T>(u[j]));
+    raise(cm);
+#pragma unroll
+    for (int j = 0; j < U; ++j) add(u[j], c + j * kThreads);
+  }
+  for (; c < ch.c1; c += kThreads) {
+    const uint4 u = __ldg(x4 + c);
+    raise(chunk_max<T>(u));
+    add(u, c);
+  }
+  const int edge = ch.edge(tid);
+  if (edge >= 0) {
+    const float f = to_f32(x[v0 + edge]);
+    raise(f);
+    if (NEXP == 2) s1 += ex2(fmaf(f, c1, nB1));
+    if (!(tail && ((is_listed[edge >> 5] >> (edge & 31)) & 1))) st += ex2(fmaf(f, ct, nBt));
+  }
+  float mx = warp_max(mt);
+  if ((tid & 31) == 0) s.warp[0][tid >> 5] = mx;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, s.warp[0][w]);
+  if (tid >= kThreads - 32) teacher_softmax(a, q, s);
+  if (C > 1) {
+    if (tid < C) *cluster.map_shared_rank(&s.part[0][q.rank], tid) = mx;
+    cluster.sync();
+    for (int r = 0; r < C; ++r) mx = fmaxf(mx, s.part[0][r]);
+  }
+  // all sums relative to the row's largest logit
+  const float Mt = mx * ct, M1 = mx * c1;
+  float listed = 0.f;
+  if (mt > -CUDART_INF_F) {  // else they are 0, or NaN
+    st *= ex2(-nBt - Mt);
+    s1 *= ex2(-nB1 - M1);
+  }
+  if (tail)
+    for (int j = tid; j < k; j += kThreads) {
+      const int i = s.id[j] - v0;
+      if (s.id[j] >= 0 && i >= lo && i < hi && is_first(s, j)) listed += ex2(fmaf(s.val[j], ct, -Mt));
+    }
+  block_sum3(s, st, s1, listed);
+  if (C > 1) {
+    if (tid < C) {
+      *cluster.map_shared_rank(&s.part[1][q.rank], tid) = st;
+      *cluster.map_shared_rank(&s.part[2][q.rank], tid) = s1;
+      *cluster.map_shared_rank(&s.part[3][q.rank], tid) = listed;
+    }
+    cluster.sync();
+    st = s1 = listed = 0.f;
+    for (int r = 0; r < C; ++r) {
+      st += s.part[1][r];
+      s1 += s.part[2][r];
+      listed += s.part[3][r];
+    }
+  }
+  const float rest = st;
+  st += listed;
+  if (NEXP == 1) s1 = st;
+  if (q.rank == 0 && tid < 32) {
+    const float loss = row_loss(a, q, s, ct, Mt, M1, st, s1, rest);
+    if (tid == 0) a.loss[q.row] = loss;
   }
 }
 
@@ -313,13 +583,25 @@ __global__ void __launch_bounds__(256) scale_rows_kernel(T* __restrict__ x, int6
 template <typename T>
 cudaError_t distill_t(const DistillArgs& a, cudaStream_t st) {
   constexpr int E = Chunk<T>::E;
-  auto slice_of = [&](int n) { return (int)(ceil_div(ceil_div((int64_t)a.V + E - 1, n), E) * E); };
+  auto slice_of = [&](int n) { return (int)(ceil_div(ceil_div((int64_t)a.V + E - 1, n), 32) * 32); };
+  // one block per row, more where rows are too few to fill the SMs, or a block's copy of the row is too large for two
+  // blocks to share an SM
+  const int64_t most = a.dlogits ? 104 * 1024 : (int64_t)1 << 40;
   int C = 1;
-  while (C < kMaxCluster && (a.N * C < kSMs || slice_of(C) * (int64_t)sizeof(T) > 104 * 1024)) C *= 2;
+  while (C < kMaxCluster && (a.N * C < kSMs || slice_of(C) * (int64_t)sizeof(T) > most)) C *= 2;
   if (a.N * C > 0x7fffffff) return cudaErrorInvalidValue;
   const int slice = slice_of(C);
-  LaunchScope scope_("distill", st);
-  return launch_clusters(distill_kernel<T>, (unsigned)(a.N * C), C, kThreads, (size_t)slice * sizeof(T), st, a, slice);
+  const unsigned grid = (unsigned)(a.N * C);
+  const bool two = a.targets && a.temperature != 1.f;
+  LaunchScope scope_(a.dlogits ? "distill_grad" : "distill_loss", st);
+  if (a.dlogits) {
+    const size_t smem = (size_t)slice * sizeof(T);
+    return two ? launch_clusters(distill_grad_kernel<T, 2>, grid, C, kThreads, smem, st, a, slice)
+               : launch_clusters(distill_grad_kernel<T, 1>, grid, C, kThreads, smem, st, a, slice);
+  }
+  const size_t smem = a.t_lse ? (size_t)(slice / 32) * 4 : 0;
+  return two ? launch_clusters(distill_loss_kernel<T, 2>, grid, C, kThreads, smem, st, a, slice)
+             : launch_clusters(distill_loss_kernel<T, 1>, grid, C, kThreads, smem, st, a, slice);
 }
 
 }  // namespace
