@@ -1,92 +1,270 @@
 // The scaled token lookup and its gradient, the sum of dout's rows over the positions of each token.
 //
-// Gradient.  group_kernel sorts the positions by token (a counting sort; each block owns the tokens of one remainder
-// and scans all ids, so blocks exchange nothing).  sum_kernel adds up each token's rows in order; a token with more
-// than kPiece positions is summed in pieces cut at multiples of kPiece of the sorted order, spread over the GPU, which
-// join_kernel adds in order.  No float atomics: the result is a function of the inputs alone.
+// Gradient.  The positions are sorted by token while the gradient is cleared: up to kSortMax positions by one cluster's
+// radix sort in shared memory (sort_kernel; the other blocks clear), more by a counting sort over all SMs
+// (group_kernel).  sum_kernel cuts the sorted order into pieces of kPiece positions, a warp each: a group inside a
+// piece is added up and written, a group that crosses a cut leaves a partial sum on each side.  join_kernel adds the
+// partial sums in order.  No float atomics, and every addition has its place: the result is a function of the inputs
+// alone.
+#include <algorithm>
 #include "vocab.cuh"
 
 namespace sdm {
 namespace {
 
-constexpr int kPiece = 32;       // positions summed by one warp
-constexpr int kGroupThreads = 1024, kGroupWarps = kGroupThreads / 32;
+constexpr int kPiece = 16;       // positions summed by one warp (with its two neighbours at most 32)
+constexpr int kLong = 16;        // a group that goes on over so many more pieces is joined by blocks
+constexpr int kSortThreads = 1024, kSortWarps = kSortThreads / 32;
+constexpr int kSortEach = 8192;  // positions of one block of the sorting cluster
+constexpr int kSortMax = 8 * kSortEach;
+constexpr int kGroupThreads = 512, kGroupWarps = kGroupThreads / 32;
+constexpr int kCluster = 8;      // blocks of a cluster
+constexpr int kOwned = 1024;     // tokens of a counting cluster at most: 64 KB of counters
+constexpr int kSteps = 64;       // of 32 ids: so many of a warp are remembered from the count to the placing
 constexpr int kSumThreads = 256, kSumWarps = kSumThreads / 32;
-constexpr int kCols = 256;       // columns of one warp's sum
 
 struct GroupWs {
-  int32_t *order;    // (N) positions, grouped by token
-  int32_t *start;    // (V) where a token's group begins
-  int32_t *count;    // (V)
-  int32_t *hot;      // (owners, tokens of an owner): tokens with more than kPiece positions, by owner
-  int32_t *hot_n;    // (owners)
+  int32_t *order;    // (N) positions, grouped by token, in order within a group
+  int32_t *token;    // (N) their tokens
+  int32_t *crossing; // (pieces) the token whose group begins in the piece and goes on after it, or -1
+  int32_t *hot;      // (pieces / kLong) the pieces in which a long group begins
+  int32_t *hot_n;
   int32_t *total;    // grouped positions
-  float *partial;    // (2 * pieces, d)
+  float *partial;    // (2 * pieces, ldp)
+  int ldp;           // d rounded up to whole 16-byte words
 };
 
-__host__ int owner_bits(int V) {  // 128 blocks, more where an owner's tokens would exceed a block's 1,024 counters
-  int b = 7;
-  while (((int64_t)1 << b) * 1024 < V) ++b;
+__host__ int owner_bits(int V) {  // 32 clusters (256 blocks of two per SM), more where an owner would have too many tokens
+  int b = 5;
+  while (((int64_t)1 << b) * kOwned < V) ++b;
   return b;
 }
 
-size_t carve(GroupWs& w, void* base, int64_t N, int d, int V) {
+size_t carve(GroupWs& w, void* base, int64_t N, int d) {
   size_t off = 0;
   auto take = [&](size_t bytes) {
     char* p = base ? static_cast<char*>(base) + off : nullptr;
     off += (bytes + 255) & ~(size_t)255;
     return p;
   };
-  const int64_t owners = (int64_t)1 << owner_bits(V), per = ceil_div(V, owners);
+  const int64_t pieces = ceil_div(N, kPiece);
+  w.ldp = (d + 3) / 4 * 4;
   w.order = reinterpret_cast<int32_t*>(take(N * 4));
-  w.start = reinterpret_cast<int32_t*>(take((size_t)V * 4));
-  w.count = reinterpret_cast<int32_t*>(take((size_t)V * 4));
-  w.hot = reinterpret_cast<int32_t*>(take(owners * per * 4));
-  w.hot_n = reinterpret_cast<int32_t*>(take(owners * 4));
+  w.token = reinterpret_cast<int32_t*>(take(N * 4));
+  w.crossing = reinterpret_cast<int32_t*>(take(pieces * 4));
+  w.hot = reinterpret_cast<int32_t*>(take((pieces / kLong + 1) * 4));
+  w.hot_n = reinterpret_cast<int32_t*>(take(4));
   w.total = reinterpret_cast<int32_t*>(take(4));
-  w.partial = reinterpret_cast<float*>(take((size_t)2 * ceil_div(N, kPiece) * d * 4));
+  w.partial = reinterpret_cast<float*>(take((size_t)2 * pieces * w.ldp * 4));
   return off;
 }
 
-// Block b owns the tokens v with v mod owners == b (v = local * owners + b).  Each warp counts and later places one
-// stretch of the ids, so the sort is stable.
-__global__ void __launch_bounds__(kGroupThreads) group_kernel(const int32_t* __restrict__ ids, int N, int V, int bits,
-                                                              int per, int padding_id, GroupWs w) {
+// Zeroes `bytes` bytes at `at`: thread t of `threads`.
+__device__ __forceinline__ void clear_bytes(char* at, int64_t bytes, int64_t t, int64_t threads) {
+  const int64_t head = min(bytes, (int64_t)(-reinterpret_cast<uintptr_t>(at) & 15)), words = (bytes - head) / 16;
+  uint4* q = reinterpret_cast<uint4*>(at + head);
+  const uint4 zero = make_uint4(0, 0, 0, 0);
+#pragma unroll 4
+  for (int64_t i = t; i < words; i += threads) q[i] = zero;
+  if (t < head) at[t] = 0;
+  if (t < bytes - head - words * 16) at[head + words * 16 + t] = 0;
+}
+
+// Cluster 0 sorts the positions by token, least significant digits first; the other clusters clear the gradient.  Block
+// r of the sorting cluster holds positions [r * each, +each) of the present order in shared memory, each warp one
+// stretch of them, as token << 16 | position.  A digit's counts by warp, block and cluster give every entry its place
+// in the next order, where it is stored in the block that holds it.  An id to be skipped sorts behind all tokens.
+__global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kSortThreads, 1)
+    sort_kernel(const int32_t* __restrict__ ids, int N, int V, int each, int digit_bits, int passes, int padding_id,
+                GroupWs w, char* grad, int64_t grad_bytes) {
   pdl_enter();
-  extern __shared__ uint32_t count[];  // (warps, per)
-  __shared__ uint32_t warp_sum_[kGroupWarps];
-  __shared__ uint32_t hot_n;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const uint32_t me = blockIdx.x, low = (1u << bits) - 1;
-  for (int i = tid; i < kGroupWarps * per; i += kGroupThreads) count[i] = 0;
-  if (tid == 0) hot_n = 0;
+  if (blockIdx.x >= kCluster) {
+    clear_bytes(grad, grad_bytes, (int64_t)(blockIdx.x - kCluster) * kSortThreads + tid,
+                (int64_t)(gridDim.x - kCluster) * kSortThreads);
+    return;
+  }
+  typedef unsigned long long u64;
+  extern __shared__ u64 entry[];  // two orders of `each`, then the warps' counts of a digit
+  __shared__ uint32_t sum[kSortWarps], here[512], base[512], valid_here;
+  const int digits = 1 << digit_bits;
+  uint32_t* count = reinterpret_cast<uint32_t*>(entry + 2 * each);
+  auto cluster = cooperative_groups::this_cluster();
+  const int rank = (int)cluster.block_rank();
+  const int first = rank * each;                     // of this block's positions
+  const int per_warp = each / kSortWarps, steps = per_warp / 32, e0 = warp * per_warp + lane;
+  if (tid == 0) valid_here = 0;
   __syncthreads();
-  const int seg = (int)(ceil_div(ceil_div(N, kGroupWarps), 32) * 32);
-  const int n0 = (int)min((int64_t)N, (int64_t)warp * seg), n1 = (int)min((int64_t)N, (int64_t)n0 + seg);
+  uint32_t valid = 0;
+#pragma unroll 8
+  for (int i = tid; i < each; i += kSortThreads) {
+    const int n = first + i;
+    int id = n < N ? ids[n] : -1;
+    const bool ok = id >= 0 && id < V && id != padding_id;
+    valid += ok;
+    entry[i] = (u64)(uint32_t)(ok ? id : V) << 16 | (uint32_t)(n & 0xffff);
+  }
+  valid = __reduce_add_sync(0xffffffffu, valid);
+  if (lane == 0) atomicAdd(&valid_here, valid);
+  u64* from = entry;
+  u64* to = entry + each;
+  uint32_t* mine = count + warp * digits;
+  for (int pass = 0; pass < passes; ++pass) {
+    const int shift = 16 + pass * digit_bits;
+    for (int i = tid; i < kSortWarps * digits; i += kSortThreads) count[i] = 0;
+    __syncthreads();
+    uint32_t place[kSortEach / kSortThreads];  // digit, and the place among the warp's entries of that digit
+#pragma unroll
+    for (int s = 0; s < kSortEach / kSortThreads; ++s) {
+      if (s >= steps) break;
+      const uint32_t digit = (uint32_t)(from[e0 + 32 * s] >> shift) & (digits - 1);
+      const uint32_t same = __match_any_sync(0xffffffffu, digit);
+      const uint32_t at = mine[digit];
+      __syncwarp();
+      if (lane == __ffs(same) - 1) mine[digit] = at + __popc(same);
+      __syncwarp();
+      place[s] = digit << 16 | (at + __popc(same & ((1u << lane) - 1)));
+    }
+    __syncthreads();
+    // counts become sums over the warps before
+    for (int g = tid; g < digits; g += kSortThreads) {
+      uint32_t run = 0;
+#pragma unroll 8
+      for (int k = 0; k < kSortWarps; ++k) {
+        const uint32_t c = count[k * digits + g];
+        count[k * digits + g] = run;
+        run += c;
+      }
+      here[g] = run;
+    }
+    cluster.sync();
+    uint32_t all = 0, ahead = 0;
+    if (tid < digits) {
+#pragma unroll
+      for (int r = 0; r < kCluster; ++r) {
+        const uint32_t c = *cluster.map_shared_rank(&here[tid], r);
+        all += c;
+        if (r < rank) ahead += c;
+      }
+    }
+    uint32_t run = all;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t up = __shfl_up_sync(0xffffffffu, run, o);
+      if (lane >= o) run += up;
+    }
+    if (lane == 31) sum[warp] = run;
+    __syncthreads();
+    if (tid < digits) {
+      uint32_t before = run - all + ahead;
+      for (int k = 0; k < warp; ++k) before += sum[k];
+      base[tid] = before;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int s = 0; s < kSortEach / kSortThreads; ++s) {
+      if (s >= steps) break;
+      const uint32_t digit = place[s] >> 16;
+      const uint32_t at = base[digit] + mine[digit] + (place[s] & 0xffffu);
+      const uint32_t r = at / each;
+      *cluster.map_shared_rank(to + (at - r * each), r) = from[e0 + 32 * s];
+    }
+    cluster.sync();
+    u64* t = from;
+    from = to;
+    to = t;
+  }
+  uint32_t total = 0;
+  if (rank == 0 && tid < kCluster) total = *cluster.map_shared_rank(&valid_here, tid);
+  total = __reduce_add_sync(0xffffffffu, total);
+  if (rank == 0 && tid == 0) {
+    *w.total = (int32_t)total;
+    *w.hot_n = 0;
+  }
+  for (int i = tid; i < each; i += kSortThreads) {
+    if (first + i >= N) break;
+    const u64 e = from[i];
+    w.order[first + i] = (int32_t)(e & 0xffff);
+    w.token[first + i] = (int32_t)(e >> 16);
+  }
+  cluster.sync();
+}
+
+// Cluster b owns the tokens v with v mod owners == b (v = local * owners + b).  Each warp counts and later places one stretch of the ids, so the sort is stable; a word of lanes per 32
+// ids tells it which of them to come back to.
+__global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kGroupThreads, 2)
+    group_kernel(const int32_t* __restrict__ ids, int N, int V, int bits, int per, int padding_id, GroupWs w, char* grad,
+                 int64_t grad_bytes) {
+  pdl_enter();
+  const uint32_t me = blockIdx.x / kCluster, low = (1u << bits) - 1;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  extern __shared__ uint32_t count[];  // (warps, per)
+  __shared__ uint32_t size_here[kOwned];  // of each token in this block's ids
+  __shared__ uint32_t warp_sum_[kGroupWarps], below_here;
+  __shared__ uint32_t seen[kGroupWarps][kSteps];  // lanes of a step whose id is owned
+  auto cluster = cooperative_groups::this_cluster();
+  const int rank = (int)cluster.block_rank();
+  for (int i = tid; i < kGroupWarps * per; i += kGroupThreads) count[i] = 0;
+  clear_bytes(grad, grad_bytes, (int64_t)blockIdx.x * kGroupThreads + tid, (int64_t)gridDim.x * kGroupThreads);
+  __syncthreads();
+  const int seg = (int)(ceil_div(ceil_div(N, kGroupWarps * kCluster), 32) * 32);
+  const int n0 = (int)min((int64_t)N, (int64_t)(rank * kGroupWarps + warp) * seg), n1 = (int)min((int64_t)N, (int64_t)n0 + seg);
+  const int steps = (n1 - n0 + 31) / 32;
   uint32_t* mine = count + warp * per;
   uint32_t below = 0;
-  for (int n = n0 + lane; n < n1; n += 32) {
-    const int id = ids[n];
-    if (id < 0 || id >= V || id == padding_id) continue;
-    const uint32_t owner = (uint32_t)id & low;
-    below += owner < me;
-    if (owner == me) atomicAdd(&mine[id >> bits], 1u);
+  constexpr int U = 8;
+  for (int s0 = 0; s0 < steps; s0 += U) {
+    int id[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int n = n0 + (s0 + u) * 32 + lane;
+      id[u] = n < n1 ? ids[n] : -1;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const bool ok = id[u] >= 0 && id[u] < V && id[u] != padding_id;
+      const uint32_t owner = (uint32_t)id[u] & low;
+      below += ok && owner < me;
+      const bool owned = ok && owner == me;
+      const uint32_t lanes = __ballot_sync(0xffffffffu, owned);
+      if (owned) atomicAdd(&mine[id[u] >> bits], 1u);
+      if (lane == 0 && s0 + u < kSteps) seen[warp][s0 + u] = lanes;
+    }
   }
   below = __reduce_add_sync(0xffffffffu, below);
   if (lane == 0) warp_sum_[warp] = below;
   __syncthreads();
-  uint32_t base = 0;
-  for (int i = 0; i < kGroupWarps; ++i) base += warp_sum_[i];
-  __syncthreads();
-  // the group of local token tid: its size, then its start
-  uint32_t size = 0;
-  if (tid < per)
+  if (tid == 0) {
+    uint32_t b = 0;
+    for (int i = 0; i < kGroupWarps; ++i) b += warp_sum_[i];
+    below_here = b;
+  }
+  for (int t = tid; t < per; t += kGroupThreads) {  // counts become offsets within the block's share of the token
+    uint32_t size = 0;
+#pragma unroll
     for (int i = 0; i < kGroupWarps; ++i) {
-      const uint32_t c = count[i * per + tid];
-      count[i * per + tid] = size;
+      const uint32_t c = count[i * per + t];
+      count[i * per + t] = size;
       size += c;
     }
-  uint32_t run = size;
+    size_here[t] = size;
+  }
+  cluster.sync();
+  // two neighbouring tokens per thread: their sizes in the whole cluster and in the blocks before this one
+  uint32_t size[2] = {0, 0}, ahead[2] = {0, 0}, base = 0;
+#pragma unroll
+  for (int r = 0; r < kCluster; ++r) {
+    base += *cluster.map_shared_rank(&below_here, r);
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const uint32_t c = 2 * tid + e < per ? *cluster.map_shared_rank(&size_here[2 * tid + e], r) : 0u;
+      size[e] += c;
+      if (r < rank) ahead[e] += c;
+    }
+  }
+  cluster.barrier_arrive();  // this block reads no other one from here on
+  const uint32_t both = size[0] + size[1];
+  uint32_t run = both;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const uint32_t up = __shfl_up_sync(0xffffffffu, run, o);
@@ -94,37 +272,66 @@ __global__ void __launch_bounds__(kGroupThreads) group_kernel(const int32_t* __r
   }
   if (lane == 31) warp_sum_[warp] = run;
   __syncthreads();
-  uint32_t first = base + run - size;
-  for (int i = 0; i < warp; ++i) first += warp_sum_[i];
-  if (tid < per) {
-    const int64_t v = ((int64_t)tid << bits) + me;
-    if (v < V) {
-      w.start[v] = (int32_t)first;
-      w.count[v] = (int32_t)size;
-      if (size > kPiece) w.hot[(int64_t)me * per + atomicAdd(&hot_n, 1u)] = (int32_t)v;
+  uint32_t first = base + run - both;
+#pragma unroll
+  for (int i = 0; i < kGroupWarps; ++i) first += i < warp ? warp_sum_[i] : 0u;
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    const int t = 2 * tid + e;
+    if (t < per) {
+#pragma unroll
+      for (int i = 0; i < kGroupWarps; ++i) count[i * per + t] += first + ahead[e];
     }
-    for (int i = 0; i < kGroupWarps; ++i) count[i * per + tid] += first;
+    first += size[e];
   }
-  if (me == low && tid == kGroupThreads - 1) *w.total = (int32_t)(first + size);
+  if (me == low && rank == 0 && tid == kGroupThreads - 1) {
+    *w.total = (int32_t)first;
+    *w.hot_n = 0;
+  }
   __syncthreads();
-  if (tid == 0) w.hot_n[me] = (int32_t)hot_n;
-  for (int nb = n0; nb < n1; nb += 32) {
-    const int n = nb + lane;
-    const int id = n < n1 ? ids[n] : -1;
+  auto place = [&](int n, int id) {
     const bool owned = id >= 0 && id < V && id != padding_id && ((uint32_t)id & low) == me;
-    if (!__any_sync(0xffffffffu, owned)) continue;
+    if (!__any_sync(0xffffffffu, owned)) return;
     const int local = owned ? id >> bits : -1;
     const uint32_t same = __match_any_sync(0xffffffffu, local);
-    const int rank = __popc(same & ((1u << lane) - 1));
+    const int rank_ = __popc(same & ((1u << lane) - 1));
     uint32_t at = 0;
-    if (owned) at = mine[local] + rank;
+    if (owned) at = mine[local] + rank_;
     __syncwarp();
     if (owned) {
       w.order[at] = n;
-      if (rank == 0) mine[local] += __popc(same);
+      w.token[at] = id;
+      if (rank_ == 0) mine[local] += __popc(same);
     }
     __syncwarp();
+  };
+#pragma unroll 1
+  for (int half = 0; half < kSteps; half += 32) {
+    uint32_t todo = __ballot_sync(0xffffffffu, half + lane < steps && seen[warp][half + lane] != 0);
+    while (todo) {  // eight steps' ids at a time
+      int n[U], id[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        n[u] = todo ? n0 + (half + __ffs(todo) - 1) * 32 + lane : n1;
+        todo &= todo - 1;
+        id[u] = n[u] < n1 ? ids[n[u]] : -1;
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) place(n[u], id[u]);
+    }
   }
+#pragma unroll 1
+  for (int s = kSteps; s < steps; s += U) {
+    int id[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int n = n0 + (s + u) * 32 + lane;
+      id[u] = n < n1 ? ids[n] : -1;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) place(n0 + (s + u) * 32 + lane, id[u]);
+  }
+  cluster.barrier_wait();
 }
 
 template <int BYTES> struct Word;
@@ -139,125 +346,190 @@ struct Pack {
   __device__ float get(int e) const { return to_f32(reinterpret_cast<const T*>(&u)[e]); }
 };
 
-// One warp's sum over positions order[j0 .. j1) of the 256 columns from c0 on; lane's columns are c0 + VEC * (lane +
-// 32 q) + e.
-template <typename T, int VEC>
-struct Sum {
-  static constexpr int NQ = kCols / (32 * VEC);
-  float acc[NQ][VEC];
-
-  __device__ void run(const T* __restrict__ dout, int64_t ld, const int32_t* __restrict__ order, int j0, int j1,
-                      int c0, int d) {
-    const int lane = threadIdx.x & 31;
-#pragma unroll
-    for (int q = 0; q < NQ; ++q)
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) acc[q][e] = 0.f;
-    for (int jb = j0; jb < j1; jb += 32) {
-      const int n = min(32, j1 - jb);
-      const int pos = lane < n ? order[jb + lane] : 0;
-#pragma unroll 4
-      for (int j = 0; j < n; ++j) {
-        const T* r = dout + (int64_t)__shfl_sync(0xffffffffu, pos, j) * ld;
-#pragma unroll
-        for (int q = 0; q < NQ; ++q) {
-          const int c = c0 + VEC * (lane + 32 * q);
-          if (c < d) {
-            const Pack<T, VEC> p = {__ldg(reinterpret_cast<const typename Word<VEC * sizeof(T)>::type*>(r + c))};
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) acc[q][e] += p.get(e);
-          }
-        }
-      }
-    }
-  }
-};
-
+// VEC sums times scale (plus the old gradient) to `at`, aligned to their size or 16 bytes.
 template <typename G, int VEC>
 __device__ __forceinline__ void store_grad(G* at, const float* v, float scale, int accumulate) {
+  constexpr int BYTES = VEC * sizeof(G) > 16 ? 16 : VEC * sizeof(G), N = BYTES / sizeof(G);
+  typedef typename Word<BYTES>::type W;
 #pragma unroll
-  for (int e = 0; e < VEC; ++e) {
-    const float s = v[e] * scale;
-    at[e] = from_f32<G>(accumulate ? to_f32(at[e]) + s : s);
+  for (int k = 0; k < VEC; k += N) {
+    union {
+      W u;
+      G g[N];
+    } y;
+    if (accumulate) y.u = *reinterpret_cast<const W*>(at + k);
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const float s = v[k + e] * scale;
+      y.g[e] = from_f32<G>(accumulate ? to_f32(y.g[e]) + s : s);
+    }
+    *reinterpret_cast<W*>(at + k) = y.u;
   }
 }
 
-// Items: (token, 256 columns) for every token, then (piece, 256 columns).
-template <typename T, typename G, int VEC>
-__global__ void __launch_bounds__(kSumThreads) sum_kernel(const int32_t* __restrict__ ids, const T* __restrict__ dout,
-                                                          int64_t ld, int d, int V, int col_blocks, int64_t items,
-                                                          float scale, int accumulate, GroupWs w,
-                                                          G* __restrict__ grad) {
+// Warp (piece, 32 VEC NQ columns): the sums of the piece's groups.  A lane's columns are c + 32 VEC q + e.  32 elements
+// of a lane are in flight: several columns of a few rows, or of more rows where the pieces are few.
+template <typename T, typename G, int VEC, int NQ>
+__global__ void __launch_bounds__(kSumThreads, sizeof(T) == 2 ? 4 : 3) sum_kernel(const T* __restrict__ dout,
+                                                              int64_t ld, int d,
+                                                              int col_blocks, int64_t items, float scale,
+                                                              int accumulate, GroupWs w, G* __restrict__ grad) {
   pdl_enter();
+  constexpr int kRows = 32 / (VEC * NQ) < kPiece ? 32 / (VEC * NQ) : kPiece;
+  typedef typename Word<VEC * sizeof(T)>::type W;
   const int64_t item = (int64_t)blockIdx.x * kSumWarps + (threadIdx.x >> 5);
   if (item >= items) return;
   const int lane = threadIdx.x & 31;
-  const int64_t what = item / col_blocks;
-  const int c0 = (int)(item % col_blocks) * kCols;
-  Sum<T, VEC> s;
-  if (what < V) {
-    const int n = w.count[what];
-    if (n > kPiece || (n == 0 && accumulate)) return;
-    const int j0 = w.start[what];
-    s.run(dout, ld, w.order, j0, j0 + n, c0, d);
-#pragma unroll
-    for (int q = 0; q < Sum<T, VEC>::NQ; ++q) {
-      const int c = c0 + VEC * (lane + 32 * q);
-      if (c < d) store_grad<G, VEC>(grad + what * d + c, s.acc[q], scale, accumulate);
-    }
+  const int piece = (int)(col_blocks == 1 ? item : item / col_blocks);
+  const int c = (int)(item - (int64_t)piece * col_blocks) * (32 * VEC * NQ) + VEC * lane;
+  const int total = *w.total, j0 = piece * kPiece, n = min(kPiece, total - j0);
+  if (n <= 0) {
+    if (c == 0) w.crossing[piece] = -1;
     return;
   }
-  const int64_t piece = what - V;
-  const int total = *w.total;
-  const int j0 = (int)(piece * kPiece), j1 = min(total, j0 + kPiece);
-  if (j0 >= j1) return;
-  const int a = ids[w.order[j0]], b = ids[w.order[j1 - 1]];
+  // lane l: the position before the piece (l = 0), the piece's (1 .. n), and the one after it (n + 1)
+  const int j = j0 - 1 + lane;
+  const bool there = lane <= n + 1 && j >= 0 && j < total;
+  const int pos = there ? w.order[j] : -1, id = there ? w.token[j] : -1;
+  const int later = j0 + kLong * kPiece < total ? w.token[j0 + kLong * kPiece] : -1;
+  const int before = __shfl_sync(0xffffffffu, id, 0), after = __shfl_sync(0xffffffffu, id, n + 1);
+  const uint32_t ends = __ballot_sync(0xffffffffu, id != __shfl_down_sync(0xffffffffu, id, 1) || lane == n) >> 1;
+  float acc[NQ][VEC];
 #pragma unroll
-  for (int side = 0; side < 2; ++side) {  // the group that the piece begins in, and the one that begins in it
-    const int v = side ? b : a;
-    if (side && b == a) break;
-    const int n = w.count[v];
-    if (n <= kPiece) continue;
-    const int g0 = w.start[v], g1 = g0 + n;
-    s.run(dout, ld, w.order, max(g0, j0), min(g1, j1), c0, d);
-    float* out = w.partial + (2 * piece + side) * d;
+  for (int q = 0; q < NQ; ++q)
 #pragma unroll
-    for (int q = 0; q < Sum<T, VEC>::NQ; ++q) {
-      const int c = c0 + VEC * (lane + 32 * q);
-      if (c < d) {
+    for (int e = 0; e < VEC; ++e) acc[q][e] = 0.f;
+  bool head = true;  // in the group that holds the piece's first position
+#pragma unroll 1
+  for (int i0 = 0; i0 < n; i0 += kRows) {
+    Pack<T, VEC> p[kRows][NQ];
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) out[c + e] = s.acc[q][e];
+    for (int k = 0; k < kRows; ++k) {
+      const int at = __shfl_sync(0xffffffffu, pos, min(i0 + k, n - 1) + 1);
+      const T* r = dout + (int64_t)at * ld + c;
+#pragma unroll
+      for (int q = 0; q < NQ; ++q)
+        if (c + 32 * VEC * q < d && i0 + k < n) p[k][q].u = __ldg(reinterpret_cast<const W*>(r + 32 * VEC * q));
+    }
+#pragma unroll
+    for (int k = 0; k < kRows; ++k) {
+      const int i = i0 + k;
+      if (i >= n) break;
+#pragma unroll
+      for (int q = 0; q < NQ; ++q)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) acc[q][e] += p[k][q].get(e);
+      if ((ends >> i) & 1) {
+        const int v = __shfl_sync(0xffffffffu, id, i + 1);
+        const bool came = head && v == before, goes = i == n - 1 && v == after, crosses = came || goes;
+        if (i == n - 1 && c == 0) {
+          const bool long_ = goes && !came && v == later;
+          if (long_) w.hot[atomicAdd(w.hot_n, 1)] = piece;  // in any order: each is joined by itself
+          w.crossing[piece] = goes && !came && !long_ ? v : -1;
+        }
+        if (crosses) {
+          float* out = w.partial + (2 * (int64_t)piece + (head ? 0 : 1)) * w.ldp + c;
+#pragma unroll
+          for (int q = 0; q < NQ; ++q)
+            if (c + 32 * VEC * q < d) store_grad<float, VEC>(out + 32 * VEC * q, acc[q], 1.f, 0);
+        } else {
+          G* out = grad + (int64_t)v * d + c;
+#pragma unroll
+          for (int q = 0; q < NQ; ++q)
+            if (c + 32 * VEC * q < d) store_grad<G, VEC>(out + 32 * VEC * q, acc[q], scale, accumulate);
+        }
+#pragma unroll
+        for (int q = 0; q < NQ; ++q)
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) acc[q][e] = 0.f;
+        head = false;
       }
     }
   }
 }
 
-// Block (owner, 32 columns): adds up the pieces of the owner's large groups.  Warp w takes every eighth piece, and the
-// warps' sums are added in order.
 template <typename G>
-__global__ void __launch_bounds__(256) join_kernel(int d, int per, float scale, int accumulate, GroupWs w,
-                                                   G* __restrict__ grad) {
+__device__ __forceinline__ void store_joined(G* row, int c, int d, float4 s, float scale, int accumulate) {
+  const float v[4] = {s.x, s.y, s.z, s.w};
+  if (d % 4 == 0 && (reinterpret_cast<uintptr_t>(row) & (4 * sizeof(G) - 1)) == 0) {
+    store_grad<G, 4>(row + c, v, scale, accumulate);
+  } else {
+    for (int e = 0; e < 4 && c + e < d; ++e) store_grad<G, 1>(row + c + e, v + e, scale, accumulate);
+  }
+}
+
+__device__ __forceinline__ void add4(float4& a, const float4& b) {
+  a.x += b.x;
+  a.y += b.y;
+  a.z += b.z;
+  a.w += b.w;
+}
+
+// The first hot_blocks * cols blocks: 128 columns of the long groups i, i + hot_blocks, ...; warp w takes every
+// sixteenth piece, and the warps' sums are added in order.  The others, a warp per piece: the group that begins in the
+// piece and goes on over fewer than kLong more.
+constexpr int kJoinWarps = 16;
+template <typename G>
+__global__ void __launch_bounds__(32 * kJoinWarps, 2) join_kernel(int d, int pieces, int hot_blocks, int cols,
+                                                                  float scale, int accumulate, GroupWs w,
+                                                                  G* __restrict__ grad) {
   pdl_enter();
-  __shared__ float part[8][32];
+  __shared__ float4 part[kJoinWarps][32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int n = w.hot_n[blockIdx.x];
-  const int c = blockIdx.y * 32 + lane;
-  for (int i = 0; i < n; ++i) {
-    const int64_t v = w.hot[(int64_t)blockIdx.x * per + i];
-    const int g0 = w.start[v], g1 = g0 + w.count[v];
-    const int m0 = g0 / kPiece, m1 = (g1 - 1) / kPiece;
-    float sum = 0.f;
+  const int total = *w.total;
+  // a group's partial sums: slot 1 of the piece it begins in (slot 0 if it begins with the piece), slot 0 of the others
+  if ((int)blockIdx.x >= hot_blocks * cols) {
+    const int m = ((int)blockIdx.x - hot_blocks * cols) * kJoinWarps + warp;
+    if (m >= pieces) return;
+    const int v = w.crossing[m];
+    if (v < 0) return;
+    const int at = (m + 1 + lane) * kPiece;  // the first position of a later piece
+    const uint32_t in = __ballot_sync(0xffffffffu, lane < kLong && at < total && w.token[min(at, total - 1)] == v);
+    const int more = __ffs(~in) - 1;
+    const float* first = w.partial + (2 * (int64_t)m + (w.token[m * kPiece] != v ? 1 : 0)) * w.ldp;
+    const float* rest = w.partial + 2 * (int64_t)(m + 1) * w.ldp;
+    constexpr int NC = 6;  // 768 columns in flight
+    for (int c0 = lane * 4; c0 < d; c0 += 128 * NC) {
+      float4 sum[NC];
+#pragma unroll
+      for (int q = 0; q < NC; ++q)
+        if (c0 + 128 * q < d) sum[q] = *reinterpret_cast<const float4*>(first + c0 + 128 * q);
+#pragma unroll 2
+      for (int k = 0; k < more; ++k) {
+#pragma unroll
+        for (int q = 0; q < NC; ++q)
+          if (c0 + 128 * q < d) add4(sum[q], *reinterpret_cast<const float4*>(rest + (int64_t)2 * k * w.ldp + c0 + 128 * q));
+      }
+#pragma unroll
+      for (int q = 0; q < NC; ++q)
+        if (c0 + 128 * q < d) store_joined(grad + (int64_t)v * d, c0 + 128 * q, d, sum[q], scale, accumulate);
+    }
+    return;
+  }
+  const int c = ((int)blockIdx.x % cols) * 128 + lane * 4, hot_n = *w.hot_n;
+  for (int i = (int)blockIdx.x / cols; i < hot_n; i += hot_blocks) {
+    const int m = w.hot[i];
+    const int v = w.token[(m + 1) * kPiece];
+    int more = 0;  // the pieces after m that begin with v
+    for (int k0 = m + 1; k0 < pieces; k0 += 32 * kJoinWarps) {
+      const int k = k0 + (int)threadIdx.x;
+      const int n = __syncthreads_count(k < pieces && k * kPiece < total && w.token[min(k * kPiece, total - 1)] == v);
+      more += n;
+      if (n < 32 * kJoinWarps) break;
+    }
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
     if (c < d) {
-#pragma unroll 4
-      for (int m = m0 + warp; m <= m1; m += 8)
-        sum += w.partial[(2 * (int64_t)m + (g0 > m * kPiece ? 1 : 0)) * d + c];
+      const int slot = w.token[m * kPiece] != v ? 1 : 0;
+#pragma unroll 8
+      for (int k = warp; k <= more; k += kJoinWarps)
+        add4(sum, *reinterpret_cast<const float4*>(w.partial + (2 * (int64_t)(m + k) + (k == 0 ? slot : 0)) * w.ldp + c));
     }
     part[warp][lane] = sum;
     __syncthreads();
     if (warp == 0 && c < d) {
 #pragma unroll
-      for (int k = 1; k < 8; ++k) sum += part[k][lane];
-      store_grad<G, 1>(grad + v * d + c, &sum, scale, accumulate);
+      for (int k = 1; k < kJoinWarps; ++k) add4(sum, part[k][lane]);
+      store_joined(grad + (int64_t)v * d, c, d, sum, scale, accumulate);
     }
     __syncthreads();
   }
@@ -318,52 +590,80 @@ cudaError_t lookup_t(const int32_t* ids, const T* emb, int64_t N, int d, int V, 
   }
 }
 
-template <typename T, typename G, int VEC>
-cudaError_t launch_sum(const int32_t* ids, const T* dout, int64_t ld, int64_t N, int d, int V, float scale,
-                       int accumulate, const GroupWs& w, G* grad, cudaStream_t st) {
-  const int col_blocks = (int)ceil_div(d, kCols);
-  const int64_t items = (V + ceil_div(N, kPiece)) * col_blocks, blocks = ceil_div(items, kSumWarps);
+template <typename T, typename G, int VEC, int NQ>
+cudaError_t launch_sum_q(const T* dout, int64_t ld, int64_t N, int d, float scale, int accumulate,
+                         const GroupWs& w, G* grad, cudaStream_t st) {
+  const int col_blocks = (int)ceil_div(d, 32 * VEC * NQ);
+  const int64_t items = ceil_div(N, kPiece) * col_blocks, blocks = ceil_div(items, kSumWarps);
   if (blocks > 0x7fffffff) return cudaErrorInvalidValue;
   LaunchScope scope_("embed_grad_sum", st);
-  return launch_k(sum_kernel<T, G, VEC>, dim3((unsigned)blocks), dim3(kSumThreads), 0, st, ids, dout, ld, d, V,
+  return launch_k(sum_kernel<T, G, VEC, NQ>, dim3((unsigned)blocks), dim3(kSumThreads), 0, st, dout, ld, d,
                   col_blocks, items, scale, accumulate, w, grad);
+}
+template <typename T, typename G, int VEC>
+cudaError_t launch_sum(const T* dout, int64_t ld, int64_t N, int d, float scale, int accumulate,
+                       const GroupWs& w, G* grad, cudaStream_t st) {
+  // 256 columns per warp while that still gives the SMs a warp per scheduler slot, else as few as a lane loads at once
+  if (VEC == 8 || ceil_div(N, kPiece) * ceil_div(d, 256) >= kSMs * 24)
+    return launch_sum_q<T, G, VEC, 8 / VEC>(dout, ld, N, d, scale, accumulate, w, grad, st);
+  return launch_sum_q<T, G, VEC, 1>(dout, ld, N, d, scale, accumulate, w, grad, st);
 }
 
 template <typename T, typename G>
 cudaError_t grad_t(const int32_t* ids, const T* dout, int64_t ld, int64_t N, int d, int V, float scale,
                    int padding_id, int accumulate, G* grad, void* ws, cudaStream_t st) {
   GroupWs w;
-  carve(w, ws, N, d, V);
-  const int bits = owner_bits(V), owners = 1 << bits, per = (int)ceil_div(V, owners);
-  const size_t smem = (size_t)kGroupWarps * per * 4;
-  cudaError_t e = cudaFuncSetAttribute(group_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kGroupWarps * 1024 * 4);
-  if (e != cudaSuccess) return e;
-  {
-    LaunchScope scope_("embed_grad_group", st);
-    e = launch_k(group_kernel, dim3((unsigned)owners), dim3(kGroupThreads), smem, st, ids, (int)N, V, bits, per,
-                 padding_id, w);
+  carve(w, ws, N, d);
+  const int64_t bytes = accumulate ? 0 : (int64_t)V * d * sizeof(G);
+  cudaError_t e;
+  // One cluster sorts 65,536 positions in less time than clearing a table of 100 MB takes the others; the counting
+  // sort's cost grows with the table instead (at 5,000 positions of 50,021 tokens it took SORT_NOTE).
+  if (N <= kSortMax) {
+    int id_bits = 1;
+    while (((int64_t)1 << id_bits) <= V) ++id_bits;  // V itself stands for an id to be skipped
+    const int passes = (id_bits + 8) / 9, digit_bits = (id_bits + passes - 1) / passes;
+    const int each = (int)(ceil_div(std::max(N, (int64_t)1), kCluster * kSortThreads) * kSortThreads);
+    const size_t smem = (size_t)each * 16 + ((size_t)kSortWarps << digit_bits) * 4;
+    e = cudaFuncSetAttribute(sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSortEach * 16 + kSortWarps * 512 * 4);
     if (e != cudaSuccess) return e;
+    const int64_t clear = std::min((int64_t)2 * kSMs / kCluster, ceil_div(bytes, 16 * kSortThreads * kCluster));
+    LaunchScope scope_("embed_grad_sort", st);
+    e = launch_k(sort_kernel, dim3((unsigned)((1 + clear) * kCluster)), dim3(kSortThreads), smem, st, ids, (int)N, V, each,
+                 digit_bits, passes, padding_id, w, reinterpret_cast<char*>(grad), bytes);
+  } else {
+    const int bits = owner_bits(V), owners = 1 << bits, per = (int)ceil_div(V, owners);
+    e = cudaFuncSetAttribute(group_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kGroupWarps * kOwned * 4);
+    if (e != cudaSuccess) return e;
+    LaunchScope scope_("embed_grad_group", st);
+    e = launch_k(group_kernel, dim3((unsigned)(owners * kCluster)), dim3(kGroupThreads), (size_t)kGroupWarps * per * 4, st,
+                 ids, (int)N, V, bits, per, padding_id, w, reinterpret_cast<char*>(grad), bytes);
   }
+  if (e != cudaSuccess || N == 0) return e;
   switch (vec_of(16 / sizeof(T), d, ld, dout, sizeof(T), grad, sizeof(G))) {
     case 8:
-      if constexpr (sizeof(T) == 2) e = launch_sum<T, G, 8>(ids, dout, ld, N, d, V, scale, accumulate, w, grad, st);
+      if constexpr (sizeof(T) == 2) e = launch_sum<T, G, 8>(dout, ld, N, d, scale, accumulate, w, grad, st);
       else e = cudaErrorInvalidValue;
       break;
-    case 4: e = launch_sum<T, G, 4>(ids, dout, ld, N, d, V, scale, accumulate, w, grad, st); break;
-    case 2: e = launch_sum<T, G, 2>(ids, dout, ld, N, d, V, scale, accumulate, w, grad, st); break;
-    default: e = launch_sum<T, G, 1>(ids, dout, ld, N, d, V, scale, accumulate, w, grad, st); break;
+    case 4: e = launch_sum<T, G, 4>(dout, ld, N, d, scale, accumulate, w, grad, st); break;
+    case 2: e = launch_sum<T, G, 2>(dout, ld, N, d, scale, accumulate, w, grad, st); break;
+    default: e = launch_sum<T, G, 1>(dout, ld, N, d, scale, accumulate, w, grad, st); break;
   }
   if (e != cudaSuccess || N <= kPiece) return e;
+  const int pieces = (int)ceil_div(N, kPiece), cols = (int)ceil_div(d, 128);
+  const int hot_blocks = std::min(pieces / kLong + 1, 64);
+  const int64_t blocks = (int64_t)hot_blocks * cols + ceil_div(pieces, kJoinWarps);
+  if (blocks > 0x7fffffff) return cudaErrorInvalidValue;
   LaunchScope scope_("embed_grad_join", st);
-  return launch_k(join_kernel<G>, dim3((unsigned)owners, (unsigned)ceil_div(d, 32)), dim3(256), 0, st, d, per, scale,
+  return launch_k(join_kernel<G>, dim3((unsigned)blocks), dim3(32 * kJoinWarps), 0, st, d, pieces, hot_blocks, cols, scale,
                   accumulate, w, grad);
 }
 
 }  // namespace
 
 size_t embed_grad_workspace_bytes(int64_t N, int d, int V) {
+  (void)V;
   GroupWs w;
-  return carve(w, nullptr, N, d, V);
+  return carve(w, nullptr, N, d);
 }
 
 cudaError_t launch_embed_scaled(const int32_t* ids, const void* emb, int64_t N, int d, int V, float scale, int dtype,

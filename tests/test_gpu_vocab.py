@@ -476,7 +476,9 @@ def grad64(ids, dout, V, scale, skip):
 @pytest.mark.parametrize("N,V,d,kind", [(0, 5, 8, "any"), (1, 1, 1, "any"), (1, 200, 768, "any"), (33, 1, 16, "any"),
                                         (31, 3, 24, "any"), (500, 40, 33, "any"), (3000, 2000, 64, "zipf"),
                                         (5000, 300, 330, "zipf"), (4096, 130, 258, "runs"), (2000, 70000, 12, "any"),
-                                        (1037, 9, 768, "one"), (700, 140000, 8, "any")])
+                                        (1037, 9, 768, "one"), (700, 140000, 8, "any"), (300, 5, 20, "one"),
+                                        (250, 70, 6, "one"), (65536, 1000, 8, "zipf"), (65537, 40000, 4, "any"),
+                                        (70001, 300, 8, "zipf"), (80000, 12, 5, "one")])
 def test_embed_grad(cuda_ok, dt, gdt, N, V, d, kind):
     rng = np.random.default_rng(N + V)
     if kind == "zipf":
