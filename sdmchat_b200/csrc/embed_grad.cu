@@ -15,8 +15,9 @@ namespace {
 constexpr int kPiece = 16;       // positions summed by one warp (with its two neighbours at most 32)
 constexpr int kLong = 16;        // a group that goes on over so many more pieces is joined by blocks
 constexpr int kSortThreads = 1024, kSortWarps = kSortThreads / 32;
-constexpr int kSortEach = 8192;  // positions of one block of the sorting cluster
-constexpr int kSortMax = 8 * kSortEach;
+constexpr int kSortCluster = 16; // blocks of the sorting cluster (more than the portable 8)
+constexpr int kSortEach = 4096;  // positions of one of them
+constexpr int kSortMax = kSortCluster * kSortEach;
 constexpr int kGroupThreads = 512, kGroupWarps = kGroupThreads / 32;
 constexpr int kCluster = 8;      // blocks of a cluster
 constexpr int kOwned = 1024;     // tokens of a counting cluster at most: 64 KB of counters
@@ -70,23 +71,34 @@ __device__ __forceinline__ void clear_bytes(char* at, int64_t bytes, int64_t t, 
   if (t < bytes - head - words * 16) at[head + words * 16 + t] = 0;
 }
 
+// The lanes of the warp with this lane's digit, a ballot per bit (a digit has 9 at most).
+__device__ __forceinline__ uint32_t same_digit(uint32_t digit) {
+  uint32_t same = 0xffffffffu;
+#pragma unroll
+  for (int b = 0; b < 9; ++b) {
+    const uint32_t set = __ballot_sync(0xffffffffu, (digit >> b) & 1);
+    same &= (digit >> b) & 1 ? set : ~set;
+  }
+  return same;
+}
+
 // Cluster 0 sorts the positions by token, least significant digits first; the other clusters clear the gradient.  Block
 // r of the sorting cluster holds positions [r * each, +each) of the present order in shared memory, each warp one
 // stretch of them, as token << 16 | position.  A digit's counts by warp, block and cluster give every entry its place
 // in the next order, where it is stored in the block that holds it.  An id to be skipped sorts behind all tokens.
-__global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kSortThreads, 1)
+__global__ void __launch_bounds__(kSortThreads, 1)
     sort_kernel(const int32_t* __restrict__ ids, int N, int V, int each, int digit_bits, int passes, int padding_id,
                 GroupWs w, char* grad, int64_t grad_bytes) {
   pdl_enter();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  if (blockIdx.x >= kCluster) {
-    clear_bytes(grad, grad_bytes, (int64_t)(blockIdx.x - kCluster) * kSortThreads + tid,
-                (int64_t)(gridDim.x - kCluster) * kSortThreads);
+  if (blockIdx.x >= kSortCluster) {
+    clear_bytes(grad, grad_bytes, (int64_t)(blockIdx.x - kSortCluster) * kSortThreads + tid,
+                (int64_t)(gridDim.x - kSortCluster) * kSortThreads);
     return;
   }
   typedef unsigned long long u64;
   extern __shared__ u64 entry[];  // two orders of `each`, then the warps' counts of a digit
-  __shared__ uint32_t sum[kSortWarps], here[512], base[512], valid_here;
+  __shared__ uint32_t sum[kSortWarps], sum_own[kSortWarps], here[512], base[512], base_own[512], valid_here;
   const int digits = 1 << digit_bits;
   uint32_t* count = reinterpret_cast<uint32_t*>(entry + 2 * each);
   auto cluster = cooperative_groups::this_cluster();
@@ -113,12 +125,15 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kSortThreads,
     const int shift = 16 + pass * digit_bits;
     for (int i = tid; i < kSortWarps * digits; i += kSortThreads) count[i] = 0;
     __syncthreads();
-    uint32_t place[kSortEach / kSortThreads];  // digit, and the place among the warp's entries of that digit
+    constexpr int S = kSortEach / kSortThreads;
+    uint32_t place[S];  // digit, and the place among the warp's entries of that digit
+    u64 held[S];
 #pragma unroll
-    for (int s = 0; s < kSortEach / kSortThreads; ++s) {
+    for (int s = 0; s < S; ++s) {
       if (s >= steps) break;
-      const uint32_t digit = (uint32_t)(from[e0 + 32 * s] >> shift) & (digits - 1);
-      const uint32_t same = __match_any_sync(0xffffffffu, digit);
+      held[s] = from[e0 + 32 * s];
+      const uint32_t digit = (uint32_t)(held[s] >> shift) & (digits - 1);
+      const uint32_t same = same_digit(digit);
       const uint32_t at = mine[digit];
       __syncwarp();
       if (lane == __ffs(same) - 1) mine[digit] = at + __popc(same);
@@ -127,47 +142,67 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kSortThreads,
     }
     __syncthreads();
     // counts become sums over the warps before
-    for (int g = tid; g < digits; g += kSortThreads) {
-      uint32_t run = 0;
+    uint32_t own = 0;
+    if (tid < digits) {
 #pragma unroll 8
       for (int k = 0; k < kSortWarps; ++k) {
-        const uint32_t c = count[k * digits + g];
-        count[k * digits + g] = run;
-        run += c;
+        const uint32_t c = count[k * digits + tid];
+        count[k * digits + tid] = own;
+        own += c;
       }
-      here[g] = run;
+      here[tid] = own;
     }
     cluster.sync();
     uint32_t all = 0, ahead = 0;
     if (tid < digits) {
 #pragma unroll
-      for (int r = 0; r < kCluster; ++r) {
+      for (int r = 0; r < kSortCluster; ++r) {
         const uint32_t c = *cluster.map_shared_rank(&here[tid], r);
         all += c;
         if (r < rank) ahead += c;
       }
     }
-    uint32_t run = all;
+    // where a digit begins in the cluster's next order (for this block's entries), and in this block's own
+    uint32_t run = all, run_own = own;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const uint32_t up = __shfl_up_sync(0xffffffffu, run, o);
-      if (lane >= o) run += up;
+      const uint32_t up = __shfl_up_sync(0xffffffffu, run, o), up_own = __shfl_up_sync(0xffffffffu, run_own, o);
+      if (lane >= o) {
+        run += up;
+        run_own += up_own;
+      }
     }
-    if (lane == 31) sum[warp] = run;
+    if (lane == 31) {
+      sum[warp] = run;
+      sum_own[warp] = run_own;
+    }
     __syncthreads();
     if (tid < digits) {
-      uint32_t before = run - all + ahead;
-      for (int k = 0; k < warp; ++k) before += sum[k];
-      base[tid] = before;
+      uint32_t before = run - all + ahead, before_own = run_own - own;
+      for (int k = 0; k < warp; ++k) {
+        before += sum[k];
+        before_own += sum_own[k];
+      }
+      base_own[tid] = before_own;
+      base[tid] = before - before_own;
+    }
+    __syncthreads();
+    // first within the block, so that what goes to another block leaves in whole lines
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+      if (s >= steps) break;
+      const uint32_t digit = place[s] >> 16;
+      from[base_own[digit] + mine[digit] + (place[s] & 0xffffu)] = held[s];
     }
     __syncthreads();
 #pragma unroll
-    for (int s = 0; s < kSortEach / kSortThreads; ++s) {
+    for (int s = 0; s < S; ++s) {
       if (s >= steps) break;
-      const uint32_t digit = place[s] >> 16;
-      const uint32_t at = base[digit] + mine[digit] + (place[s] & 0xffffu);
+      const uint32_t i = s * kSortThreads + tid;
+      const u64 e = from[i];
+      const uint32_t at = base[(uint32_t)(e >> shift) & (digits - 1)] + i;
       const uint32_t r = at / each;
-      *cluster.map_shared_rank(to + (at - r * each), r) = from[e0 + 32 * s];
+      *cluster.map_shared_rank(to + (at - r * each), r) = e;
     }
     cluster.sync();
     u64* t = from;
@@ -175,7 +210,7 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kSortThreads,
     to = t;
   }
   uint32_t total = 0;
-  if (rank == 0 && tid < kCluster) total = *cluster.map_shared_rank(&valid_here, tid);
+  if (rank == 0 && tid < kSortCluster) total = *cluster.map_shared_rank(&valid_here, tid);
   total = __reduce_add_sync(0xffffffffu, total);
   if (rank == 0 && tid == 0) {
     *w.total = (int32_t)total;
@@ -622,14 +657,14 @@ cudaError_t grad_t(const int32_t* ids, const T* dout, int64_t ld, int64_t N, int
     int id_bits = 1;
     while (((int64_t)1 << id_bits) <= V) ++id_bits;  // V itself stands for an id to be skipped
     const int passes = (id_bits + 8) / 9, digit_bits = (id_bits + passes - 1) / passes;
-    const int each = (int)(ceil_div(std::max(N, (int64_t)1), kCluster * kSortThreads) * kSortThreads);
+    const int each = (int)(ceil_div(std::max(N, (int64_t)1), kSortCluster * kSortThreads) * kSortThreads);
     const size_t smem = (size_t)each * 16 + ((size_t)kSortWarps << digit_bits) * 4;
-    e = cudaFuncSetAttribute(sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSortEach * 16 + kSortWarps * 512 * 4);
+    e = cudaFuncSetAttribute(sort_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (e != cudaSuccess) return e;
-    const int64_t clear = std::min((int64_t)2 * kSMs / kCluster, ceil_div(bytes, 16 * kSortThreads * kCluster));
+    const int64_t clear = std::min((int64_t)2 * kSMs / kSortCluster, ceil_div(bytes, 16 * kSortThreads * kSortCluster));
     LaunchScope scope_("embed_grad_sort", st);
-    e = launch_k(sort_kernel, dim3((unsigned)((1 + clear) * kCluster)), dim3(kSortThreads), smem, st, ids, (int)N, V, each,
-                 digit_bits, passes, padding_id, w, reinterpret_cast<char*>(grad), bytes);
+    e = launch_clusters(sort_kernel, (unsigned)((1 + clear) * kSortCluster), kSortCluster, kSortThreads, smem, st, ids,
+                        (int)N, V, each, digit_bits, passes, padding_id, w, reinterpret_cast<char*>(grad), bytes);
   } else {
     const int bits = owner_bits(V), owners = 1 << bits, per = (int)ceil_div(V, owners);
     e = cudaFuncSetAttribute(group_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kGroupWarps * kOwned * 4);
