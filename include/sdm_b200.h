@@ -250,7 +250,7 @@ sdm_status sdm_embed(const int32_t* ids, const void* emb, int64_t N, int d, int 
 typedef struct {
   const int32_t* history;      /* (S, history_n), row stride history_ld */
   int64_t history_ld;
-  int history_n;
+  int history_n;               /* less than 2^20 */
   const int32_t* history_len;  /* (S) */
   const int32_t* prompt_len;   /* (S) */
   const float* repetition;     /* (S) */

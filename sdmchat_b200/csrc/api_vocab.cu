@@ -17,7 +17,7 @@ const sdm_logit_rules kNoRules = {nullptr, 0,       0,       nullptr, nullptr, n
 // Rules for S rows over V tokens.
 sdm_status check_rules(const sdm_logit_rules& r, int64_t rows) {
   if (r.history) {
-    if (r.history_n < 0 || r.history_ld < r.history_n) return SDM_ERR_SHAPE;
+    if (r.history_n < 0 || r.history_n > kMaxHistory || r.history_ld < r.history_n) return SDM_ERR_SHAPE;
   } else if (r.history_len || r.prompt_len) {
     return SDM_ERR_ARG;
   }

@@ -402,15 +402,17 @@ __device__ __forceinline__ void store_grad(G* at, const float* v, float scale, i
   }
 }
 
-// Warp (piece, 32 VEC NQ columns): the sums of the piece's groups.  A lane's columns are c + 32 VEC q + e.  32 elements
-// of a lane are in flight: several columns of a few rows, or of more rows where the pieces are few.
+// Warp (piece, 32 VEC NQ columns): the sums of the piece's groups.  A lane's columns are c + 32 VEC q + e.  As many rows
+// as 64 registers hold are in flight together (all of the piece's for bfloat16): with fewer, and more warps in their
+// stead, the same sums took longer.
 template <typename T, typename G, int VEC, int NQ>
-__global__ void __launch_bounds__(kSumThreads, sizeof(T) == 2 ? 4 : 3) sum_kernel(const T* __restrict__ dout,
+__global__ void __launch_bounds__(kSumThreads, 2) sum_kernel(const T* __restrict__ dout,
                                                               int64_t ld, int d,
                                                               int col_blocks, int64_t items, float scale,
                                                               int accumulate, GroupWs w, G* __restrict__ grad) {
   pdl_enter();
-  constexpr int kRows = 32 / (VEC * NQ) < kPiece ? 32 / (VEC * NQ) : kPiece;
+  constexpr int kRowRegs = NQ * (VEC * sizeof(T) < 4 ? 1 : VEC * sizeof(T) / 4);
+  constexpr int kRows = 64 / kRowRegs < kPiece ? 64 / kRowRegs : kPiece;
   typedef typename Word<VEC * sizeof(T)>::type W;
   const int64_t item = (int64_t)blockIdx.x * kSumWarps + (threadIdx.x >> 5);
   if (item >= items) return;
@@ -632,8 +634,8 @@ cudaError_t launch_sum_q(const T* dout, int64_t ld, int64_t N, int d, float scal
   const int64_t items = ceil_div(N, kPiece) * col_blocks, blocks = ceil_div(items, kSumWarps);
   if (blocks > 0x7fffffff) return cudaErrorInvalidValue;
   LaunchScope scope_("embed_grad_sum", st);
-  return launch_k(sum_kernel<T, G, VEC, NQ>, dim3((unsigned)blocks), dim3(kSumThreads), 0, st, dout, ld, d,
-                  col_blocks, items, scale, accumulate, w, grad);
+  return launch_next(sum_kernel<T, G, VEC, NQ>, (unsigned)blocks, kSumThreads, st, dout, ld, d, col_blocks, items, scale,
+                     accumulate, w, grad);
 }
 template <typename T, typename G, int VEC>
 cudaError_t launch_sum(const T* dout, int64_t ld, int64_t N, int d, float scale, int accumulate,
@@ -651,8 +653,8 @@ cudaError_t grad_t(const int32_t* ids, const T* dout, int64_t ld, int64_t N, int
   carve(w, ws, N, d);
   const int64_t bytes = accumulate ? 0 : (int64_t)V * d * sizeof(G);
   cudaError_t e;
-  // One cluster sorts 65,536 positions in less time than clearing a table of 100 MB takes the others; the counting
-  // sort's cost grows with the table instead (at 5,000 positions of 50,021 tokens it took SORT_NOTE).
+  // One cluster sorts 65,536 positions in the time (20 us) in which the others clear a table of 100 MB; the counting
+  // sort's cost grows with the table besides (the same two took 33 us, 5,000 positions of 50,021 tokens 31 against 14).
   if (N <= kSortMax) {
     int id_bits = 1;
     while (((int64_t)1 << id_bits) <= V) ++id_bits;  // V itself stands for an id to be skipped
@@ -689,8 +691,8 @@ cudaError_t grad_t(const int32_t* ids, const T* dout, int64_t ld, int64_t N, int
   const int64_t blocks = (int64_t)hot_blocks * cols + ceil_div(pieces, kJoinWarps);
   if (blocks > 0x7fffffff) return cudaErrorInvalidValue;
   LaunchScope scope_("embed_grad_join", st);
-  return launch_k(join_kernel<G>, dim3((unsigned)blocks), dim3(32 * kJoinWarps), 0, st, d, pieces, hot_blocks, cols, scale,
-                  accumulate, w, grad);
+  return launch_next(join_kernel<G>, (unsigned)blocks, 32 * kJoinWarps, st, d, pieces, hot_blocks, cols, scale, accumulate,
+                     w, grad);
 }
 
 }  // namespace

@@ -12,14 +12,14 @@ namespace {
 namespace cg = cooperative_groups;
 typedef unsigned long long u64;
 
-// A token's word: it occurs in the history; it has bias entries; how often it was generated.
-constexpr uint32_t kSeen = 0x80000000u, kBias = 0x40000000u, kTimes = 0x3fffffffu;
+// A token's word: it occurs in the prompt; it has bias entries, and the number of the first; how often it was generated.
+constexpr uint32_t kSeen = 0x80000000u, kBias = 0x40000000u, kTimes = kMaxHistory;
+constexpr int kBiasAt = 20;
+static_assert(kMaxBias <= 1024 && kMaxHistory < (1 << kBiasAt), "a token's word holds both");
 
 struct RowRules {
   float repetition, frequency, presence;
   const uint32_t* mask;  // this row's mask words, or null
-  const int32_t* bias_ids;
-  const float* bias_values;
   int bias_n;
   bool marks;            // the row has history or biases
 };
@@ -36,55 +36,116 @@ __device__ __forceinline__ RowRules row_rules(const sdm_logit_rules& r, int64_t 
       q.mask = reinterpret_cast<const uint32_t*>(r.mask) + g * (((int64_t)V + 31) / 32);
   }
   q.bias_n = r.bias_ids ? r.bias_n : 0;
-  q.bias_ids = r.bias_ids + (q.bias_n ? row * r.bias_n : 0);
-  q.bias_values = r.bias_values + (q.bias_n ? row * r.bias_n : 0);
   q.marks = q.bias_n > 0 || (r.history && r.history_n > 0);
   return q;
 }
 
+// Shared memory of the marks: a word per token of the slice, then the bias entries (ids, sums).
+inline size_t marks_bytes(const sdm_logit_rules& r, int slice) {
+  return (size_t)slice * 4 + (r.bias_ids ? (size_t)r.bias_n * 8 : 0);
+}
+
+__device__ __forceinline__ int row_length(const sdm_logit_rules& r, int64_t row) {
+  const int width = r.history ? r.history_n : 0;
+  return width == 0 ? 0 : r.history_len ? max(0, min((int)r.history_len[row], width)) : width;
+}
+
 // Fills word[0 .. n) for tokens v0 .. v0 + n - 1 (v0 may be negative: a slice that starts before the row) from the
-// row's history and biases.  Whole-number atomics: the words do not depend on their order.  Ends with a barrier.
+// row's history and biases, and bias[j] with the sum of the entries of entry j's token where entry j is the first of
+// them.  Whole-number atomics: the words do not depend on their order.  Ends with a barrier.
+template <int THREADS>
 __device__ __forceinline__ void mark_tokens(const sdm_logit_rules& r, const RowRules& q, int64_t row, int v0, int n,
-                                            int V, uint32_t* word) {
-  for (int i = threadIdx.x; i < n; i += blockDim.x) word[i] = 0;
+                                            int V, uint32_t* word, float* bias) {
+  // the row's first history entries and its biases are on their way before its length is known
+  constexpr int U = 2048 / THREADS;
+  const int tid = threadIdx.x;
+  const int width = r.history ? r.history_n : 0;
+  const int32_t* h = r.history + (width ? row * r.history_ld : 0);
+  int32_t tok[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) tok[u] = u * THREADS + tid < width ? h[u * THREADS + tid] : -1;
+  const int len = row_length(r, row);
+  const int made = width > 0 && r.prompt_len ? max(0, min((int)r.prompt_len[row], len)) : 0;
+  int32_t* bias_id = reinterpret_cast<int32_t*>(bias + q.bias_n);
+  float* bias_value = bias;
+  for (int j = tid; j < q.bias_n; j += THREADS) {
+    bias_id[j] = r.bias_ids[row * q.bias_n + j];
+    bias_value[j] = r.bias_values[row * q.bias_n + j];
+  }
+  for (int i = tid * 4; i < n; i += THREADS * 4) *reinterpret_cast<uint4*>(word + i) = make_uint4(0, 0, 0, 0);
   __syncthreads();
-  if (!q.marks) return;
-  if (r.history && r.history_n > 0) {
-    int len = r.history_len ? r.history_len[row] : r.history_n;
-    len = max(0, min(len, r.history_n));
-    int made = r.prompt_len ? r.prompt_len[row] : 0;
-    made = max(0, min(made, len));
-    const int32_t* h = r.history + row * r.history_ld;
-    for (int j = threadIdx.x; j < len; j += blockDim.x) {
-      const int v = h[j];
-      if (v < 0 || v >= V || v < v0 || v - v0 >= n) continue;
-      atomicOr(&word[v - v0], kSeen);
-      if (j >= made) atomicAdd(&word[v - v0], 1u);
+  for (int j0 = 0; j0 < len; j0 += U * THREADS) {
+    if (j0 > 0) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int j = j0 + u * THREADS + tid;
+        tok[u] = j < len ? h[j] : -1;
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int j = j0 + u * THREADS + tid, v = tok[u];
+      if (j >= len || v < 0 || v >= V || v < v0 || v - v0 >= n) continue;
+      if (j < made) atomicOr(&word[v - v0], kSeen);
+      else atomicAdd(&word[v - v0], 1u);
     }
   }
-  for (int j = threadIdx.x; j < q.bias_n; j += blockDim.x) {
-    const int v = q.bias_ids[j];
-    if (v >= 0 && v < V && v >= v0 && v - v0 < n) atomicOr(&word[v - v0], kBias);
+  float sum[kMaxBias / THREADS] = {};
+#pragma unroll
+  for (int k = 0; k < kMaxBias / THREADS; ++k) {
+    const int j = k * THREADS + tid;
+    if (j >= q.bias_n) break;
+    const int v = bias_id[j];
+    if (v < 0 || v >= V || v < v0 || v - v0 >= n) continue;
+    bool first = true;
+    for (int i = 0; i < j; ++i) first &= bias_id[i] != v;
+    for (int i = 0; i < q.bias_n; ++i)
+      if (bias_id[i] == v) sum[k] = __fadd_rn(sum[k], bias_value[i]);
+    if (first) atomicOr(&word[v - v0], kBias | (uint32_t)j << kBiasAt);
   }
   __syncthreads();
+  if (q.bias_n > 0) {  // uniform over the block
+#pragma unroll
+    for (int k = 0; k < kMaxBias / THREADS; ++k)
+      if (k * THREADS + tid < q.bias_n) bias[k * THREADS + tid] = sum[k];
+    __syncthreads();
+  }
 }
 
 // The rules of one marked token, in the plain form's order of operations (each rounded to float32, none fused), so
 // that tokens the plain form ties are tied here too.
-__device__ __noinline__ float ruled(float x, uint32_t w, const RowRules& q, int v) {
-  if (w & kSeen) x = x > 0.f ? __fdiv_rn(x, q.repetition) : __fmul_rn(x, q.repetition);
+__device__ __forceinline__ float ruled(float x, uint32_t w, const RowRules& q, const float* bias) {
+  if (w & (kSeen | kTimes)) x = x > 0.f ? __fdiv_rn(x, q.repetition) : __fmul_rn(x, q.repetition);
   const uint32_t g = w & kTimes;
   if (g) {
     x = __fsub_rn(x, __fmul_rn(q.frequency, (float)g));
     x = __fsub_rn(x, q.presence);
   }
-  if (w & kBias) {
-    float b = 0.f;
-    for (int j = 0; j < q.bias_n; ++j)
-      if (q.bias_ids[j] == v) b = __fadd_rn(b, q.bias_values[j]);
-    x = __fadd_rn(x, b);
-  }
+  if (w & kBias) x = __fadd_rn(x, bias[(w >> kBiasAt) & (kMaxBias - 1)]);
   return x;
+}
+
+// The rules on a thread's E elements f (tokens x[0 .. E)), whose words are its own.  Marked tokens are few but for the
+// commonest ones, so each lane takes its marked elements one after the other, through their places in shared memory:
+// all E of them under predicates took 1.5 times as long over 256 rows of 32,768 after 2,048 tokens.
+template <typename T, int E>
+__device__ __forceinline__ void rule_chunk(float* f, const T* x, uint32_t* word, const RowRules& q, const float* bias) {
+  uint32_t marked = 0;
+#pragma unroll
+  for (int e = 0; e < E; e += 4) {
+    const uint4 w = *reinterpret_cast<const uint4*>(word + e);
+    marked |= (uint32_t)(w.x != 0) << e | (uint32_t)(w.y != 0) << (e + 1) | (uint32_t)(w.z != 0) << (e + 2) |
+              (uint32_t)(w.w != 0) << (e + 3);
+  }
+  for (uint32_t left = marked; left; left &= left - 1) {
+    const int e = __ffs(left) - 1;
+    word[e] = __float_as_uint(ruled(to_f32(x[e]), word[e], q, bias));
+  }
+  if (marked) {
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      if ((marked >> e) & 1) f[e] = __uint_as_float(word[e]);
+  }
 }
 
 // Mask bits of the E tokens from v on (v >= 0, v < V).
@@ -102,11 +163,12 @@ constexpr int kProcessThreads = 256;
 // Block (slice, row): 256 x E x U positions of the row, U chunks per thread.  The loads are issued first, so that they
 // are on their way while the history is marked.
 template <typename T, int U>
-__global__ void __launch_bounds__(kProcessThreads) process_kernel(sdm_logit_rules r, const T* logits, int64_t ld,
+__global__ void __launch_bounds__(kProcessThreads, 4) process_kernel(sdm_logit_rules r, const T* logits, int64_t ld,
                                                                   int V, int slices, T* out, int64_t ld_out) {
   pdl_enter();
   constexpr int E = Chunk<T>::E, tile = kProcessThreads * E * U;
   extern __shared__ __align__(16) uint32_t word[];
+  float* bias = reinterpret_cast<float*>(word + tile);
   const int64_t row = blockIdx.x / slices;
   const int slice = blockIdx.x % slices;
   const T* x = logits + row * ld;
@@ -123,7 +185,13 @@ __global__ void __launch_bounds__(kProcessThreads) process_kernel(sdm_logit_rule
     if (v >= 0 && v + E <= V) raw[k] = *reinterpret_cast<const uint4*>(x + v);
   }
   const RowRules q = row_rules(r, row, V);
-  if (q.marks) mark_tokens(r, q, row, v0, tile, V, word);
+  uint32_t bits[U];
+#pragma unroll
+  for (int k = 0; k < U; ++k) {
+    const int64_t v = (int64_t)v0 + (k * kProcessThreads + (int)threadIdx.x) * E;
+    bits[k] = q.mask && v >= 0 && v + E <= V ? mask_bits<E>(q.mask, (int)v, V) : 0xffffffffu;
+  }
+  if (q.marks) mark_tokens<kProcessThreads>(r, q, row, v0, tile, V, word, bias);
 #pragma unroll
   for (int k = 0; k < U; ++k) {
     const int i = (k * kProcessThreads + (int)threadIdx.x) * E;
@@ -133,21 +201,11 @@ __global__ void __launch_bounds__(kProcessThreads) process_kernel(sdm_logit_rule
     if (whole && aligned_out) {
       float f[E];
       Chunk<T>::unpack(raw[k], f);
-      if (q.marks) {
-#pragma unroll
-        for (int e = 0; e < E; e += 4) {
-          const uint4 w = *reinterpret_cast<const uint4*>(word + i + e);
-          if (w.x) f[e] = ruled(f[e], w.x, q, (int)v + e);
-          if (w.y) f[e + 1] = ruled(f[e + 1], w.y, q, (int)v + e + 1);
-          if (w.z) f[e + 2] = ruled(f[e + 2], w.z, q, (int)v + e + 2);
-          if (w.w) f[e + 3] = ruled(f[e + 3], w.w, q, (int)v + e + 3);
-        }
-      }
+      if (q.marks) rule_chunk<T, E>(f, x + v, word + i, q, bias);
       if (q.mask) {
-        const uint32_t b = mask_bits<E>(q.mask, (int)v, V);
 #pragma unroll
         for (int e = 0; e < E; ++e)
-          if (!((b >> e) & 1)) f[e] = -CUDART_INF_F;
+          if (!((bits[k] >> e) & 1)) f[e] = -CUDART_INF_F;
       }
       *reinterpret_cast<uint4*>(y + v) = Chunk<T>::pack(f);
     } else {
@@ -155,7 +213,7 @@ __global__ void __launch_bounds__(kProcessThreads) process_kernel(sdm_logit_rule
         const int64_t u = v + e;
         if (u < 0 || u >= V) continue;
         float f = to_f32(x[u]);
-        if (q.marks && word[i + e]) f = ruled(f, word[i + e], q, (int)u);
+        if (q.marks && word[i + e]) f = ruled(f, word[i + e], q, bias);
         if (q.mask && !((q.mask[u >> 5] >> (u & 31)) & 1)) f = -CUDART_INF_F;
         y[u] = from_f32<T>(f);
       }
@@ -523,6 +581,7 @@ __global__ void __launch_bounds__(kThreads, 2) choose_kernel(sdm_logit_rules r, 
   extern __shared__ __align__(16) uint32_t word[];  // slice words: the marks, then in their place the logits
   __shared__ ChooseShared s;
   float* y = reinterpret_cast<float*>(word);
+  float* bias = y + slice;
   auto cluster = cg::this_cluster();
   const unsigned C = cluster.num_blocks(), rank = cluster.block_rank();
   auto started = cluster.barrier_arrive();  // another block's shared memory is touched once all have started
@@ -550,7 +609,7 @@ __global__ void __launch_bounds__(kThreads, 2) choose_kernel(sdm_logit_rules r, 
   const int top_k = c.top_k ? c.top_k[row] : c.top_k_all;
   const float top_p = c.top_p ? c.top_p[row] : c.top_p_all;
   const float u = c.u ? c.u[row] : 0.f;
-  if (q.marks) mark_tokens(r, q, row, v0, slice, V, word);
+  if (q.marks) mark_tokens<kThreads>(r, q, row, v0, slice, V, word, bias);
   u64 best = 0;
   for (int i0 = 0; i0 < hi; i0 += U * kThreads * E) {
     if (i0 > 0) {
@@ -580,16 +639,7 @@ __global__ void __launch_bounds__(kThreads, 2) choose_kernel(sdm_logit_rules r, 
         }
       }
       float top = -CUDART_INF_F;
-      if (q.marks) {
-#pragma unroll
-        for (int e = 0; e < E; e += 4) {
-          const uint4 w = *reinterpret_cast<const uint4*>(word + i + e);
-          if (w.x) f[e] = ruled(f[e], w.x, q, v + e);
-          if (w.y) f[e + 1] = ruled(f[e + 1], w.y, q, v + e + 1);
-          if (w.z) f[e + 2] = ruled(f[e + 2], w.z, q, v + e + 2);
-          if (w.w) f[e + 3] = ruled(f[e + 3], w.w, q, v + e + 3);
-        }
-      }
+      if (q.marks) rule_chunk<T, E>(f, x + v, word + i, q, bias);
 #pragma unroll
       for (int e = 0; e < E; ++e) {
         if (!((bits >> e) & 1)) f[e] = -CUDART_INF_F;
@@ -814,7 +864,7 @@ cudaError_t process_u(const sdm_logit_rules& r, const T* x, int64_t ld, int64_t 
   const bool marks = (r.history && r.history_n > 0) || (r.bias_ids && r.bias_n > 0);
   LaunchScope scope_("logits_process", st);
   return launch_k(process_kernel<T, U>, dim3((unsigned)(slices * S)), dim3(kProcessThreads),
-                  marks ? (size_t)tile * 4 : 0, st, r, x, ld, V, (int)slices, out, ld_out);
+                  marks ? marks_bytes(r, tile) : 0, st, r, x, ld, V, (int)slices, out, ld_out);
 }
 
 template <typename T>
@@ -837,7 +887,7 @@ cudaError_t choose_t(const sdm_logit_rules& r, const sdm_choice_params& c, const
   if (S * C > 0x7fffffff) return cudaErrorInvalidValue;
   const int slice = slice_of(C);
   LaunchScope scope_("logits_choose", st);
-  return launch_clusters(choose_kernel<T>, (unsigned)(S * C), C, kThreads, (size_t)slice * 4, st, r, c, x, ld, V, slice,
+  return launch_clusters(choose_kernel<T>, (unsigned)(S * C), C, kThreads, marks_bytes(r, slice), st, r, c, x, ld, V, slice,
                          ids, logprob);
 }
 

@@ -10,6 +10,7 @@ constexpr int kSMs = 148;
 constexpr int kMaxCluster = 8;          // portable cluster size
 constexpr int kMaxChoiceV = 1 << 18;    // a row's float32 logits fit a cluster's shared memory: 8 x 128 KB
 constexpr int kMaxBias = 1024;
+constexpr int kMaxHistory = (1 << 20) - 1;
 constexpr int kMaxTeacher = 512;
 
 cudaError_t launch_logits_process(const sdm_logit_rules& r, const void* logits, int64_t ld, int64_t S, int V,
@@ -41,6 +42,22 @@ size_t embed_grad_workspace_bytes(int64_t N, int d, int V);
 cudaError_t launch_embed_grad(const int32_t* ids, const void* dout, int64_t ld, int64_t N, int d, int V, float scale,
                               int padding_id, int dtype, int grad_dtype, int accumulate, void* grad, void* ws,
                               cudaStream_t st);
+
+// A launch that may start while its predecessor in the stream ends, whatever its size (launch_k allows that to small
+// ones only): for kernels that always follow one of their own operator's and whose blocks wait in pdl_enter.
+template <typename... KArgs, typename... Args>
+inline cudaError_t launch_next(void (*kern)(KArgs...), unsigned grid, int block, cudaStream_t st, Args&&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3((unsigned)block);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kern, static_cast<Args&&>(args)...);
+}
 
 // A cluster launch of kern (blocks of one row share a cluster).  Programmatic dependent launch as in launch_k.
 template <typename... KArgs, typename... Args>
