@@ -57,7 +57,7 @@ template <int THREADS>
 __device__ __forceinline__ void mark_tokens(const sdm_logit_rules& r, const RowRules& q, int64_t row, int v0, int n,
                                             int V, uint32_t* word, float* bias) {
   // the row's first history entries and its biases are on their way before its length is known
-  constexpr int U = 2048 / THREADS;
+  constexpr int U = THREADS > 1024 ? 1 : 2048 / THREADS;
   const int tid = threadIdx.x;
   const int width = r.history ? r.history_n : 0;
   const int32_t* h = r.history + (width ? row * r.history_ld : 0);
@@ -222,15 +222,15 @@ __global__ void __launch_bounds__(kProcessThreads, 4) process_kernel(sdm_logit_r
 }
 
 // -------------------------------------------------------------------------------------------------------- choose
-constexpr int kThreads = 512, kWarps = kThreads / 32;
-constexpr int kBins = kThreads;    // one per thread when they are scanned
+constexpr int kMaxWarps = 32;      // a block has NT = 512 or 1,024 threads
+constexpr int kBins = 512;         // at most one per thread when they are scanned
 constexpr int kSplit = 256;        // parts of a key range
 constexpr int kList = 1024;        // candidates that one block ranks
-constexpr int kListK = 256;        // a top_k up to this is found among candidates
+constexpr int kListK = 256;        // a top_k up to this, all blocks of a row together, is found among candidates
 
-// float -> unsigned in the same order (-0 has been made +0, NaN -infinity).
+// float -> unsigned in the same order; -0 and +0 are one value (NaN has been made -infinity).
 __device__ __forceinline__ uint32_t order_key(float y) {
-  const uint32_t b = __float_as_uint(y);
+  const uint32_t b = __float_as_uint(__fadd_rn(y, 0.f));
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 __device__ __forceinline__ float key_value(uint32_t k) {
@@ -296,22 +296,25 @@ struct Cut {
 };
 
 struct ChooseShared {
-  u64 best[kMaxCluster], total[kMaxCluster];
-  float low[kMaxCluster];
+  u64 total[kMaxCluster];
+  float top[kMaxCluster];
   uint32_t ties[kMaxCluster], listed[kMaxCluster];
+  int first[kMaxCluster];
   union {
-    // this block's histogram: tokens, and masses in three limbs of 14 bits (a slice's 2^15 tokens cannot overflow one)
+    // this block's histogram: tokens, and masses in three limbs of 14 bits (a slice's tokens, under 2^16, cannot overflow one)
     struct {
       uint32_t count[kBins], limb[3][kBins];
     };
     u64 sorted[kList];              // block 0's list in order, once the histogram is done with
   };
-  u64 mass_before[kBins + 1];       // over the cluster: of the bins above each bin
+  u64 joined_mass[kBins];           // over the cluster, then summed over the bins before:
+  uint32_t joined_count[kBins];
+  u64 mass_before[kBins + 1];
   uint32_t count_before[kBins + 1];
   u64 split_mass[kSplit + 1];       // the same of a split key range
   uint32_t split_count[kSplit + 1];
-  u64 warp64[kWarps];
-  uint32_t warp32[kWarps];
+  u64 warp64[kMaxWarps];
+  uint32_t warp32[kMaxWarps];
   uint32_t list_n;
   int bin;
   uint32_t klo, khi;
@@ -320,9 +323,9 @@ struct ChooseShared {
   u64 list[kList];                  // candidates: key << 32 | ~token
 };
 
-template <int N>
+template <int NT, int N>
 __device__ __forceinline__ void clear_bins(ChooseShared& s) {
-  for (int b = threadIdx.x; b < N; b += kThreads) s.count[b] = s.limb[0][b] = s.limb[1][b] = s.limb[2][b] = 0;
+  for (int b = threadIdx.x; b < N; b += NT) s.count[b] = s.limb[0][b] = s.limb[1][b] = s.limb[2][b] = 0;
 }
 __device__ __forceinline__ void add_mass(ChooseShared& s, int b, u64 w) {
   const uint32_t w0 = (uint32_t)w & 0x3fffu, w1 = (uint32_t)(w >> 14) & 0x3fffu, w2 = (uint32_t)(w >> 28);
@@ -331,21 +334,13 @@ __device__ __forceinline__ void add_mass(ChooseShared& s, int b, u64 w) {
   if (w2) atomicAdd(&s.limb[2][b], w2);
 }
 
-// Sums the blocks' histograms over the cluster, and writes the sums over the bins before each bin.
-template <int N, typename Cluster>
-__device__ void join_bins(Cluster& cluster, ChooseShared& s, bool masses, u64* mass_before, uint32_t* count_before) {
-  cluster.sync();
+// Sums over the bins before each of N bins, from a count and a mass per thread (bin).
+template <int N>
+__device__ void scan_bins(ChooseShared& s, uint32_t c, u64 m, u64* mass_before, uint32_t* count_before) {
   const int b = threadIdx.x, lane = b & 31, warp = b >> 5;
-  u64 m = 0, im = 0;
-  uint32_t c = 0, ic = 0;
+  uint32_t ic = c;
+  u64 im = m;
   if (b < N) {
-    for (unsigned r = 0; r < cluster.num_blocks(); ++r) {
-      c += *cluster.map_shared_rank(&s.count[b], r);
-      if (masses)
-        m += (u64)*cluster.map_shared_rank(&s.limb[0][b], r) + ((u64)*cluster.map_shared_rank(&s.limb[1][b], r) << 14) +
-             ((u64)*cluster.map_shared_rank(&s.limb[2][b], r) << 28);
-    }
-    ic = c;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const uint32_t up = __shfl_up_sync(0xffffffffu, ic, o);
@@ -373,6 +368,31 @@ __device__ void join_bins(Cluster& cluster, ChooseShared& s, bool masses, u64* m
   __syncthreads();
 }
 
+// Sums the blocks' histograms over the cluster (each block a share of the bins, sent to all), and over the bins.
+template <int NT, int N, typename Cluster>
+__device__ void join_bins(Cluster& cluster, ChooseShared& s, bool masses, u64* mass_before, uint32_t* count_before) {
+  const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank(), share = N / C;
+  cluster.sync();
+  // thread: a bin of the share and a block, whose part it fetches and to which it sends the sum
+  if (threadIdx.x < N) {
+    const int b = rank * share + (int)threadIdx.x / C, r = (int)threadIdx.x % C;
+    uint32_t c = *cluster.map_shared_rank(&s.count[b], r);
+    u64 m = 0;
+    if (masses)
+      m = (u64)*cluster.map_shared_rank(&s.limb[0][b], r) + ((u64)*cluster.map_shared_rank(&s.limb[1][b], r) << 14) +
+          ((u64)*cluster.map_shared_rank(&s.limb[2][b], r) << 28);
+    for (int o = 1; o < C; o <<= 1) {
+      c += __shfl_xor_sync(0xffffffffu, c, o);
+      m += __shfl_xor_sync(0xffffffffu, m, o);
+    }
+    *cluster.map_shared_rank(&s.joined_count[b], r) = c;
+    if (masses) *cluster.map_shared_rank(&s.joined_mass[b], r) = m;
+  }
+  cluster.sync();
+  const int b = threadIdx.x;
+  scan_bins<N>(s, b < N ? s.joined_count[b] : 0u, b < N && masses ? s.joined_mass[b] : 0, mass_before, count_before);
+}
+
 // The first of N bins through which the running count (by_count) or mass reaches `target`; N - 1 if none does.
 template <int N>
 __device__ __forceinline__ int find_bin(ChooseShared& s, const u64* mass_before, const uint32_t* count_before,
@@ -394,20 +414,24 @@ __device__ __forceinline__ int gap_bin(float v, float m, float scale) {
   return v == m ? 0 : min(kBins - 1, (int)((m - v) * scale));
 }
 
-// Lists this block's tokens of bins first .. last above -infinity, and tells the cluster how many they are.  Returns
-// the cluster's number (lists are cut at kList).
-template <typename Cluster>
-__device__ uint32_t list_bins(Cluster& cluster, ChooseShared& s, const float* y, int lo, int hi, int v0, float m,
-                              float scale, int first, int last) {
+// Lists this block's tokens for which `take` holds, and tells the cluster how many they are.  Returns the cluster's
+// number (lists are cut at kList, and the number is then above it).
+template <int NT, typename Cluster, typename F>
+__device__ uint32_t list_tokens(Cluster& cluster, ChooseShared& s, const float* y, int lo, int hi, int v0, F take) {
   if (threadIdx.x == 0) s.list_n = 0;
   __syncthreads();
-  for (int i = lo + threadIdx.x; i < hi; i += kThreads) {
-    const float v = y[i];
-    const int b = gap_bin(v, m, scale);
-    if (b >= first && b <= last && v > -CUDART_INF_F) {
+  auto one = [&](float v, int i) {
+    if (take(v) && i >= lo && i < hi) {
       const uint32_t at = atomicAdd(&s.list_n, 1u);
       if (at < kList) s.list[at] = (u64)order_key(v) << 32 | (0xffffffffu - (uint32_t)(v0 + i));
     }
+  };
+  for (int i = threadIdx.x * 4; i < hi; i += NT * 4) {
+    const float4 v = *reinterpret_cast<const float4*>(y + i);
+    one(v.x, i);
+    one(v.y, i + 1);
+    one(v.z, i + 2);
+    one(v.w, i + 3);
   }
   __syncthreads();
   if (threadIdx.x < cluster.num_blocks()) *cluster.map_shared_rank(&s.listed[cluster.block_rank()], threadIdx.x) = s.list_n;
@@ -419,17 +443,17 @@ __device__ uint32_t list_bins(Cluster& cluster, ChooseShared& s, const float* y,
 
 // Block 0: brings the cluster's lists (n tokens, n <= kList) together in s.sorted, largest first.  All keys differ,
 // so the order does not depend on how the lists were filled.
-template <typename Cluster>
+template <int NT, typename Cluster>
 __device__ void sort_lists(Cluster& cluster, ChooseShared& s, uint32_t n) {
   uint32_t at = s.listed[0];
   for (unsigned r = 1; r < cluster.num_blocks(); ++r) {
     const uint32_t k = s.listed[r];
     const u64* from = cluster.map_shared_rank(&s.list[0], r);
-    for (uint32_t i = threadIdx.x; i < k; i += kThreads) s.list[at + i] = from[i];
+    for (uint32_t i = threadIdx.x; i < k; i += NT) s.list[at + i] = from[i];
     at += k;
   }
   __syncthreads();
-  for (uint32_t i = threadIdx.x; i < n; i += kThreads) {
+  for (uint32_t i = threadIdx.x; i < n; i += NT) {
     const u64 mine = s.list[i];
     uint32_t rank = 0;
 #pragma unroll 4
@@ -441,6 +465,7 @@ __device__ void sort_lists(Cluster& cluster, ChooseShared& s, uint32_t n) {
 
 // Masses of the block's two tokens sorted[2 tid], sorted[2 tid + 1] (0 from `n` on): their sum over all tokens before
 // is returned, `all` is the sum over all.
+template <int NT>
 __device__ u64 scan_sorted(ChooseShared& s, const Masses& M, uint32_t n, u64& w0, u64& w1, u64& all) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const uint32_t i = 2 * threadIdx.x;
@@ -451,7 +476,7 @@ __device__ u64 scan_sorted(ChooseShared& s, const Masses& M, uint32_t n, u64& w0
   __syncthreads();
   u64 before = run - w0 - w1;
   all = 0;
-  for (int w = 0; w < kWarps; ++w) {
+  for (int w = 0; w < (NT / 32); ++w) {
     if (w < warp) before += s.warp64[w];
     all += s.warp64[w];
   }
@@ -462,13 +487,14 @@ __device__ u64 scan_sorted(ChooseShared& s, const Masses& M, uint32_t n, u64& w0
 // Where a row's running count or mass, largest logit first, reaches `target` (1 <= target <= the row's whole), from
 // the joined histogram: the bin's tokens are listed and ranked by one block.  A bin of more than kList tokens (ties, or
 // a row that is almost level) has its key range split in kSplit until one key is left.
-template <typename Cluster>
+template <int NT, typename Cluster>
 __device__ Cut search(Cluster& cluster, ChooseShared& s, const float* y, int lo, int hi, int v0, const Masses& M,
                       float scale, bool by_count, bool masses, u64 target, int which) {
   const int B = find_bin<kBins>(s, s.mass_before, s.count_before, by_count, target);
   u64 above_mass = s.mass_before[B];
   uint32_t above = s.count_before[B];
-  const uint32_t n = list_bins(cluster, s, y, lo, hi, v0, M.m, scale, B, B);
+  const uint32_t n = list_tokens<NT>(cluster, s, y, lo, hi, v0,
+                                 [&](float v) { return gap_bin(v, M.m, scale) == B && v > -CUDART_INF_F; });
   // -infinity is not listed: where the count runs into it, all that is listed is kept
   const bool short_ = by_count && target - above > n;
   if (short_) {
@@ -477,9 +503,9 @@ __device__ Cut search(Cluster& cluster, ChooseShared& s, const float* y, int lo,
   }
   if (n <= kList) {
     if (cluster.block_rank() == 0) {
-      sort_lists(cluster, s, n);
+      sort_lists<NT>(cluster, s, n);
       u64 w0, w1, all;
-      u64 before = above_mass + scan_sorted(s, M, masses ? n : 0, w0, w1, all);
+      u64 before = above_mass + scan_sorted<NT>(s, M, masses ? n : 0, w0, w1, all);
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const uint32_t i = 2 * threadIdx.x + e;
@@ -507,7 +533,7 @@ __device__ Cut search(Cluster& cluster, ChooseShared& s, const float* y, int lo,
   }
   __syncthreads();
   uint32_t kl = 0xffffffffu, kh = 0;
-  for (int i = lo + threadIdx.x; i < hi; i += kThreads) {
+  for (int i = lo + threadIdx.x; i < hi; i += NT) {
     const float v = y[i];
     if (gap_bin(v, M.m, scale) == B) {
       const uint32_t k = order_key(v);
@@ -537,9 +563,9 @@ __device__ Cut search(Cluster& cluster, ChooseShared& s, const float* y, int lo,
   for (int step = 0; step < 5 && kl != kh; ++step) {  // 32-bit keys are down to one after four
     const int shift = max(0, 24 - __clz(kh - kl));
     cluster.sync();  // the histogram's last readers are done
-    clear_bins<kSplit>(s);
+    clear_bins<NT, kSplit>(s);
     __syncthreads();
-    for (int i = lo + threadIdx.x; i < hi; i += kThreads) {
+    for (int i = lo + threadIdx.x; i < hi; i += NT) {
       const float v = y[i];
       const uint32_t k = order_key(v);
       if (k >= kl && k <= kh) {
@@ -548,7 +574,7 @@ __device__ Cut search(Cluster& cluster, ChooseShared& s, const float* y, int lo,
         if (masses) add_mass(s, b, M(v));
       }
     }
-    join_bins<kSplit>(cluster, s, masses, s.split_mass, s.split_count);
+    join_bins<NT, kSplit>(cluster, s, masses, s.split_mass, s.split_count);
     const int b = find_bin<kSplit>(s, s.split_mass, s.split_count, by_count, by_count ? target - above : target - above_mass);
     in = s.split_count[b + 1] - s.split_count[b];
     above += s.split_count[b];
@@ -572,8 +598,8 @@ __device__ __forceinline__ u64 share_of(float top_p, u64 W) {
 __device__ __forceinline__ float log_mass(u64 K) { return logf((float)K * 9.094947017729282e-13f); }  // K / 2^40
 
 // A cluster of blocks per row, each with a slice of the row's processed logits in shared memory.
-template <typename T>
-__global__ void __launch_bounds__(kThreads, 2) choose_kernel(sdm_logit_rules r, sdm_choice_params c,
+template <typename T, int NT>
+__global__ void __launch_bounds__(NT, 1024 / NT) choose_kernel(sdm_logit_rules r, sdm_choice_params c,
                                                           const T* __restrict__ logits, int64_t ld, int V, int slice,
                                                           int32_t* __restrict__ ids, float* __restrict__ logprob) {
   pdl_enter();
@@ -600,7 +626,7 @@ __global__ void __launch_bounds__(kThreads, 2) choose_kernel(sdm_logit_rules r, 
     return q;
   };
 #pragma unroll
-  for (int k = 0; k < U; ++k) raw[k] = load((k * kThreads + tid) * E);
+  for (int k = 0; k < U; ++k) raw[k] = load((k * NT + tid) * E);
 
   const RowRules q = row_rules(r, row, V);
   const float T0 = c.temperature ? c.temperature[row] : c.temperature_all;
@@ -609,16 +635,16 @@ __global__ void __launch_bounds__(kThreads, 2) choose_kernel(sdm_logit_rules r, 
   const int top_k = c.top_k ? c.top_k[row] : c.top_k_all;
   const float top_p = c.top_p ? c.top_p[row] : c.top_p_all;
   const float u = c.u ? c.u[row] : 0.f;
-  if (q.marks) mark_tokens<kThreads>(r, q, row, v0, slice, V, word, bias);
-  u64 best = 0;
-  for (int i0 = 0; i0 < hi; i0 += U * kThreads * E) {
+  if (q.marks) mark_tokens<NT>(r, q, row, v0, slice, V, word, bias);
+  float top = -CUDART_INF_F;  // of this thread's tokens
+  for (int i0 = 0; i0 < hi; i0 += U * NT * E) {
     if (i0 > 0) {
 #pragma unroll
-      for (int k = 0; k < U; ++k) raw[k] = load(i0 + (k * kThreads + tid) * E);
+      for (int k = 0; k < U; ++k) raw[k] = load(i0 + (k * NT + tid) * E);
     }
 #pragma unroll
     for (int k = 0; k < U; ++k) {
-      const int i = i0 + (k * kThreads + tid) * E, v = v0 + i;
+      const int i = i0 + (k * NT + tid) * E, v = v0 + i;
       if (i >= hi) break;
       float f[E];
       const bool whole = i >= lo && i + E <= hi;
@@ -638,59 +664,115 @@ __global__ void __launch_bounds__(kThreads, 2) choose_kernel(sdm_logit_rules r, 
             if (i + e >= lo && i + e < hi && !((q.mask[(v + e) >> 5] >> ((v + e) & 31)) & 1)) bits &= ~(1u << e);
         }
       }
-      float top = -CUDART_INF_F;
       if (q.marks) rule_chunk<T, E>(f, x + v, word + i, q, bias);
+      if (bits != 0xffffffffu) {
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+          if (!((bits >> e) & 1)) f[e] = -CUDART_INF_F;
+      }
 #pragma unroll
       for (int e = 0; e < E; ++e) {
-        if (!((bits >> e) & 1)) f[e] = -CUDART_INF_F;
-        f[e] = __fadd_rn(fmaxf(f[e], -CUDART_INF_F), 0.f);  // NaN is -infinity; -0 and +0 are one value in the order
+        f[e] = fmaxf(f[e], -CUDART_INF_F);  // NaN is -infinity
         top = fmaxf(top, f[e]);
       }
 #pragma unroll
       for (int e = 0; e < E; e += 4)
         *reinterpret_cast<float4*>(y + i + e) = make_float4(f[e], f[e + 1], f[e + 2], f[e + 3]);
-      const uint32_t tk = order_key(top);
-      if (tk > (uint32_t)(best >> 32)) {  // this thread's tokens come in index order: the first largest stays
-        int at = E - 1;
-#pragma unroll
-        for (int e = E - 1; e >= 0; --e)
-          if (f[e] == top) at = e;
-        at = max(at, lo - i);  // all -infinity: any of the row's own
-        best = (u64)tk << 32 | (0xffffffffu - (uint32_t)(v + at));
-      }
     }
   }
-  const float group_top = best ? key_value((uint32_t)(best >> 32)) : -CUDART_INF_F;
-  float low = group_top > -CUDART_INF_F ? group_top : CUDART_INF_F;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
-    low = fminf(low, __shfl_xor_sync(0xffffffffu, low, o));
-  }
+  const bool by_k = !greedy && top_k > 0 && top_k < V, by_p = !greedy && top_p < 1.f;
+  float mine = warp_max(top), low = top > -CUDART_INF_F ? -top : -CUDART_INF_F;
+  low = warp_max(low);  // of the threads' largest, the smallest (negated)
   if (lane == 0) {
-    s.warp64[warp] = best;
-    s.warp32[warp] = __float_as_uint(low);
+    s.warp64[warp] = (u64)__float_as_uint(mine) << 32 | __float_as_uint(low);
   }
   __syncthreads();
-  cluster.barrier_wait(std::move(started));
-  if (tid < (int)C) {
-    u64 b = 0;
-    float l = CUDART_INF_F;
-    for (int w = 0; w < kWarps; ++w) {
-      b = max(b, s.warp64[w]);
-      l = fminf(l, __uint_as_float(s.warp32[w]));
+  float m = -CUDART_INF_F;
+  low = -CUDART_INF_F;
+#pragma unroll
+  for (int w = 0; w < (NT / 32); ++w) {
+    m = fmaxf(m, __uint_as_float((uint32_t)(s.warp64[w] >> 32)));
+    low = fmaxf(low, __uint_as_float((uint32_t)s.warp64[w]));
+  }
+
+  // A small top_k.  A block's threads' largest logits are as many tokens of its slice, so the top_k-th largest of them
+  // is at or below the slice's own: the tokens from there up (a few more than top_k) are listed, and block 0 does the
+  // rest on the blocks' lists.
+  if (by_k && top_k * (int)C <= kListK) {
+    const float scale = (float)(kBins - 1) / (m + low);
+    for (int b = tid; b < kBins; b += NT) s.count[b] = 0;
+    __syncthreads();
+    if (top > -CUDART_INF_F) atomicAdd(&s.count[gap_bin(top, m, scale)], 1u);
+    __syncthreads();
+    scan_bins<kBins>(s, tid < kBins ? s.count[tid] : 0u, 0, s.mass_before, s.count_before);
+    const int last = find_bin<kBins>(s, s.mass_before, s.count_before, true, (u64)top_k);
+    // below every logit of the bins 0 .. last (the last bin has all that are smaller still)
+    const float least = scale > 0.f && last < kBins - 1 ? m - ((float)last + 1.01f) / scale : -CUDART_INF_F;
+    cluster.barrier_wait(std::move(started));
+    const uint32_t n = list_tokens<NT>(cluster, s, y, lo, hi, v0,
+                                   [&](float v) { return v >= least && v > -CUDART_INF_F; });
+    if (n <= kList) {
+      if (rank == 0 && n == 0 && tid == 0) {  // nothing is allowed
+        ids[row] = -1;
+        if (logprob) logprob[row] = -CUDART_INF_F;
+      }
+      if (rank == 0 && n > 0) {
+        sort_lists<NT>(cluster, s, n);
+        const float most = key_value((uint32_t)(s.sorted[0] >> 32));
+        const Masses M(most, Tr);
+        const uint32_t kept = min(n, (uint32_t)top_k);
+        u64* mass = s.list;  // the kept tokens' masses, by rank
+        if (warp == 0) {
+          u64 W = 0;
+          for (uint32_t i0 = 0; i0 < kept; i0 += 32) {
+            const uint32_t i = i0 + lane;
+            const u64 w = i < kept ? M(key_value((uint32_t)(s.sorted[i] >> 32))) : 0;
+            if (i < kept) mass[i] = w;
+            W += warp_sum64(w);
+          }
+          const u64 share = by_p ? share_of(top_p, W) : W;
+          u64 K = 0;
+          uint32_t stay = 0;
+          for (uint32_t i0 = 0; i0 < kept; i0 += 32) {
+            const uint32_t i = i0 + lane;
+            const u64 w = i < kept ? mass[i] : 0, through = K + warp_scan64(w, lane);
+            const uint32_t in = __ballot_sync(0xffffffffu, i < kept && through - w < share);
+            stay += __popc(in);
+            const u64 end = __shfl_sync(0xffffffffu, through, in ? 31 - __clz(in) : 0);
+            if (in) K = end;
+            if (in != 0xffffffffu) break;
+          }
+          if (lane == 0) {
+            s.list_n = stay;
+            s.cut.mass = K;
+          }
+        }
+        __syncthreads();
+        const uint32_t stay = s.list_n;
+        const u64 K = s.cut.mass, target = draw_target(u, K);
+        for (uint32_t i = tid; i < stay; i += NT) {  // the mass of the kept tokens of lower index
+          const uint32_t token = 0xffffffffu - (uint32_t)s.sorted[i];
+          u64 run = 0;
+          for (uint32_t j = 0; j < stay; ++j)
+            if (0xffffffffu - (uint32_t)s.sorted[j] < token) run += mass[j];
+          if (run <= target && target - run < mass[i]) {
+            ids[row] = (int32_t)token;
+            if (logprob) logprob[row] = scaled_gap(key_value((uint32_t)(s.sorted[i] >> 32)), most, Tr) - log_mass(K);
+          }
+        }
+      }
+      cluster.sync();  // the lists were read by block 0
+      return;
     }
-    *cluster.map_shared_rank(&s.best[rank], tid) = b;
-    *cluster.map_shared_rank(&s.low[rank], tid) = l;
+    cluster.sync();  // s.listed is read before it is written again
+  } else {
+    cluster.barrier_wait(std::move(started));
   }
+
+  // the row's largest logit, and its first token
+  if (tid < (int)C) *cluster.map_shared_rank(&s.top[rank], tid) = m;
   cluster.sync();
-  best = 0;
-  low = CUDART_INF_F;
-  for (unsigned k = 0; k < C; ++k) {
-    best = max(best, s.best[k]);
-    low = fminf(low, s.low[k]);
-  }
-  const float m = key_value((uint32_t)(best >> 32));
+  for (unsigned k = 0; k < C; ++k) m = fmaxf(m, s.top[k]);
   if (m == -CUDART_INF_F) {  // nothing is allowed: the same in every block of the cluster
     if (rank == 0 && tid == 0) {
       ids[row] = -1;
@@ -699,76 +781,30 @@ __global__ void __launch_bounds__(kThreads, 2) choose_kernel(sdm_logit_rules r, 
     return;
   }
   const Masses M(m, Tr);
-  const bool by_k = !greedy && top_k > 0 && top_k < V, by_p = !greedy && top_p < 1.f;
-
-  // A small top_k.  A thread's largest logits are as many tokens of the row, so the top_k-th largest of them is at or
-  // below the row's: tokens above it (a few more than top_k) are listed, and one block does the rest on the list.
-  if (by_k && top_k <= kListK) {
-    const float scale = (float)(kBins - 1) / (m - low);
-    clear_bins<kBins>(s);
-    __syncthreads();
-    if (group_top > -CUDART_INF_F) atomicAdd(&s.count[gap_bin(group_top, m, scale)], 1u);
-    join_bins<kBins>(cluster, s, false, s.mass_before, s.count_before);
-    const int last = find_bin<kBins>(s, s.mass_before, s.count_before, true, (u64)top_k);
-    const uint32_t n = list_bins(cluster, s, y, lo, hi, v0, m, scale, 0, last);
-    if (n <= kList) {
-      if (rank == 0) {
-        sort_lists(cluster, s, n);
-        const uint32_t kept = min(n, (uint32_t)top_k);
-        u64 w[2], W, K;
-        u64 before = scan_sorted(s, M, kept, w[0], w[1], W);
-        const u64 share = by_p ? share_of(top_p, W) : W;
-        uint32_t mine = 0;  // kept ones of this thread's two
-        if (2 * tid < kept && before < share) mine = 2 * tid + 1 < kept && before + w[0] < share ? 2 : 1;
-        const uint32_t stay = __syncthreads_count(mine >= 1) + __syncthreads_count(mine == 2);
-        scan_sorted(s, M, stay, w[0], w[1], K);
-        const u64 target = draw_target(u, K);
-        u64* mass = s.list;  // the kept tokens' masses, by rank
-        if (2 * tid < kList) {
-          mass[2 * tid] = w[0];
-          mass[2 * tid + 1] = w[1];
-        }
-        __syncthreads();
-        for (uint32_t i = tid; i < stay; i += kThreads) {  // the mass of the kept tokens of lower index
-          const uint32_t token = 0xffffffffu - (uint32_t)s.sorted[i];
-          u64 run = 0;
-          for (uint32_t j = 0; j < stay; ++j)
-            if (0xffffffffu - (uint32_t)s.sorted[j] < token) run += mass[j];
-          if (run <= target && target - run < mass[i]) {
-            ids[row] = (int32_t)token;
-            if (logprob) logprob[row] = scaled_gap(key_value((uint32_t)(s.sorted[i] >> 32)), m, Tr) - log_mass(K);
-          }
-        }
-      }
-      cluster.sync();  // the lists were read by block 0
-      return;
-    }
-    cluster.sync();  // the histogram is made anew
-  }
 
   // what is kept
   Cut cut = {0, 0, 0, 0};  // all: every key is above 0
   if (by_k || by_p) {
     const float scale = (float)kBins / (28.5f * Tr);  // beyond exp(-28.5) a mass is 0
-    clear_bins<kBins>(s);
+    clear_bins<NT, kBins>(s);
     __syncthreads();
-    for (int i = lo + tid; i < hi; i += kThreads) {
+    for (int i = lo + tid; i < hi; i += NT) {
       const float v = y[i];
       const int b = gap_bin(v, m, scale);
       if (by_k) atomicAdd(&s.count[b], 1u);
       if (by_p) add_mass(s, b, M(v));
     }
-    join_bins<kBins>(cluster, s, by_p, s.mass_before, s.count_before);
+    join_bins<NT, kBins>(cluster, s, by_p, s.mass_before, s.count_before);
     u64 kept = s.mass_before[kBins];
     if (by_k) {
-      cut = search(cluster, s, y, lo, hi, v0, M, scale, true, by_p, (u64)top_k, 0);
+      cut = search<NT>(cluster, s, y, lo, hi, v0, M, scale, true, by_p, (u64)top_k, 0);
       kept = cut.mass;
     }
-    if (by_p) cut = search(cluster, s, y, lo, hi, v0, M, scale, false, true, share_of(top_p, kept), 1);
+    if (by_p) cut = search<NT>(cluster, s, y, lo, hi, v0, M, scale, false, true, share_of(top_p, kept), 1);
   }
 
   // each warp's kept mass over its own stretch of the slice
-  const int seg = slice / kWarps, s0 = max(lo, warp * seg), s1 = min(hi, (warp + 1) * seg);
+  const int seg = slice / (NT / 32), s0 = max(lo, warp * seg), s1 = min(hi, (warp + 1) * seg);
   const bool partial = cut.ties < cut.tie_count;
   const u64 tie_mass = cut.tie_count ? M(key_value(cut.key)) : 0;
   uint32_t sum_hi = 0, tied = 0;
@@ -794,7 +830,7 @@ __global__ void __launch_bounds__(kThreads, 2) choose_kernel(sdm_logit_rules r, 
     __syncthreads();
     if (tid < (int)C) {
       uint32_t n = 0;
-      for (int w = 0; w < kWarps; ++w) n += s.warp32[w];
+      for (int w = 0; w < (NT / 32); ++w) n += s.warp32[w];
       *cluster.map_shared_rank(&s.ties[rank], tid) = n;
     }
     cluster.sync();
@@ -803,12 +839,24 @@ __global__ void __launch_bounds__(kThreads, 2) choose_kernel(sdm_logit_rules r, 
     tied = cut.ties > tie_before ? min(tied, cut.ties - tie_before) : 0;
   }
   if (cut.tie_count) sum += (u64)tied * tie_mass;
+  if (greedy) {  // the first token that has the largest logit
+    int at = 0x7fffffff;
+    for (int i = s1 - 1 - lane; i >= s0; i -= 32)
+      if (y[i] == m) at = v0 + i;
+    at = __reduce_min_sync(0xffffffffu, at);
+    if (lane == 0) s.warp32[warp] = (uint32_t)at;
+  }
   if (lane == 0) s.warp64[warp] = sum;
   __syncthreads();
   if (tid < (int)C) {
     u64 t = 0;
-    for (int w = 0; w < kWarps; ++w) t += s.warp64[w];
+    int at = 0x7fffffff;
+    for (int w = 0; w < (NT / 32); ++w) {
+      t += s.warp64[w];
+      at = min(at, (int)s.warp32[w]);
+    }
     *cluster.map_shared_rank(&s.total[rank], tid) = t;
+    *cluster.map_shared_rank(&s.first[rank], tid) = at;
   }
   cluster.sync();  // the last access to another block's shared memory is before this
   u64 K = 0, before = 0;
@@ -819,7 +867,9 @@ __global__ void __launch_bounds__(kThreads, 2) choose_kernel(sdm_logit_rules r, 
   const float log_k = log_mass(K);
   if (greedy) {
     if (rank == 0 && tid == 0) {
-      ids[row] = (int32_t)(0xffffffffu - (uint32_t)best);
+      int at = s.first[0];
+      for (unsigned k = 1; k < C; ++k) at = min(at, s.first[k]);
+      ids[row] = at;
       if (logprob) logprob[row] = 0.f - log_k;
     }
     return;
@@ -877,18 +927,29 @@ cudaError_t process_t(const sdm_logit_rules& r, const T* x, int64_t ld, int64_t 
   return process_u<T, 1>(r, x, ld, S, V, out, ld_out, st);
 }
 
+template <typename T, int NT>
+cudaError_t choose_n(const sdm_logit_rules& r, const sdm_choice_params& c, const T* x, int64_t ld, int64_t S, int V, int C,
+                     int slice, int32_t* ids, float* logprob, cudaStream_t st) {
+  LaunchScope scope_("logits_choose", st);
+  return launch_clusters(choose_kernel<T, NT>, (unsigned)(S * C), C, NT, marks_bytes(r, slice), st, r, c, x, ld, V, slice,
+                         ids, logprob);
+}
+
 template <typename T>
 cudaError_t choose_t(const sdm_logit_rules& r, const sdm_choice_params& c, const T* x, int64_t ld, int64_t S, int V,
                      int32_t* ids, float* logprob, cudaStream_t st) {
   constexpr int E = Chunk<T>::E;
   int C = 1;
-  auto slice_of = [&](int n) { return (int)(ceil_div(ceil_div((int64_t)V + E - 1, n), kThreads) * kThreads); };
-  while (C < kMaxCluster && (S * C < kSMs || slice_of(C) * 4 > 100 * 1024)) C *= 2;
+  auto slice_of = [&](int n) { return (int)(ceil_div(ceil_div((int64_t)V + E - 1, n), 1024) * 1024); };
+  // More blocks per row while all of them can be on the GPU together (two per SM, and a cluster within a GPC), or while
+  // a slice does not fit a block's shared memory.  256 rows of 32,768: 38 us in whole rows, 40 in halves, 68 in quarters.
+  while (C < kMaxCluster && (S * C * 2 <= 256 || slice_of(C) * 4 > 144 * 1024)) C *= 2;
   if (S * C > 0x7fffffff) return cudaErrorInvalidValue;
   const int slice = slice_of(C);
-  LaunchScope scope_("logits_choose", st);
-  return launch_clusters(choose_kernel<T>, (unsigned)(S * C), C, kThreads, marks_bytes(r, slice), st, r, c, x, ld, V, slice,
-                         ids, logprob);
+  // 1,024 threads where each still has eight tokens (33 rows of 50,021 in quarters: 34 us, 39 with 512), else 512 (one
+  // row of 32,768 in eighths: 8.3 us, 9.9 with 1,024)
+  if (slice > 8192) return choose_n<T, 1024>(r, c, x, ld, S, V, C, slice, ids, logprob, st);
+  return choose_n<T, 512>(r, c, x, ld, S, V, C, slice, ids, logprob, st);
 }
 
 }  // namespace
