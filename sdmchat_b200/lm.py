@@ -7,8 +7,9 @@ in the reference) and the transformer/sdmonly comparison arms are not part of th
 
 The decode API is new (the reference has no carried-state decode): `prefill` runs the chunked prefill and keeps
 each layer's final memory state, `decode_step` advances every stream by one token reading and writing that state in
-place, and `generate` does greedy decoding.
+place, and `generate` decodes greedily or by sampling under rules on the logits (vocab.py).
 """
+import dataclasses
 import math
 
 import torch
@@ -16,6 +17,7 @@ import torch.nn as nn
 
 from ._lib import check, lib, ptr, stream_ptr, workspace, dtype_code
 from .modules import RMSNorm, RunTimeSdm, SwiGLU, TrainedSdm, matched_sdm_n_sub, _forward_only
+from .vocab import LogitRules, sample_logits
 
 
 class OneSdmLM(nn.Module):
@@ -257,9 +259,9 @@ class OneSdmLM(nn.Module):
         device = device or self.emb.weight.device
         return [m.init_state(S, device) for m in self.mems]
 
-    def prefill(self, idx, state):
+    def prefill(self, idx, state, logits=False):
         """Run the prompt idx (S, T) through the chunked path, leave each layer's final memory in `state`, and
-        return the greedy next token of every stream (S,) int32."""
+        return the greedy next token of every stream (S,) int32, or (logits) its logits (S, V)."""
         _forward_only(self.emb.weight)
         x, _ = self.enfold(idx)
         reset = (idx == self.bos_id) if self.reset_at_bos else None
@@ -275,11 +277,11 @@ class OneSdmLM(nn.Module):
                 x = self.mlps[i].block(x, self.mnorms[i].w, self.mnorms[i].eps)
             elif self.ffn == "sdm":
                 x = self.sdms[i]._run(x, add_residual=True)[0]
-        return self._head(x[:, -1], "argmax")
+        return self._head(x[:, -1], "logits" if logits else "argmax")
 
-    def decode_step(self, ids, state, reset=None):
+    def decode_step(self, ids, state, reset=None, logits=False):
         """Advance every stream by one token ids (S,): all layers read and write their carried state in place.
-        Returns the greedy next token (S,) int32."""
+        Returns the greedy next token (S,) int32, or (logits) its logits (S, V)."""
         _forward_only(self.emb.weight)
         x, _ = self.enfold(ids)
         if reset is None and self.reset_at_bos:
@@ -292,7 +294,7 @@ class OneSdmLM(nn.Module):
                 x = self.mlps[i].block(x, self.mnorms[i].w, self.mnorms[i].eps)
             elif self.ffn == "sdm":
                 x = self.sdms[i]._run(x, add_residual=True)[0]
-        return self._head(x, "argmax")
+        return self._head(x, "logits" if logits else "argmax")
 
     def decode_graph(self, state):
         """Capture one decode_step over `state` (all its streams) as a CUDA graph; returns step(ids) -> next ids.
@@ -325,9 +327,20 @@ class OneSdmLM(nn.Module):
         step.graph = graph
         return step
 
-    def generate(self, prompt, steps, use_graph=True):
-        """Greedy decoding: prompt (S, T) -> (S, steps) generated ids (int64)."""
+    def generate(self, prompt, steps, use_graph=True, rules=None, u=None, temperature=0.0, top_k=0, top_p=1.0,
+                 return_logprobs=False):
+        """Decoding: prompt (S, T) -> (S, steps) generated ids (int64), greedy unless told otherwise.
+
+        rules: a LogitRules whose penalties, biases and masks hold for every step; its history is the prompt and what
+        has been generated, kept here (masks that change from step to step are the caller's to write into rules.mask
+        between calls of sample_logits).  temperature, top_k, top_p: as in sample_logits.  u (S, steps): the numbers in
+        [0, 1) that pick the tokens, by default torch.rand's.  A stream whose rules allow no token gets -1 from there
+        on.  return_logprobs: also the tokens' log-probabilities (S, steps) under the distribution drawn from."""
+        sampled = rules is not None or u is not None or torch.is_tensor(temperature) or temperature != 0
         state = self.init_decode(prompt.shape[0], prompt.device)
+        if sampled or return_logprobs:
+            return self._generate_sampled(prompt, steps, use_graph, rules or LogitRules(), u, temperature, top_k, top_p,
+                                          return_logprobs, state)
         nxt = self.prefill(prompt, state)
         out = [nxt.clone()]
         step = self.decode_graph(state) if (use_graph and steps > 2) else (lambda ids: self.decode_step(ids, state))
@@ -335,6 +348,58 @@ class OneSdmLM(nn.Module):
             nxt = step(nxt)
             out.append(nxt.clone())
         return torch.stack(out, 1).long()
+
+    def _generate_sampled(self, prompt, steps, use_graph, rules, u, temperature, top_k, top_p, return_logprobs, state):
+        S, T = prompt.shape
+        dev = prompt.device
+        if u is None and (torch.is_tensor(temperature) or temperature != 0):
+            u = torch.rand(S, steps, device=dev)
+        i32 = dict(dtype=torch.int32, device=dev)
+        # everything that a step reads or advances lives at a fixed address, so that a step can be a graph
+        own = {"history": torch.full((S, T + steps), -1, **i32), "len": torch.full((S,), T, **i32),
+               "ids": torch.empty(S, **i32), "alive": torch.ones(S, dtype=torch.bool, device=dev),
+               "out": torch.full((S, steps), -1, **i32),
+               "logprob": torch.full((S, steps), -math.inf, dtype=torch.float32, device=dev)}
+        own["history"][:, :T] = prompt
+        rules = dataclasses.replace(rules, history=own["history"], history_len=own["len"],
+                                    prompt_len=torch.full((S,), T, **i32))
+
+        def choose(logits):
+            at = (own["len"] - T).long()[:, None]
+            ids, lp = sample_logits(logits, rules, None if u is None else u.gather(1, at)[:, 0], temperature, top_k, top_p)
+            own["alive"] &= ids >= 0
+            ids = torch.where(own["alive"], ids, -1)
+            own["out"].scatter_(1, at, ids[:, None])
+            own["logprob"].scatter_(1, at, torch.where(own["alive"], lp, -math.inf)[:, None])
+            own["history"].scatter_(1, own["len"].long()[:, None], ids[:, None])
+            own["ids"].copy_(ids.clamp(min=0))
+            own["len"] += 1
+
+        def step():
+            choose(self.decode_step(own["ids"], state, logits=True))
+
+        if steps > 0:
+            choose(self.prefill(prompt, state, logits=True))
+        if use_graph and steps > 2:
+            kept = [{k: v.clone() for k, v in d.items()} for d in (*state, own)]
+            side = torch.cuda.Stream(dev)
+            side.wait_stream(torch.cuda.current_stream(dev))
+            with torch.cuda.stream(side), torch.no_grad():
+                step()  # weight caches and workspaces exist before the capture
+            torch.cuda.current_stream(dev).wait_stream(side)
+            for d, was in zip((*state, own), kept):
+                for k in d:
+                    d[k].copy_(was[k])
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph), torch.no_grad():
+                step()
+            for _ in range(steps - 1):
+                graph.replay()
+        else:
+            for _ in range(steps - 1):
+                step()
+        out = own["out"].long()
+        return (out, own["logprob"]) if return_logprobs else out
 
 
 DEFAULTS = dict(d=256, layers=4, mlp_f=688, heads=4, n_sub=32, d_a=32, k=16)

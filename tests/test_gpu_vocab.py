@@ -547,3 +547,65 @@ def test_calls_run_on_the_current_stream(cuda_ok):
     side.synchronize()
     for a, b in zip(want, got):
         assert torch.equal(a, b)
+
+
+# ----------------------------------------------------------------------------------------------- the path together
+def small_model(V=500):
+    torch.manual_seed(3)
+    m = S.build_onesdm("onesdm_allsdm", V, dict(d=64, layers=2, mlp_f=176, heads=4, n_sub=8, d_a=8, k=4, chunk=16))
+    with torch.no_grad():
+        for p in m.parameters():
+            if p.dim() >= 2 and float(p.abs().max()) == 0:
+                torch.nn.init.normal_(p, std=0.3)
+        m.emb.weight.mul_(20)
+    return m.to_bf16_stream().to(DEV)
+
+
+def test_generate_greedy_under_rules_that_change_nothing(cuda_ok):
+    m = small_model()
+    prompt = torch.randint(0, 500, (3, 20), generator=gen(1), device=DEV)
+    with torch.no_grad():
+        want = m.generate(prompt, 8)
+        got, lp = m.generate(prompt, 8, rules=S.LogitRules(), return_logprobs=True)
+        assert torch.equal(got, want) and (lp <= 0).all() and torch.isfinite(lp).all()
+        assert torch.equal(m.generate(prompt, 8, rules=S.LogitRules(), use_graph=False), want)
+        assert torch.equal(m.generate(prompt, 1, rules=S.LogitRules()), want[:, :1])
+
+
+def test_generate_sampled(cuda_ok):
+    m = small_model()
+    S_, T, n, V = 5, 12, 16, 500
+    prompt = torch.randint(0, V, (S_, T), generator=gen(2), device=DEV)
+    u = torch.rand(S_, n, generator=gen(3), device=DEV)
+    allowed = torch.zeros(2, -(-V // 32), dtype=torch.int32, device=DEV)
+    allowed[0, 3] = -1  # tokens 96 .. 127
+    row = torch.tensor([-1, 0, 0, 1, -1], device=DEV)
+    rules = S.LogitRules(presence=1e4, mask=allowed, mask_row=row)
+    kw = dict(rules=rules, u=u, temperature=0.8, top_k=40, top_p=0.9, return_logprobs=True)
+    with torch.no_grad():
+        a, la = m.generate(prompt, n, **kw)
+        b, lb = m.generate(prompt, n, use_graph=False, **kw)
+    assert torch.equal(a, b) and torch.equal(la, lb)  # a graph's steps are the same steps
+    for i in (0, 1, 2, 4):
+        assert len(set(a[i].tolist())) == n  # the presence penalty forbids a token twice
+    assert ((a[1:3] >= 96) & (a[1:3] < 128)).all()
+    assert (a[3] == -1).all() and torch.isneginf(la[3]).all()  # its mask allows nothing
+    # step by step by hand: prefix logits, the same rules and numbers
+    with torch.no_grad():
+        logits = m(torch.cat([prompt, a[:, :4].clamp(min=0)], 1))[:, -1]
+    hist = torch.cat([prompt, a[:, :4]], 1)
+    r = S.LogitRules(history=hist, prompt_len=torch.full((S_,), T, device=DEV), presence=1e4, mask=allowed, mask_row=row)
+    ids, _ = S.sample_logits(logits, r, u=u[:, 4], temperature=0.8, top_k=40, top_p=0.9)
+    # decode and prefix logits differ by bf16 rounding, which may move a draw near a boundary: most agree
+    assert (ids.long() == a[:, 4]).sum() >= S_ - 1
+
+
+def test_distil_example(cuda_ok):
+    import importlib.util
+    import os
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "distil_on_policy.py")
+    spec = importlib.util.spec_from_file_location("distil_on_policy", path)
+    mod = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(mod)
+    losses = mod.main(["--steps", "25", "--vocab", "512", "--d", "64", "--batch", "8", "--prompt", "8", "--new", "8"])
+    assert all(np.isfinite(losses)) and np.mean(losses[-5:]) < 0.8 * np.mean(losses[:5])
