@@ -1,6 +1,8 @@
 // The scaled token lookup and its gradient, the sum of dout's rows over the positions of each token.
 //
-// Gradient.  The positions are sorted by token while the gradient is cleared: up to kSortMax positions by one cluster's
+// Gradient.  Up to kFewMax positions are done in one launch (few_kernel): blocks clear the rows that no id names, and the
+// first position of each token adds up its others.  For more, the positions are sorted by token while the gradient is
+// cleared: up to kSortMax positions by one cluster's
 // radix sort in shared memory (sort_kernel; the other blocks clear), more by a counting sort over all SMs
 // (group_kernel).  sum_kernel cuts the sorted order into pieces of kPiece positions, a warp each: a group inside a
 // piece is added up and written, a group that crosses a cut leaves a partial sum on each side.  join_kernel adds the
@@ -13,6 +15,8 @@ namespace sdm {
 namespace {
 
 constexpr int kPiece = 16;       // positions summed by one warp (with its two neighbours at most 32)
+constexpr int kFewMax = 1024;    // positions that one launch compares with one another: 16 to 24 us over a table of
+                                 // 32,768 x 768, against 31 by sorting; at 2,048 it takes 40, and sorting 32
 constexpr int kLong = 16;        // a group that goes on over so many more pieces is joined by blocks
 constexpr int kSortThreads = 1024, kSortWarps = kSortThreads / 32;
 constexpr int kSortCluster = 16; // blocks of the sorting cluster (more than the portable 8)
@@ -485,6 +489,76 @@ __global__ void __launch_bounds__(kSumThreads, 2) sum_kernel(const T* __restrict
   }
 }
 
+// Few positions: warp (position, 32 VEC columns) passes on unless its position is the first of its token, else it adds up
+// the token's rows in order; then block b zeroes its share of the table's rows but for those that an id names.
+template <typename T, typename G, int VEC>
+__global__ void __launch_bounds__(256) few_kernel(const int32_t* __restrict__ ids, const T* __restrict__ dout, int64_t ld,
+                                                  int N, int d, int V, int col_blocks, int share, int zero_words,
+                                                  float scale, int padding_id, int accumulate, G* __restrict__ grad) {
+  pdl_enter();
+  __shared__ int32_t id_[kFewMax];       // ids, -1 where skipped
+  __shared__ uint16_t list[8][kFewMax];  // a warp's positions
+  extern __shared__ unsigned char named[];  // a flag per row of the block's share
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  uint16_t* at = list[warp];
+  const int64_t r0 = (int64_t)blockIdx.x * share, r1 = min((int64_t)V, r0 + share);
+  if (!accumulate)
+    for (int i = tid; i < share; i += 256) named[i] = 0;
+  __syncthreads();
+  for (int n = tid; n < N; n += 256) {
+    int id = ids[n];
+    if (id < 0 || id >= V || id == padding_id) id = -1;
+    id_[n] = id;
+    if (!accumulate && id >= r0 && id < r1) named[id - r0] = 1;
+  }
+  __syncthreads();
+  for (int64_t item = (int64_t)blockIdx.x * 8 + warp; item < (int64_t)N * col_blocks; item += (int64_t)gridDim.x * 8) {
+    const int n = (int)(item / col_blocks), c = (int)(item - (int64_t)n * col_blocks) * 32 * VEC + VEC * lane;
+    const int v = id_[n];
+    if (v < 0) continue;
+    bool earlier = false;
+    for (int i = lane; i < n; i += 32) earlier |= id_[i] == v;
+    if (__any_sync(0xffffffffu, earlier)) continue;
+    int m = 0;  // the token's positions, in order
+    for (int i0 = n & ~31; i0 < N; i0 += 32) {
+      const bool same = i0 + lane < N && id_[i0 + lane] == v;
+      const uint32_t lanes = __ballot_sync(0xffffffffu, same);
+      if (same) at[m + __popc(lanes & ((1u << lane) - 1))] = (uint16_t)(i0 + lane);
+      m += __popc(lanes);
+    }
+    __syncwarp();
+    float acc[VEC] = {};
+    constexpr int R = 16;  // rows whose loads are in flight
+    for (int i0 = 0; i0 < m; i0 += R) {
+      Pack<T, VEC> p[R];
+#pragma unroll
+      for (int u = 0; u < R; ++u)
+        if (i0 + u < m && c < d)
+          p[u].u = __ldg(reinterpret_cast<const typename Word<VEC * sizeof(T)>::type*>(dout + (int64_t)at[i0 + u] * ld + c));
+#pragma unroll
+      for (int u = 0; u < R; ++u)
+        if (i0 + u < m) {
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) acc[e] += p[u].get(e);
+        }
+    }
+    __syncwarp();
+    if (c < d) store_grad<G, VEC>(grad + (int64_t)v * d + c, acc, scale, accumulate);
+  }
+  if (!accumulate)
+    for (int64_t r = r0 + warp; r < r1; r += 8) {
+      if (named[r - r0]) continue;
+      if (zero_words) {  // rows of whole 16-byte words
+        uint4* row = reinterpret_cast<uint4*>(grad + r * d);
+        for (int i = lane; i < zero_words; i += 32) row[i] = make_uint4(0, 0, 0, 0);
+      } else {
+        G* row = grad + r * d;
+        const float none[VEC] = {};
+        for (int c = VEC * lane; c < d; c += 32 * VEC) store_grad<G, VEC>(row + c, none, 0.f, 0);
+      }
+    }
+}
+
 template <typename G>
 __device__ __forceinline__ void store_joined(G* row, int c, int d, float4 s, float scale, int accumulate) {
   const float v[4] = {s.x, s.y, s.z, s.w};
@@ -646,9 +720,34 @@ cudaError_t launch_sum(const T* dout, int64_t ld, int64_t N, int d, float scale,
   return launch_sum_q<T, G, VEC, 1>(dout, ld, N, d, scale, accumulate, w, grad, st);
 }
 
+template <typename T, typename G, int VEC>
+cudaError_t launch_few(const int32_t* ids, const T* dout, int64_t ld, int64_t N, int d, int V, float scale, int padding_id,
+                       int accumulate, G* grad, cudaStream_t st) {
+  const int col_blocks = (int)ceil_div(d, 32 * VEC);
+  int64_t blocks = std::max(ceil_div(N * col_blocks, 8), accumulate ? (int64_t)1 : ceil_div(V, 8));
+  blocks = std::max(std::min(blocks, (int64_t)kSMs * 8), ceil_div(V, 32768));  // eight blocks per SM; a block's flags
+  const int share = (int)ceil_div(V, blocks);
+  const bool whole = (int64_t)d * sizeof(G) % 16 == 0 && (reinterpret_cast<uintptr_t>(grad) & 15) == 0;
+  LaunchScope scope_("embed_grad_few", st);
+  return launch_k(few_kernel<T, G, VEC>, dim3((unsigned)blocks), dim3(256), (size_t)share, st, ids, dout, ld,
+                  (int)N, d, V, col_blocks, share, whole ? (int)((int64_t)d * sizeof(G) / 16) : 0, scale, padding_id,
+                  accumulate, grad);
+}
+
 template <typename T, typename G>
 cudaError_t grad_t(const int32_t* ids, const T* dout, int64_t ld, int64_t N, int d, int V, float scale,
                    int padding_id, int accumulate, G* grad, void* ws, cudaStream_t st) {
+  const int vec = vec_of(16 / sizeof(T), d, ld, dout, sizeof(T), grad, sizeof(G));
+  if (N <= kFewMax) {
+    switch (vec) {
+      case 8:
+        if constexpr (sizeof(T) == 2) return launch_few<T, G, 8>(ids, dout, ld, N, d, V, scale, padding_id, accumulate, grad, st);
+        return cudaErrorInvalidValue;
+      case 4: return launch_few<T, G, 4>(ids, dout, ld, N, d, V, scale, padding_id, accumulate, grad, st);
+      case 2: return launch_few<T, G, 2>(ids, dout, ld, N, d, V, scale, padding_id, accumulate, grad, st);
+      default: return launch_few<T, G, 1>(ids, dout, ld, N, d, V, scale, padding_id, accumulate, grad, st);
+    }
+  }
   GroupWs w;
   carve(w, ws, N, d);
   const int64_t bytes = accumulate ? 0 : (int64_t)V * d * sizeof(G);
@@ -675,8 +774,8 @@ cudaError_t grad_t(const int32_t* ids, const T* dout, int64_t ld, int64_t N, int
     e = launch_k(group_kernel, dim3((unsigned)(owners * kCluster)), dim3(kGroupThreads), (size_t)kGroupWarps * per * 4, st,
                  ids, (int)N, V, bits, per, padding_id, w, reinterpret_cast<char*>(grad), bytes);
   }
-  if (e != cudaSuccess || N == 0) return e;
-  switch (vec_of(16 / sizeof(T), d, ld, dout, sizeof(T), grad, sizeof(G))) {
+  if (e != cudaSuccess) return e;
+  switch (vec) {
     case 8:
       if constexpr (sizeof(T) == 2) e = launch_sum<T, G, 8>(dout, ld, N, d, scale, accumulate, w, grad, st);
       else e = cudaErrorInvalidValue;
@@ -685,7 +784,7 @@ cudaError_t grad_t(const int32_t* ids, const T* dout, int64_t ld, int64_t N, int
     case 2: e = launch_sum<T, G, 2>(dout, ld, N, d, scale, accumulate, w, grad, st); break;
     default: e = launch_sum<T, G, 1>(dout, ld, N, d, scale, accumulate, w, grad, st); break;
   }
-  if (e != cudaSuccess || N <= kPiece) return e;
+  if (e != cudaSuccess) return e;
   const int pieces = (int)ceil_div(N, kPiece), cols = (int)ceil_div(d, 128);
   const int hot_blocks = std::min(pieces / kLong + 1, 64);
   const int64_t blocks = (int64_t)hot_blocks * cols + ceil_div(pieces, kJoinWarps);
