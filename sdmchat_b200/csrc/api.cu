@@ -6,6 +6,8 @@ using namespace sdm;
 
 namespace sdm {
 cudaError_t read_and_clear_timeout(int* flag, cudaStream_t st);
+cudaError_t read_and_clear_distill_timeout(int* flag, cudaStream_t st);
+cudaError_t set_distill_wait_limit(unsigned long long ns);
 }  // namespace sdm
 
 namespace {
@@ -407,15 +409,17 @@ extern "C" {
 int sdm_abi_version(void) { return 4; }
 
 sdm_status sdm_device_status(void* stream) {
-  int gemm = 0, scan = 0;
+  int gemm = 0, scan = 0, distill = 0;
   if (read_and_clear_timeout(&gemm, S(stream)) != cudaSuccess) return SDM_ERR_CUDA;
   if (read_and_clear_scan_timeout(&scan, S(stream)) != cudaSuccess) return SDM_ERR_CUDA;
-  return (gemm || scan) ? SDM_ERR_TIMEOUT : SDM_OK;
+  if (read_and_clear_distill_timeout(&distill, S(stream)) != cudaSuccess) return SDM_ERR_CUDA;
+  return (gemm || scan || distill) ? SDM_ERR_TIMEOUT : SDM_OK;
 }
 
 sdm_status sdm_set_wait_limit_ns(uint64_t ns) {
   if (set_gemm_wait_limit(ns) != cudaSuccess) return SDM_ERR_CUDA;
   if (set_scan_wait_limit(ns) != cudaSuccess) return SDM_ERR_CUDA;
+  if (set_distill_wait_limit(ns) != cudaSuccess) return SDM_ERR_CUDA;
   return SDM_OK;
 }
 

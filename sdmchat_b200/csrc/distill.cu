@@ -9,6 +9,7 @@
 // block, or of a cluster of blocks that exchange their maxima and sums; the gradient is formed from that copy.
 #include <math_constants.h>
 #include <type_traits>
+#include "tma.cuh"
 #include "vocab.cuh"
 
 namespace sdm {
@@ -122,22 +123,24 @@ struct Row {
 };
 
 template <typename T>
-__device__ __forceinline__ Row row_of(const DistillArgs& a, int slice, int C, int rank, const T*& x) {
+__device__ __forceinline__ Row row_of(const DistillArgs& a, int slice, int C, int rank, int64_t row, const T*& x) {
   Row q;
   q.C = C;
   q.rank = rank;
-  q.row = blockIdx.x / C;
+  q.row = row;
   x = static_cast<const T*>(a.logits) + q.row * a.ld;
   q.V = a.V;
   q.k = a.k;
-  q.w = a.row_weight ? a.row_weight[q.row] : 1.f;
-  q.tgt = a.targets ? a.targets[q.row] : -1;
-  q.hard = q.tgt >= 0 && q.tgt < q.V;
   q.inv_t = 1.f / a.temperature;
   q.v0 = rank * slice - row_offset(x);
   q.lo = max(0, -q.v0);
   q.hi = max(q.lo, min(slice, q.V - q.v0));
   return q;
+}
+__device__ __forceinline__ void load_terms(const DistillArgs& a, Row& q) {
+  q.w = a.row_weight ? a.row_weight[q.row] : 1.f;
+  q.tgt = a.targets ? a.targets[q.row] : -1;
+  q.hard = q.tgt >= 0 && q.tgt < q.V;
 }
 
 // The row's entries and the logits they point at (every block of a cluster takes all of them).
@@ -155,7 +158,8 @@ __device__ __forceinline__ void load_teacher(const DistillArgs& a, const Row& q,
 }
 
 // One warp: log p of each entry, and their sum (-1: the row has no entry).
-__device__ __forceinline__ void teacher_softmax(const DistillArgs& a, const Row& q, DistillShared& s) {
+template <typename S>
+__device__ __forceinline__ void teacher_softmax(const DistillArgs& a, const Row& q, S& s) {
   const int lane = threadIdx.x & 31;
   float lse, tm = -CUDART_INF_F;
   bool any = false;
@@ -182,7 +186,8 @@ __device__ __forceinline__ void teacher_softmax(const DistillArgs& a, const Row&
 }
 
 // Whether entry j is the first with its id; ids are looked through only where one is repeated.
-__device__ __forceinline__ bool is_first(const DistillShared& s, int j) {
+template <typename S>
+__device__ __forceinline__ bool is_first(const S& s, int j) {
   if (s.repeated)
     for (int i = 0; i < j; ++i)
       if (s.id[i] == s.id[j]) return false;
@@ -190,7 +195,8 @@ __device__ __forceinline__ bool is_first(const DistillShared& s, int j) {
 }
 
 // The row's loss from its sums (one warp): st, s1 over all tokens at T and at 1, rest over the unlisted ones at T.
-__device__ __forceinline__ float row_loss(const DistillArgs& a, const Row& q, const DistillShared& s, float ct,
+template <typename S>
+__device__ __forceinline__ float row_loss(const DistillArgs& a, const Row& q, const S& s, float ct,
                                           float Bt, float B1, float st, float s1, float rest) {
   const int lane = threadIdx.x & 31;
   float loss = 0.f;
@@ -242,7 +248,8 @@ __global__ void __launch_bounds__(kThreads, 3) distill_grad_kernel(DistillArgs a
   const int C = (int)cluster.num_blocks(), tid = threadIdx.x;
   if (C > 1) cluster.sync();
   const T* x;
-  const Row q = row_of<T>(a, slice, C, (int)cluster.block_rank(), x);
+  Row q = row_of<T>(a, slice, C, (int)cluster.block_rank(), blockIdx.x / C, x);
+  load_terms(a, q);
   T* g = static_cast<T*>(a.dlogits) + q.row * a.ld_grad;
   const int lo = q.lo, hi = q.hi, v0 = q.v0, k = q.k;
   const bool vec_out = row_offset(g) == row_offset(x);
@@ -417,6 +424,256 @@ __global__ void __launch_bounds__(kThreads, 3) distill_grad_kernel(DistillArgs a
   }
 }
 
+// Loss and gradient of many rows that fit a block's shared memory three times: a persistent block per SM, so that a
+// row's time is that of its arithmetic alone.  Two teams of eight warps take the rows in turn, so that one's reductions
+// fall into the other's sums; a warp for each team runs ahead, copies rows into three buffers and prepares their teachers.
+constexpr int kTeams = 2, kTeam = 256, kTeamWarps = kTeam / 32, kBuffers = 3, kTeamTeacher = 128;
+constexpr int kRowsThreads = kTeams * (kTeam + 32);
+// Barriers go by rows mod 6, the teams' and the buffers' common period: each has one team that waits on it and one that
+// arrives, row by row, so that no wait can mistake a phase for the one two before it.
+constexpr int kRing = kTeams * kBuffers;
+
+struct TeamTeacher {
+  int id[kTeamTeacher];
+  float logp[kTeamTeacher], val[kTeamTeacher];
+  float target_val, p_sum, w;
+  int repeated, tgt;
+};
+
+template <typename T, int NEXP>
+__global__ void __launch_bounds__(kRowsThreads, 1) distill_rows_kernel(DistillArgs a, int slice) {
+  pdl_enter();
+  constexpr int E = Chunk<T>::E;
+  typedef typename std::conditional<sizeof(T) == 2, uint16_t, uint32_t>::type Tag;
+  extern __shared__ __align__(128) uint4 buffers[];
+  __shared__ TeamTeacher teachers[kBuffers];
+  __shared__ float red[kTeams][4][kTeamWarps];
+  __shared__ uint64_t full[kRing], empty[kRing];
+  const int lane = threadIdx.x & 31, k = a.k;
+  const int words = slice / E;
+  if (threadIdx.x == 0) {
+    for (int r = 0; r < kRing; ++r) {
+      tma::mbar_init(&full[r], 2);  // the copy is under way (and its bytes), the teacher is there
+      tma::mbar_init(&empty[r], kTeam);
+    }
+    tma::mbar_init_fence();
+  }
+  __syncthreads();
+  // row i of the block goes to team i mod 2 and buffer i mod 3; a wait that gives up waits once more for the copy that
+  // may be under way, and leaves
+  auto give_up = [&](int i) { tma::mbar_wait(&full[i % kRing], (i / kRing) & 1); };
+  if (threadIdx.x >= kTeams * kTeam) {  // the warps that run ahead
+    int i = ((int)threadIdx.x - kTeams * kTeam) / 32;
+    for (int64_t row = blockIdx.x + (int64_t)i * gridDim.x; row < a.N; row += (int64_t)kTeams * gridDim.x, i += kTeams) {
+      const int b = i % kBuffers;
+      const T* x;
+      Row q = row_of<T>(a, slice, 1, 0, row, x);
+      load_terms(a, q);
+      int id[kTeamTeacher / 32];
+      float t[kTeamTeacher / 32], val[kTeamTeacher / 32];
+#pragma unroll
+      for (int u = 0; u < kTeamTeacher / 32; ++u) {
+        const int j = lane + 32 * u;
+        id[u] = j < k ? a.t_ids[row * k + j] : -1;
+        t[u] = j < k ? a.t_logits[row * k + j] : 0.f;
+      }
+#pragma unroll
+      for (int u = 0; u < kTeamTeacher / 32; ++u) {
+        if (id[u] < 0 || id[u] >= q.V || t[u] == -CUDART_INF_F) id[u] = -1;
+        val[u] = id[u] >= 0 ? to_f32(x[id[u]]) : 0.f;
+      }
+      const float target_val = q.hard ? to_f32(x[q.tgt]) : 0.f;
+      const int last = i - kBuffers;  // the row that had the buffer
+      if (last >= 0 && !tma::mbar_wait(&empty[last % kRing], (last / kRing) & 1)) return give_up(last);
+      const Chunks ch(q, E);
+      TeamTeacher& s = teachers[b];
+      if (lane == 0) {
+        const uint32_t bytes = (uint32_t)(ch.c1 - ch.c0) * 16;
+        tma::mbar_arrive_expect_tx(&full[i % kRing], bytes);
+        if (bytes) tma::load_1d(buffers + b * words + ch.c0, x + q.v0 + ch.c0 * E, bytes, &full[i % kRing]);
+        s.target_val = target_val;
+        s.repeated = 0;
+        s.w = q.w;
+        s.tgt = q.tgt;
+      }
+#pragma unroll
+      for (int u = 0; u < kTeamTeacher / 32; ++u) {
+        const int j = lane + 32 * u;
+        if (j < k) {
+          s.id[j] = id[u];
+          s.logp[j] = id[u] >= 0 ? __fdiv_rn(t[u], a.temperature) : -CUDART_INF_F;
+          s.val[j] = val[u];
+        }
+      }
+      __syncwarp();
+      teacher_softmax(a, q, s);
+      __syncwarp();
+      if (lane == 0) tma::mbar_arrive(&full[i % kRing]);
+    }
+    return;
+  }
+
+  const int team = (int)threadIdx.x / kTeam;
+  const int tid = (int)threadIdx.x % kTeam, warp = tid >> 5;
+  auto team_sync = [&]() { asm volatile("bar.sync %0, %1;" ::"r"(team + 1), "n"(kTeam) : "memory"); };
+  const float ct = (1.f / a.temperature) * kLog2e, c1 = kLog2e;
+  int i = team;
+  for (int64_t row = blockIdx.x + (int64_t)team * gridDim.x; row < a.N; row += (int64_t)kTeams * gridDim.x, i += kTeams) {
+    const int b = i % kBuffers;
+    const T* x;
+    Row q = row_of<T>(a, slice, 1, 0, row, x);
+    T* g = static_cast<T*>(a.dlogits) + row * a.ld_grad;
+    const bool vec_out = row_offset(g) == row_offset(x);
+    const Chunks ch(q, E);
+    const int edge = ch.edge(tid), lo = q.lo, hi = q.hi, v0 = q.v0;
+    uint4* buf4 = buffers + b * words;
+    T* buf = reinterpret_cast<T*>(buf4);
+    TeamTeacher& s = teachers[b];
+    float mx = -CUDART_INF_F, edge_val = 0.f;
+    if (edge >= 0) {
+      edge_val = to_f32(x[v0 + edge]);
+      mx = edge_val == edge_val ? edge_val : -CUDART_INF_F;
+    }
+    if (!tma::mbar_wait(&full[i % kRing], (i / kRing) & 1)) return give_up(i);
+    q.w = s.w;
+    q.tgt = s.tgt;
+    q.hard = q.tgt >= 0 && q.tgt < q.V;
+    if (edge >= 0) buf[edge] = from_f32<T>(edge_val);
+    if (q.w == 0.f) {
+      if (tid == 0) a.loss[row] = 0.f;
+      for (int c = ch.c0 + tid; c < ch.c1; c += kTeam) {
+        if (vec_out) {
+          *reinterpret_cast<uint4*>(g + v0 + c * E) = make_uint4(0, 0, 0, 0);
+        } else {
+          for (int e = 0; e < E; ++e) g[v0 + c * E + e] = from_f32<T>(0.f);
+        }
+      }
+      if (edge >= 0) g[v0 + edge] = from_f32<T>(0.f);
+      tma::fence_proxy_async();
+      tma::mbar_arrive(&empty[i % kRing]);
+      continue;
+    }
+    for (int c = ch.c0 + tid; c < ch.c1; c += kTeam) mx = fmaxf(mx, chunk_max<T>(buf4[c]));
+    mx = warp_max(mx);
+    if (lane == 0) red[team][0][warp] = mx;
+    team_sync();
+    // the listed tokens leave the sums, as in the kernel of a block per row
+    Tag* tag = reinterpret_cast<Tag*>(buf);
+    const int mine = tid < k && s.id[tid] >= 0 ? s.id[tid] - v0 : -1;  // k <= kTeamTeacher < kTeam
+    if (mine >= 0) tag[mine] = (Tag)tid;
+#pragma unroll
+    for (int w = 0; w < kTeamWarps; ++w) mx = fmaxf(mx, red[team][0][w]);
+    team_sync();
+    if (mine >= 0) {
+      if (tag[mine] != (Tag)tid) s.repeated = 1;
+      buf[mine] = from_f32<T>(-CUDART_INF_F);
+    }
+    team_sync();
+    const float nBt = -(mx * ct), nB1 = -(mx * c1);
+    float st = 0.f, s1 = 0.f, listed = 0.f;
+    constexpr bool kMix = NEXP == 2 && sizeof(T) == 2;
+    pair_t s1p = pair(0.f, 0.f);
+#pragma unroll 2
+    for (int c = ch.c0 + tid; c < ch.c1; c += kTeam) {
+      float f[E];
+      Chunk<T>::unpack(buf4[c], f);
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        st += ex2(fmaf(f[e], ct, nBt));
+        if (NEXP == 2 && !kMix) s1 += ex2(fmaf(f[e], c1, nB1));
+      }
+      if (kMix) {
+#pragma unroll
+        for (int e = 0; e < E; e += 2)
+          s1p = add_pair(s1p, exp2_pair(fma_pair(pair(f[e], f[e + 1]), pair(c1, c1), pair(nB1, nB1))));
+      }
+    }
+    if (kMix) s1 = both(s1p).x + both(s1p).y;
+    if (edge >= 0) {
+      const float f = to_f32(buf[edge]);
+      st += ex2(fmaf(f, ct, nBt));
+      if (NEXP == 2) s1 += ex2(fmaf(f, c1, nB1));
+    }
+    const bool own = mine >= 0 && is_first(s, tid);
+    if (own) {
+      listed = ex2(fmaf(s.val[tid], ct, nBt));
+      if (NEXP == 2) s1 += ex2(fmaf(s.val[tid], c1, nB1));
+    }
+    st = warp_sum(st);
+    s1 = warp_sum(s1);
+    listed = warp_sum(listed);
+    if (lane == 0) {
+      red[team][1][warp] = st;
+      red[team][2][warp] = s1;
+      red[team][3][warp] = listed;
+    }
+    team_sync();
+    st = s1 = listed = 0.f;
+#pragma unroll
+    for (int w = 0; w < kTeamWarps; ++w) {
+      st += red[team][1][w];
+      s1 += red[team][2][w];
+      listed += red[team][3][w];
+    }
+    const float rest = st;
+    st += listed;
+    if (NEXP == 1 || st != st) s1 = st;
+    const float P = s.p_sum;
+    const bool soft = P != -1.f;
+    const float pr = soft && a.t_lse ? fmaxf(0.f, 1.f - P) : 0.f;
+    const float scale = q.w * a.grad_scale;
+    const float ks = soft ? scale * a.alpha * a.temperature : 0.f, kh = q.hard ? scale * (1.f - a.alpha) : 0.f;
+    const float qt = soft ? ks * (P + pr) / st : 0.f;
+    const float qr = pr > 0.f ? qt - ks * pr / rest : qt;
+    const float q1 = q.hard ? kh / s1 : 0.f;
+    const float qm = NEXP == 1 ? qr + q1 : qr;
+    auto value = [&](float f) {
+      float r = qm * ex2(fmaf(f, ct, nBt));
+      if (NEXP == 2) r = fmaf(q1, ex2(fmaf(f, c1, nB1)), r);
+      return r;
+    };
+    if (vec_out) {
+#pragma unroll 2
+      for (int c = ch.c0 + tid; c < ch.c1; c += kTeam) {
+        float f[E];
+        Chunk<T>::unpack(buf4[c], f);
+#pragma unroll
+        for (int e = 0; e < E; ++e) f[e] = value(f[e]);
+        *reinterpret_cast<uint4*>(g + v0 + c * E) = Chunk<T>::pack(f);
+      }
+    } else {
+      for (int p = ch.c0 * E + tid; p < ch.c1 * E; p += kTeam) g[v0 + p] = from_f32<T>(value(to_f32(buf[p])));
+    }
+    if (edge >= 0) g[v0 + edge] = from_f32<T>(value(to_f32(buf[edge])));
+    if (warp == kTeamWarps - 1) {
+      const float loss = row_loss(a, q, s, ct, -nBt, -nB1, st, s1, rest);
+      if (lane == 0) a.loss[row] = loss;
+    }
+    team_sync();
+    if (own) {
+      const int id = s.id[tid];
+      float p = expf(s.logp[tid]);
+      if (s.repeated)
+        for (int j = tid + 1; j < k; ++j)
+          if (s.id[j] == id) p += expf(s.logp[j]);
+      float r = qt * ex2(fmaf(s.val[tid], ct, nBt)) - ks * p;
+      if (q.hard) {
+        r += q1 * ex2(fmaf(s.val[tid], c1, nB1));
+        if (id == q.tgt) r -= kh;
+      }
+      g[id] = from_f32<T>(r);
+    }
+    if (q.hard && warp == kTeamWarps - 1) {
+      bool listed_too = false;
+      for (int j = lane; j < k; j += 32) listed_too |= s.id[j] == q.tgt;
+      if (!__any_sync(0xffffffffu, listed_too) && lane == 0)
+        g[q.tgt] = from_f32<T>(qr * ex2(fmaf(s.target_val, ct, nBt)) + q1 * ex2(fmaf(s.target_val, c1, nB1)) - kh);
+    }
+    tma::fence_proxy_async();  // this row's marks before the next row's copy
+    tma::mbar_arrive(&empty[i % kRing]);
+  }
+}
+
 // The loss alone: the row streams through registers, each thread keeping the largest logit it has seen and its sums
 // relative to that.  Where the teacher's remaining mass counts, a bit per token tells which are listed.
 template <typename T, int NEXP>
@@ -429,7 +686,8 @@ __global__ void __launch_bounds__(kThreads, 6) distill_loss_kernel(DistillArgs a
   const int C = (int)cluster.num_blocks(), tid = threadIdx.x;
   if (C > 1) cluster.sync();
   const T* x;
-  const Row q = row_of<T>(a, slice, C, (int)cluster.block_rank(), x);
+  Row q = row_of<T>(a, slice, C, (int)cluster.block_rank(), blockIdx.x / C, x);
+  load_terms(a, q);
   const int lo = q.lo, hi = q.hi, v0 = q.v0, k = q.k;
   if (q.w == 0.f) {
     if (q.rank == 0 && tid == 0) a.loss[q.row] = 0.f;
@@ -594,6 +852,14 @@ cudaError_t distill_t(const DistillArgs& a, cudaStream_t st) {
   const unsigned grid = (unsigned)(a.N * C);
   const bool two = a.targets && a.temperature != 1.f;
   LaunchScope scope_(a.dlogits ? "distill_grad" : "distill_loss", st);
+  // rows that three buffers hold, enough of them that every SM gets several
+  const size_t rows_smem = (size_t)kBuffers * slice_of(1) * sizeof(T);
+  if (a.dlogits && C == 1 && a.k <= kTeamTeacher && a.N >= 4 * kSMs && rows_smem <= 200 * 1024) {
+    auto kern = two ? distill_rows_kernel<T, 2> : distill_rows_kernel<T, 1>;
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)rows_smem);
+    if (e != cudaSuccess) return e;
+    return launch_k(kern, dim3(kSMs), dim3(kRowsThreads), rows_smem, st, a, slice);
+  }
   if (a.dlogits) {
     const size_t smem = (size_t)slice * sizeof(T);
     return two ? launch_clusters(distill_grad_kernel<T, 2>, grid, C, kThreads, smem, st, a, slice)
@@ -605,6 +871,9 @@ cudaError_t distill_t(const DistillArgs& a, cudaStream_t st) {
 }
 
 }  // namespace
+
+cudaError_t read_and_clear_distill_timeout(int* flag, cudaStream_t st) { return tma::read_and_clear_wait_timeout(flag, st); }
+cudaError_t set_distill_wait_limit(unsigned long long ns) { return tma::set_wait_limit(ns); }
 
 cudaError_t launch_distill(const DistillArgs& a, int dtype, cudaStream_t st) {
   if (a.N == 0) return cudaSuccess;

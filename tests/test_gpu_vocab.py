@@ -326,7 +326,8 @@ PERR = 100 * U
                                                  (5, 1000, 8, 1.0, 0.7, True, False), (4, 2053, 64, 0.7, 1.0, False, True),
                                                  (200, 311, 16, 3.0, 0.3, True, True), (2, 32768, 100, 2.0, 0.5, True, False),
                                                  (3, 50021, 512, 1.0, 0.9, True, True), (1, 131073, 33, 1.5, 0.5, True, True),
-                                                 (2, 262144, 4, 1.0, 0.0, True, False)])
+                                                 (2, 262144, 4, 1.0, 0.0, True, False), (600, 517, 20, 2.0, 0.6, True, True),
+                                                 (593, 1024, 128, 1.0, 1.0, False, False), (601, 2053, 129, 0.8, 0.5, True, False)])
 def test_distill(cuda_ok, dt, N, V, k, T, a, hard, tail):
     g = gen(V + k)
     x = (3 * torch.randn(N, V, generator=g, device=DEV)).to(dt)
@@ -367,6 +368,27 @@ def test_distill(cuda_ok, dt, N, V, k, T, a, hard, tail):
     z = x.clone()
     l2, g2 = S.distill_loss_and_grad(z, ids, tl, tg, T, a, w, lse, grad_scale=0.5, out=z)  # over the logits
     assert g2 is z and torch.equal(l2, loss) and torch.equal(z, grad)
+
+
+@pytest.mark.parametrize("dt", [F32, BF16])
+def test_distill_many_rows(cuda_ok, dt):
+    """Rows enough that every block has many, and half of them without weight, so that one half of a block runs ahead
+    of the other: the same as the rows in calls of their own (other kernels, so up to rounding)."""
+    N, V, k = 4000, 700, 9
+    g = gen(77)
+    x = (3 * torch.randn(N, V, generator=g, device=DEV)).to(dt)
+    ids = torch.randint(-1, V, (N, k), generator=g, device=DEV, dtype=torch.int32)
+    tl = torch.randn(N, k, generator=g, device=DEV)
+    tg = torch.randint(-1, V, (N,), generator=g, device=DEV, dtype=torch.int32)
+    w = (torch.rand(N, generator=g, device=DEV) > 0.5).float()
+    w[::5] = 0.0
+    for T in (1.0, 2.0):
+        loss, grad = S.distill_loss_and_grad(x, ids, tl, tg, T, 0.5, w)
+        for lo in range(0, N, 500):
+            part = slice(lo, lo + 500)
+            l2, g2 = S.distill_loss_and_grad(x[part], ids[part], tl[part], tg[part], T, 0.5, w[part])
+            assert torch.allclose(loss[part], l2, rtol=PERR, atol=PERR)
+            assert torch.allclose(grad[part].float(), g2.float(), rtol=H if dt == BF16 else PERR, atol=PERR)
 
 
 def test_distill_strides_and_values(cuda_ok):
