@@ -427,6 +427,7 @@ __global__ void __launch_bounds__(kThreads, 3) distill_grad_kernel(DistillArgs a
 // Loss and gradient of many rows that fit a block's shared memory three times: a persistent block per SM, so that a
 // row's time is that of its arithmetic alone.  Two teams of eight warps take the rows in turn, so that one's reductions
 // fall into the other's sums; a warp for each team runs ahead, copies rows into three buffers and prepares their teachers.
+
 constexpr int kTeams = 2, kTeam = 256, kTeamWarps = kTeam / 32, kBuffers = 3, kTeamTeacher = 128;
 constexpr int kRowsThreads = kTeams * (kTeam + 32);
 // Barriers go by rows mod 6, the teams' and the buffers' common period: each has one team that waits on it and one that
@@ -573,7 +574,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) distill_rows_kernel(DistillAr
     float st = 0.f, s1 = 0.f, listed = 0.f;
     constexpr bool kMix = NEXP == 2 && sizeof(T) == 2;
     pair_t s1p = pair(0.f, 0.f);
-#pragma unroll 2
+#pragma unroll 4
     for (int c = ch.c0 + tid; c < ch.c1; c += kTeam) {
       float f[E];
       Chunk<T>::unpack(buf4[c], f);
@@ -633,7 +634,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) distill_rows_kernel(DistillAr
       return r;
     };
     if (vec_out) {
-#pragma unroll 2
+#pragma unroll 4
       for (int c = ch.c0 + tid; c < ch.c1; c += kTeam) {
         float f[E];
         Chunk<T>::unpack(buf4[c], f);
