@@ -125,36 +125,34 @@ __device__ __forceinline__ float ruled(float x, uint32_t w, const RowRules& q, c
   return x;
 }
 
-// The rules on a thread's E elements f (tokens x[0 .. E)), whose words are its own.  Marked tokens are few but for the
-// commonest ones, so each lane takes its marked elements one after the other, through their places in shared memory:
-// all E of them under predicates took 1.5 times as long over 256 rows of 32,768 after 2,048 tokens.
-template <typename T, int E>
-__device__ __forceinline__ void rule_chunk(float* f, const T* x, uint32_t* word, const RowRules& q, const float* bias) {
-  uint32_t marked = 0;
+// The rules on a thread's E elements f, whose words are at `word`.  Marked tokens are few but for the commonest ones: most
+// warps leave at the first test.
+template <int E>
+__device__ __forceinline__ void rule_chunk(float* f, const uint32_t* word, const RowRules& q, const float* bias) {
+  uint4 w[E / 4];
+  uint32_t any = 0;
 #pragma unroll
-  for (int e = 0; e < E; e += 4) {
-    const uint4 w = *reinterpret_cast<const uint4*>(word + e);
-    marked |= (uint32_t)(w.x != 0) << e | (uint32_t)(w.y != 0) << (e + 1) | (uint32_t)(w.z != 0) << (e + 2) |
-              (uint32_t)(w.w != 0) << (e + 3);
+  for (int k = 0; k < E / 4; ++k) {
+    w[k] = *reinterpret_cast<const uint4*>(word + 4 * k);
+    any |= w[k].x | w[k].y | w[k].z | w[k].w;
   }
-  for (uint32_t left = marked; left; left &= left - 1) {
-    const int e = __ffs(left) - 1;
-    word[e] = __float_as_uint(ruled(to_f32(x[e]), word[e], q, bias));
-  }
-  if (marked) {
+  if (!any) return;
 #pragma unroll
-    for (int e = 0; e < E; ++e)
-      if ((marked >> e) & 1) f[e] = __uint_as_float(word[e]);
+  for (int k = 0; k < E / 4; ++k) {
+    if (w[k].x) f[4 * k] = ruled(f[4 * k], w[k].x, q, bias);
+    if (w[k].y) f[4 * k + 1] = ruled(f[4 * k + 1], w[k].y, q, bias);
+    if (w[k].z) f[4 * k + 2] = ruled(f[4 * k + 2], w[k].z, q, bias);
+    if (w[k].w) f[4 * k + 3] = ruled(f[4 * k + 3], w[k].w, q, bias);
   }
 }
 
-// Mask bits of the E tokens from v on (v >= 0, v < V).
+// Mask bits of the E tokens from v on (v >= 0, v < V); the bits above them are set.
 template <int E>
 __device__ __forceinline__ uint32_t mask_bits(const uint32_t* mask, int v, int V) {
   const int w = v >> 5, s = v & 31;
   const uint32_t lo = __ldg(mask + w);
   const uint32_t hi = (s > 32 - E && ((int64_t)w + 1) * 32 < V) ? __ldg(mask + w + 1) : 0u;
-  return __funnelshift_r(lo, hi, s);
+  return __funnelshift_r(lo, hi, s) | ~((1u << E) - 1);
 }
 
 // ------------------------------------------------------------------------------------------------------- process
@@ -201,7 +199,7 @@ __global__ void __launch_bounds__(kProcessThreads, 4) process_kernel(sdm_logit_r
     if (whole && aligned_out) {
       float f[E];
       Chunk<T>::unpack(raw[k], f);
-      if (q.marks) rule_chunk<T, E>(f, x + v, word + i, q, bias);
+      if (q.marks) rule_chunk<E>(f, word + i, q, bias);
       if (q.mask) {
 #pragma unroll
         for (int e = 0; e < E; ++e)
@@ -420,18 +418,22 @@ template <int NT, typename Cluster, typename F>
 __device__ uint32_t list_tokens(Cluster& cluster, ChooseShared& s, const float* y, int lo, int hi, int v0, F take) {
   if (threadIdx.x == 0) s.list_n = 0;
   __syncthreads();
-  auto one = [&](float v, int i) {
-    if (take(v) && i >= lo && i < hi) {
-      const uint32_t at = atomicAdd(&s.list_n, 1u);
-      if (at < kList) s.list[at] = (u64)order_key(v) << 32 | (0xffffffffu - (uint32_t)(v0 + i));
+#pragma unroll 2
+  for (int i0 = threadIdx.x * 4; i0 < hi; i0 += NT * 4) {
+    const float4 q = *reinterpret_cast<const float4*>(y + i0);
+    const float v[4] = {q.x, q.y, q.z, q.w};
+    uint32_t in = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) in |= (uint32_t)take(v[e]) << e;
+    if (!in) continue;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int i = i0 + e;
+      if (((in >> e) & 1) && i >= lo && i < hi) {
+        const uint32_t at = atomicAdd(&s.list_n, 1u);
+        if (at < kList) s.list[at] = (u64)order_key(v[e]) << 32 | (0xffffffffu - (uint32_t)(v0 + i));
+      }
     }
-  };
-  for (int i = threadIdx.x * 4; i < hi; i += NT * 4) {
-    const float4 v = *reinterpret_cast<const float4*>(y + i);
-    one(v.x, i);
-    one(v.y, i + 1);
-    one(v.z, i + 2);
-    one(v.w, i + 3);
   }
   __syncthreads();
   if (threadIdx.x < cluster.num_blocks()) *cluster.map_shared_rank(&s.listed[cluster.block_rank()], threadIdx.x) = s.list_n;
@@ -453,12 +455,16 @@ __device__ void sort_lists(Cluster& cluster, ChooseShared& s, uint32_t n) {
     at += k;
   }
   __syncthreads();
-  for (uint32_t i = threadIdx.x; i < n; i += NT) {
-    const u64 mine = s.list[i];
+  // a token's rank is the number of larger ones, counted by four lanes
+  for (uint32_t i0 = 0; i0 < n; i0 += NT / 4) {
+    const uint32_t i = i0 + threadIdx.x / 4;
+    const u64 mine = i < n ? s.list[i] : 0;
     uint32_t rank = 0;
-#pragma unroll 4
-    for (uint32_t j = 0; j < n; ++j) rank += s.list[j] > mine;
-    s.sorted[rank] = mine;
+#pragma unroll 8
+    for (uint32_t j = threadIdx.x & 3; j < n; j += 4) rank += s.list[j] > mine;
+    rank += __shfl_xor_sync(0xffffffffu, rank, 1);
+    rank += __shfl_xor_sync(0xffffffffu, rank, 2);
+    if (i < n && (threadIdx.x & 3) == 0) s.sorted[rank] = mine;
   }
   __syncthreads();
 }
@@ -476,6 +482,7 @@ __device__ u64 scan_sorted(ChooseShared& s, const Masses& M, uint32_t n, u64& w0
   __syncthreads();
   u64 before = run - w0 - w1;
   all = 0;
+#pragma unroll 8
   for (int w = 0; w < (NT / 32); ++w) {
     if (w < warp) before += s.warp64[w];
     all += s.warp64[w];
@@ -664,7 +671,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) choose_kernel(sdm_logit_rules r
             if (i + e >= lo && i + e < hi && !((q.mask[(v + e) >> 5] >> ((v + e) & 31)) & 1)) bits &= ~(1u << e);
         }
       }
-      if (q.marks) rule_chunk<T, E>(f, x + v, word + i, q, bias);
+      if (q.marks) rule_chunk<E>(f, word + i, q, bias);
       if (bits != 0xffffffffu) {
 #pragma unroll
         for (int e = 0; e < E; ++e)
