@@ -734,11 +734,11 @@ cudaError_t launch_few(const int32_t* ids, const T* dout, int64_t ld, int64_t N,
                        int accumulate, G* grad, cudaStream_t st) {
   const int col_blocks = (int)ceil_div(d, 32 * VEC);
   int64_t blocks = std::max(ceil_div(N * col_blocks, 8), accumulate ? (int64_t)1 : ceil_div(V, 8));
-  blocks = std::max(std::min(blocks, (int64_t)kSMs * 8), ceil_div(V, 32768));  // eight blocks per SM; a block's flags
+  blocks = std::min(blocks, (int64_t)kSMs * 8);  // eight blocks per SM
   const int share = (int)ceil_div(V, blocks);
   const bool whole = (int64_t)d * sizeof(G) % 16 == 0 && (reinterpret_cast<uintptr_t>(grad) & 15) == 0;
   LaunchScope scope_("embed_grad_few", st);
-  return launch_k(few_kernel<T, G, VEC>, dim3((unsigned)blocks), dim3(256), (size_t)share, st, ids, dout, ld,
+  return launch_k(few_kernel<T, G, VEC>, dim3((unsigned)blocks), dim3(256), accumulate ? 0 : (size_t)share, st, ids, dout, ld,
                   (int)N, d, V, col_blocks, share, whole ? (int)((int64_t)d * sizeof(G) / 16) : 0, scale, padding_id,
                   accumulate, grad);
 }

@@ -498,7 +498,7 @@ def grad64(ids, dout, V, scale, skip):
 @pytest.mark.parametrize("N,V,d,kind", [(0, 5, 8, "any"), (1, 1, 1, "any"), (1, 200, 768, "any"), (33, 1, 16, "any"),
                                         (31, 3, 24, "any"), (500, 40, 33, "any"), (3000, 2000, 64, "zipf"),
                                         (5000, 300, 330, "zipf"), (4096, 130, 258, "runs"), (2000, 70000, 12, "any"),
-                                        (1037, 9, 768, "one"), (700, 140000, 8, "any"), (300, 5, 20, "one"),
+                                        (1037, 9, 768, "one"), (700, 140000, 8, "any"), (3, 1000000, 2, "any"), (300, 5, 20, "one"),
                                         (250, 70, 6, "one"), (65536, 1000, 8, "zipf"), (65537, 40000, 4, "any"),
                                         (70001, 300, 8, "zipf"), (80000, 12, 5, "one")])
 def test_embed_grad(cuda_ok, dt, gdt, N, V, d, kind):
@@ -542,6 +542,40 @@ def test_embed_autograd(cuda_ok):
     got = (E.grad.double() * E.detach().double()).sum()
     assert abs(got - want) <= 20 * U * (2.0 * E.detach().double()[ids] * c.double()).abs().sum()
     assert E.grad[7].abs().sum() == 0
+
+
+def test_offsets_beyond_32_bits(cuda_ok):
+    """Rows that lie beyond 2^31 elements give what they give by themselves."""
+    V, k = 32768, 5
+    N = 2 ** 31 // V + 40
+    x = torch.randn(N, V, generator=gen(1), device=DEV, dtype=BF16)
+    last = slice(N - 7, N)
+    ids = torch.randint(0, V, (N, k), generator=gen(2), device=DEV, dtype=torch.int32)
+    tl = torch.randn(N, k, generator=gen(3), device=DEV)
+    r = S.LogitRules(bias_ids=ids, bias_values=tl)
+    y = S.process_logits(x, r)
+    assert torch.equal(y[last], S.process_logits(x[last].clone(), S.LogitRules(bias_ids=ids[last], bias_values=tl[last])))
+    del y
+    want = S.sample_logits(x[last].clone(), temperature=0.0)[0]
+    assert torch.equal(S.sample_logits(x, temperature=0.0)[0][last], want)
+    l2, g2 = S.distill_loss_and_grad(x[last].clone(), ids[last], tl[last], temperature=1.5)
+    l0 = S.distill_loss(x, ids, tl, temperature=1.5, reduction="none")[last]
+    l1, g1 = S.distill_loss_and_grad(x, ids, tl, temperature=1.5, out=x)
+    assert torch.allclose(l0, l2, rtol=PERR) and torch.allclose(l1[last], l2, rtol=PERR)
+    assert torch.allclose(g1[last].float(), g2.float(), rtol=H, atol=PERR)
+    del x, g1
+    d = 768
+    N = 2 ** 31 // d + 40
+    dout = torch.randn(N, d, generator=gen(4), device=DEV, dtype=BF16)
+    tok = torch.zeros(N, dtype=torch.int32, device=DEV)
+    tok[-3:] = 7
+    tok[5] = 9
+    got = S.embed_grad(tok, dout, 20)
+    want = dout[-3:].float()
+    assert torch.equal(got[7], want[0] + want[1] + want[2]) and torch.equal(got[9], dout[5].float())
+    table = torch.randn(20, d, generator=gen(5), device=DEV).to(BF16)
+    del dout
+    assert torch.equal(S.embed_tokens(tok, table)[-1], table[7])
 
 
 # ------------------------------------------------------------------------------------------------------- streams
