@@ -17,11 +17,11 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kThreads = 256, kWarps = kThreads / 32;
+constexpr int kMaxWarps = 8;  // a block has NT = 64, 128 or 256 threads
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 struct DistillShared {
-  float warp[4][kWarps];
+  float warp[4][kMaxWarps];
   float part[4][kMaxCluster];     // by block: max, sums
   int id[kMaxTeacher];            // the row's entries, -1 where unused
   float logp[kMaxTeacher], val[kMaxTeacher];
@@ -94,6 +94,7 @@ __device__ __forceinline__ float chunk_max<bf16_t>(uint4 u) {
 }
 
 // Sum of up to three values over the block, each in the same order in every thread.
+template <int NT>
 __device__ __forceinline__ void block_sum3(DistillShared& s, float& a, float& b, float& c) {
   a = warp_sum(a);
   b = warp_sum(b);
@@ -106,7 +107,7 @@ __device__ __forceinline__ void block_sum3(DistillShared& s, float& a, float& b,
   __syncthreads();
   a = b = c = 0.f;
 #pragma unroll
-  for (int w = 0; w < kWarps; ++w) {
+  for (int w = 0; w < (NT / 32); ++w) {
     a += s.warp[1][w];
     b += s.warp[2][w];
     c += s.warp[3][w];
@@ -144,9 +145,9 @@ __device__ __forceinline__ void load_terms(const DistillArgs& a, Row& q) {
 }
 
 // The row's entries and the logits they point at (every block of a cluster takes all of them).
-template <typename T>
+template <int NT, typename T>
 __device__ __forceinline__ void load_teacher(const DistillArgs& a, const Row& q, const T* x, DistillShared& s) {
-  for (int j = threadIdx.x; j < q.k; j += kThreads) {
+  for (int j = threadIdx.x; j < q.k; j += NT) {
     int id = a.t_ids[q.row * q.k + j];
     const float t = a.t_logits[q.row * q.k + j];
     if (id < 0 || id >= q.V || t == -CUDART_INF_F) id = -1;
@@ -154,7 +155,7 @@ __device__ __forceinline__ void load_teacher(const DistillArgs& a, const Row& q,
     s.logp[j] = id >= 0 ? __fdiv_rn(t, a.temperature) : -CUDART_INF_F;
     s.val[j] = id >= 0 ? to_f32(x[id]) : 0.f;
   }
-  if (threadIdx.x == kThreads - 1) s.target_val = q.hard ? to_f32(x[q.tgt]) : 0.f;
+  if (threadIdx.x == NT - 1) s.target_val = q.hard ? to_f32(x[q.tgt]) : 0.f;
 }
 
 // One warp: log p of each entry, and their sum (-1: the row has no entry).
@@ -236,8 +237,8 @@ struct Chunks {
 };
 
 // Loss and gradient.  NEXP 2: the exponentials at T and at 1 differ and both are wanted; 1: one serves.
-template <typename T, int NEXP>
-__global__ void __launch_bounds__(kThreads, 3) distill_grad_kernel(DistillArgs a, int slice) {
+template <typename T, int NEXP, int NT>
+__global__ void __launch_bounds__(NT, 768 / NT) distill_grad_kernel(DistillArgs a, int slice) {
   pdl_enter();
   constexpr int E = Chunk<T>::E;
   typedef typename std::conditional<sizeof(T) == 2, uint16_t, uint32_t>::type Tag;
@@ -257,7 +258,7 @@ __global__ void __launch_bounds__(kThreads, 3) distill_grad_kernel(DistillArgs a
   const int edge = ch.edge(tid);  // at most one token of the ragged chunks per thread
 
   // the row into shared memory, all of it on its way at once
-  for (int c = ch.c0 + tid; c < ch.c1; c += kThreads)
+  for (int c = ch.c0 + tid; c < ch.c1; c += NT)
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(buf4 + c)),
                  "l"(x + v0 + c * E)
                  : "memory");
@@ -265,7 +266,7 @@ __global__ void __launch_bounds__(kThreads, 3) distill_grad_kernel(DistillArgs a
     asm volatile("cp.async.wait_all;" ::: "memory");
     if (q.rank == 0 && tid == 0) a.loss[q.row] = 0.f;
     const uint4 zero = make_uint4(0, 0, 0, 0);
-    for (int c = ch.c0 + tid; c < ch.c1; c += kThreads) {
+    for (int c = ch.c0 + tid; c < ch.c1; c += NT) {
       if (vec_out) {
         *reinterpret_cast<uint4*>(g + v0 + c * E) = zero;
       } else {
@@ -276,7 +277,7 @@ __global__ void __launch_bounds__(kThreads, 3) distill_grad_kernel(DistillArgs a
     return;
   }
 
-  load_teacher(a, q, x, s);
+  load_teacher<NT>(a, q, x, s);
   float mx = -CUDART_INF_F;
   if (edge >= 0) {
     const T v = x[v0 + edge];
@@ -285,7 +286,7 @@ __global__ void __launch_bounds__(kThreads, 3) distill_grad_kernel(DistillArgs a
     if (mx != mx) mx = -CUDART_INF_F;
   }
   asm volatile("cp.async.wait_all;" ::: "memory");
-  for (int c = ch.c0 + tid; c < ch.c1; c += kThreads) mx = fmaxf(mx, chunk_max<T>(buf4[c]));  // its own copies
+  for (int c = ch.c0 + tid; c < ch.c1; c += NT) mx = fmaxf(mx, chunk_max<T>(buf4[c]));  // its own copies
   mx = warp_max(mx);
   if ((tid & 31) == 0) s.warp[0][tid >> 5] = mx;
   if (tid == 0) s.repeated = 0;
@@ -294,15 +295,15 @@ __global__ void __launch_bounds__(kThreads, 3) distill_grad_kernel(DistillArgs a
   // others is a sum of its own and no difference.  Each entry first writes its number in its token's place: one that
   // does not find it again is not alone.
   Tag* tag = reinterpret_cast<Tag*>(buf);
-  for (int j = tid; j < k; j += kThreads) {
+  for (int j = tid; j < k; j += NT) {
     const int i = s.id[j] - v0;
     if (s.id[j] >= 0 && i >= lo && i < hi) tag[i] = (Tag)j;
   }
 #pragma unroll
-  for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, s.warp[0][w]);
-  if (tid >= kThreads - 32) teacher_softmax(a, q, s);
+  for (int w = 0; w < (NT / 32); ++w) mx = fmaxf(mx, s.warp[0][w]);
+  if (tid >= NT - 32) teacher_softmax(a, q, s);
   __syncthreads();
-  for (int j = tid; j < k; j += kThreads) {
+  for (int j = tid; j < k; j += NT) {
     const int i = s.id[j] - v0;
     if (s.id[j] < 0 || i < lo || i >= hi) continue;
     if (tag[i] != (Tag)j) s.repeated = 1;
@@ -320,11 +321,12 @@ __global__ void __launch_bounds__(kThreads, 3) distill_grad_kernel(DistillArgs a
   const float ct = q.inv_t * kLog2e, c1 = kLog2e, nBt = -(mx * ct), nB1 = -(mx * c1);
   float st = 0.f, s1 = 0.f, listed = 0.f;
   // Four exponentials per bfloat16 logit would take the exponential unit longer than memory takes for the logit and
-  // its gradient: one of the four goes to the FMA pipe.
+  // its gradient: half of those at T = 1 go to the FMA pipe here, and a quarter below (16,384 rows of 32,768: 558 us; all
+  // of these here and none below 590).
   constexpr bool kMix = NEXP == 2 && sizeof(T) == 2;
   pair_t s1p = pair(0.f, 0.f);
 #pragma unroll 2
-  for (int c = ch.c0 + tid; c < ch.c1; c += kThreads) {
+  for (int c = ch.c0 + tid; c < ch.c1; c += NT) {
     float f[E];
     Chunk<T>::unpack(buf4[c], f);
 #pragma unroll
@@ -334,23 +336,29 @@ __global__ void __launch_bounds__(kThreads, 3) distill_grad_kernel(DistillArgs a
     }
     if (kMix) {
 #pragma unroll
-      for (int e = 0; e < E; e += 2)
-        s1p = add_pair(s1p, exp2_pair(fma_pair(pair(f[e], f[e + 1]), pair(c1, c1), pair(nB1, nB1))));
+      for (int e = 0; e < E; e += 2) {
+        if (e % 4) {
+          s1p = add_pair(s1p, exp2_pair(fma_pair(pair(f[e], f[e + 1]), pair(c1, c1), pair(nB1, nB1))));
+        } else {
+          s1 += ex2(fmaf(f[e], c1, nB1));
+          s1 += ex2(fmaf(f[e + 1], c1, nB1));
+        }
+      }
     }
   }
-  if (kMix) s1 = both(s1p).x + both(s1p).y;
+  if (kMix) s1 += both(s1p).x + both(s1p).y;
   if (edge >= 0) {
     const float f = to_f32(buf[edge]);
     st += ex2(fmaf(f, ct, nBt));
     if (NEXP == 2) s1 += ex2(fmaf(f, c1, nB1));
   }
-  for (int j = tid; j < k; j += kThreads) {
+  for (int j = tid; j < k; j += NT) {
     const int i = s.id[j] - v0;
     if (s.id[j] < 0 || i < lo || i >= hi || !is_first(s, j)) continue;
     listed += ex2(fmaf(s.val[j], ct, nBt));
     if (NEXP == 2) s1 += ex2(fmaf(s.val[j], c1, nB1));
   }
-  block_sum3(s, st, s1, listed);
+  block_sum3<NT>(s, st, s1, listed);
   if (C > 1) {
     if (tid < C) {
       *cluster.map_shared_rank(&s.part[1][q.rank], tid) = st;
@@ -386,23 +394,35 @@ __global__ void __launch_bounds__(kThreads, 3) distill_grad_kernel(DistillArgs a
   };
   if (vec_out) {
 #pragma unroll 2
-    for (int c = ch.c0 + tid; c < ch.c1; c += kThreads) {
+    for (int c = ch.c0 + tid; c < ch.c1; c += NT) {
       float f[E];
       Chunk<T>::unpack(buf4[c], f);
 #pragma unroll
-      for (int e = 0; e < E; ++e) f[e] = value(f[e]);
+      for (int e = 0; e < E; e += 2) {
+        if (kMix && e == 2) {
+          const float2 t = both(fma_pair(pair(f[e], f[e + 1]), pair(c1, c1), pair(nB1, nB1)));
+          float2 e1 = both(exp2_pair(pair(t.x, t.y)));
+          if (t.x < -126.f) e1.x = 0.f;  // a logit of -infinity has no gradient
+          if (t.y < -126.f) e1.y = 0.f;
+          f[e] = fmaf(q1, e1.x, qm * ex2(fmaf(f[e], ct, nBt)));
+          f[e + 1] = fmaf(q1, e1.y, qm * ex2(fmaf(f[e + 1], ct, nBt)));
+        } else {
+          f[e] = value(f[e]);
+          f[e + 1] = value(f[e + 1]);
+        }
+      }
       *reinterpret_cast<uint4*>(g + v0 + c * E) = Chunk<T>::pack(f);
     }
   } else {
-    for (int i = ch.c0 * E + tid; i < ch.c1 * E; i += kThreads) g[v0 + i] = from_f32<T>(value(to_f32(buf[i])));
+    for (int i = ch.c0 * E + tid; i < ch.c1 * E; i += NT) g[v0 + i] = from_f32<T>(value(to_f32(buf[i])));
   }
   if (edge >= 0) g[v0 + edge] = from_f32<T>(value(to_f32(buf[edge])));
-  if (q.rank == 0 && tid >= kThreads - 32) {
+  if (q.rank == 0 && tid >= NT - 32) {
     const float loss = row_loss(a, q, s, ct, -nBt, -nB1, st, s1, rest);
-    if (tid == kThreads - 1) a.loss[q.row] = loss;
+    if (tid == NT - 1) a.loss[q.row] = loss;
   }
   __syncthreads();  // the tokens with a term of their own are written over the pass above
-  for (int j = tid; j < k; j += kThreads) {
+  for (int j = tid; j < k; j += NT) {
     const int id = s.id[j];
     if (id < 0 || id - v0 < lo || id - v0 >= hi || !is_first(s, j)) continue;
     float p = expf(s.logp[j]);
@@ -646,10 +666,6 @@ __global__ void __launch_bounds__(kRowsThreads, 1) distill_rows_kernel(DistillAr
       for (int p = ch.c0 * E + tid; p < ch.c1 * E; p += kTeam) g[v0 + p] = from_f32<T>(value(to_f32(buf[p])));
     }
     if (edge >= 0) g[v0 + edge] = from_f32<T>(value(to_f32(buf[edge])));
-    if (warp == kTeamWarps - 1) {
-      const float loss = row_loss(a, q, s, ct, -nBt, -nB1, st, s1, rest);
-      if (lane == 0) a.loss[row] = loss;
-    }
     team_sync();
     if (own) {
       const int id = s.id[tid];
@@ -664,11 +680,15 @@ __global__ void __launch_bounds__(kRowsThreads, 1) distill_rows_kernel(DistillAr
       }
       g[id] = from_f32<T>(r);
     }
-    if (q.hard && warp == kTeamWarps - 1) {
-      bool listed_too = false;
-      for (int j = lane; j < k; j += 32) listed_too |= s.id[j] == q.tgt;
-      if (!__any_sync(0xffffffffu, listed_too) && lane == 0)
-        g[q.tgt] = from_f32<T>(qr * ex2(fmaf(s.target_val, ct, nBt)) + q1 * ex2(fmaf(s.target_val, c1, nB1)) - kh);
+    if (warp == kTeamWarps - 1) {
+      const float loss = row_loss(a, q, s, ct, -nBt, -nB1, st, s1, rest);
+      if (lane == 0) a.loss[row] = loss;
+      if (q.hard) {
+        bool listed_too = false;
+        for (int j = lane; j < k; j += 32) listed_too |= s.id[j] == q.tgt;
+        if (!__any_sync(0xffffffffu, listed_too) && lane == 0)
+          g[q.tgt] = from_f32<T>(qr * ex2(fmaf(s.target_val, ct, nBt)) + q1 * ex2(fmaf(s.target_val, c1, nB1)) - kh);
+      }
     }
     tma::fence_proxy_async();  // this row's marks before the next row's copy
     tma::mbar_arrive(&empty[i % kRing]);
@@ -677,8 +697,8 @@ __global__ void __launch_bounds__(kRowsThreads, 1) distill_rows_kernel(DistillAr
 
 // The loss alone: the row streams through registers, each thread keeping the largest logit it has seen and its sums
 // relative to that.  Where the teacher's remaining mass counts, a bit per token tells which are listed.
-template <typename T, int NEXP>
-__global__ void __launch_bounds__(kThreads, 6) distill_loss_kernel(DistillArgs a, int slice) {
+template <typename T, int NEXP, int NT>
+__global__ void __launch_bounds__(NT, 1536 / NT) distill_loss_kernel(DistillArgs a, int slice) {
   pdl_enter();
   constexpr int E = Chunk<T>::E, U = 4;
   extern __shared__ uint32_t is_listed[];
@@ -695,12 +715,12 @@ __global__ void __launch_bounds__(kThreads, 6) distill_loss_kernel(DistillArgs a
     return;
   }
   const bool tail = a.t_lse != nullptr;
-  load_teacher(a, q, x, s);
+  load_teacher<NT>(a, q, x, s);
   if (tail) {
-    for (int i = tid; i < (slice + 31) / 32; i += kThreads) is_listed[i] = 0;
+    for (int i = tid; i < (slice + 31) / 32; i += NT) is_listed[i] = 0;
     if (tid == 0) s.repeated = 0;
     __syncthreads();
-    for (int j = tid; j < k; j += kThreads) {
+    for (int j = tid; j < k; j += NT) {
       const int i = s.id[j] - v0;
       if (s.id[j] < 0 || i < lo || i >= hi) continue;
       const uint32_t bit = 1u << (i & 31);
@@ -713,7 +733,7 @@ __global__ void __launch_bounds__(kThreads, 6) distill_loss_kernel(DistillArgs a
   float mt = -CUDART_INF_F, nBt = 0.f, nB1 = 0.f, st = 0.f, s1 = 0.f;
   auto raise = [&](float cm) {  // the largest logit so far
     if (cm > mt) {
-      const float nt = -(cm * ct), n1 = -(cm * c1);
+      const float nt = -__fmul_rn(cm, ct), n1 = -__fmul_rn(cm, c1);
       if (mt > -CUDART_INF_F) {
         st *= ex2(nt - nBt);
         if (NEXP == 2) s1 *= ex2(n1 - nB1);
@@ -743,18 +763,18 @@ __global__ void __launch_bounds__(kThreads, 6) distill_loss_kernel(DistillArgs a
   };
   const uint4* x4 = reinterpret_cast<const uint4*>(x + v0);  // chunk c, for c in [c0, c1)
   int c = ch.c0 + tid;
-  for (; c + (U - 1) * kThreads < ch.c1; c += U * kThreads) {
+  for (; c + (U - 1) * NT < ch.c1; c += U * NT) {
     uint4 u[U];
 #pragma unroll
-    for (int j = 0; j < U; ++j) u[j] = __ldg(x4 + c + j * kThreads);
+    for (int j = 0; j < U; ++j) u[j] = __ldg(x4 + c + j * NT);
     float cm = chunk_max<T>(u[0]);
 #pragma unroll
     for (int j = 1; j < U; ++j) cm = fmaxf(cm, chunk_max<T>(u[j]));
     raise(cm);
 #pragma unroll
-    for (int j = 0; j < U; ++j) add(u[j], c + j * kThreads);
+    for (int j = 0; j < U; ++j) add(u[j], c + j * NT);
   }
-  for (; c < ch.c1; c += kThreads) {
+  for (; c < ch.c1; c += NT) {
     const uint4 u = __ldg(x4 + c);
     raise(chunk_max<T>(u));
     add(u, c);
@@ -770,26 +790,26 @@ __global__ void __launch_bounds__(kThreads, 6) distill_loss_kernel(DistillArgs a
   if ((tid & 31) == 0) s.warp[0][tid >> 5] = mx;
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, s.warp[0][w]);
-  if (tid >= kThreads - 32) teacher_softmax(a, q, s);
+  for (int w = 0; w < (NT / 32); ++w) mx = fmaxf(mx, s.warp[0][w]);
+  if (tid >= NT - 32) teacher_softmax(a, q, s);
   if (C > 1) {
     if (tid < C) *cluster.map_shared_rank(&s.part[0][q.rank], tid) = mx;
     cluster.sync();
     for (int r = 0; r < C; ++r) mx = fmaxf(mx, s.part[0][r]);
   }
   // all sums relative to the row's largest logit
-  const float Mt = mx * ct, M1 = mx * c1;
+  const float Mt = __fmul_rn(mx, ct), M1 = __fmul_rn(mx, c1);
   float listed = 0.f;
   if (mt > -CUDART_INF_F) {  // else they are 0, or NaN
     st *= ex2(-nBt - Mt);
     s1 *= ex2(-nB1 - M1);
   }
   if (tail)
-    for (int j = tid; j < k; j += kThreads) {
+    for (int j = tid; j < k; j += NT) {
       const int i = s.id[j] - v0;
       if (s.id[j] >= 0 && i >= lo && i < hi && is_first(s, j)) listed += ex2(fmaf(s.val[j], ct, -Mt));
     }
-  block_sum3(s, st, s1, listed);
+  block_sum3<NT>(s, st, s1, listed);
   if (C > 1) {
     if (tid < C) {
       *cluster.map_shared_rank(&s.part[1][q.rank], tid) = st;
@@ -839,6 +859,21 @@ __global__ void __launch_bounds__(256) scale_rows_kernel(T* __restrict__ x, int6
   }
 }
 
+template <typename T, int NT>
+cudaError_t distill_n(const DistillArgs& a, int C, int slice, cudaStream_t st) {
+  const unsigned grid = (unsigned)(a.N * C);
+  const bool two = a.targets && a.temperature != 1.f;
+  LaunchScope scope_(a.dlogits ? "distill_grad" : "distill_loss", st);
+  if (a.dlogits) {
+    const size_t smem = (size_t)slice * sizeof(T);
+    return two ? launch_clusters(distill_grad_kernel<T, 2, NT>, grid, C, NT, smem, st, a, slice)
+               : launch_clusters(distill_grad_kernel<T, 1, NT>, grid, C, NT, smem, st, a, slice);
+  }
+  const size_t smem = a.t_lse ? (size_t)(slice / 32) * 4 : 0;
+  return two ? launch_clusters(distill_loss_kernel<T, 2, NT>, grid, C, NT, smem, st, a, slice)
+             : launch_clusters(distill_loss_kernel<T, 1, NT>, grid, C, NT, smem, st, a, slice);
+}
+
 template <typename T>
 cudaError_t distill_t(const DistillArgs& a, cudaStream_t st) {
   constexpr int E = Chunk<T>::E;
@@ -850,25 +885,23 @@ cudaError_t distill_t(const DistillArgs& a, cudaStream_t st) {
   while (C < kMaxCluster && (a.N * C < kSMs || slice_of(C) * (int64_t)sizeof(T) > most)) C *= 2;
   if (a.N * C > 0x7fffffff) return cudaErrorInvalidValue;
   const int slice = slice_of(C);
-  const unsigned grid = (unsigned)(a.N * C);
-  const bool two = a.targets && a.temperature != 1.f;
-  LaunchScope scope_(a.dlogits ? "distill_grad" : "distill_loss", st);
-  // rows that three buffers hold, enough of them that every SM gets several
-  const size_t rows_smem = (size_t)kBuffers * slice_of(1) * sizeof(T);
-  if (a.dlogits && C == 1 && a.k <= kTeamTeacher && a.N >= 4 * kSMs && rows_smem <= 200 * 1024) {
-    auto kern = two ? distill_rows_kernel<T, 2> : distill_rows_kernel<T, 1>;
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)rows_smem);
+  // Rows of which three fit a block's shared memory but not many more, enough of them that every SM gets several: 16,384
+  // rows of 32,768 bfloat16 take 545 us on persistent blocks and 558 on a block per row (373 and 440 at T = 1); 32,768 rows
+  // of 16,384 take 698 and 563.
+  const size_t row_bytes = (size_t)slice * sizeof(T);
+  if (a.dlogits && C == 1 && a.k <= kTeamTeacher && a.N >= 4 * kSMs && row_bytes > 40 * 1024 &&
+      kBuffers * row_bytes <= 200 * 1024) {
+    auto kern = a.targets && a.temperature != 1.f ? distill_rows_kernel<T, 2> : distill_rows_kernel<T, 1>;
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(kBuffers * row_bytes));
     if (e != cudaSuccess) return e;
-    return launch_k(kern, dim3(kSMs), dim3(kRowsThreads), rows_smem, st, a, slice);
+    LaunchScope scope_("distill_rows", st);
+    return launch_k(kern, dim3(kSMs), dim3(kRowsThreads), kBuffers * row_bytes, st, a, slice);
   }
-  if (a.dlogits) {
-    const size_t smem = (size_t)slice * sizeof(T);
-    return two ? launch_clusters(distill_grad_kernel<T, 2>, grid, C, kThreads, smem, st, a, slice)
-               : launch_clusters(distill_grad_kernel<T, 1>, grid, C, kThreads, smem, st, a, slice);
-  }
-  const size_t smem = a.t_lse ? (size_t)(slice / 32) * 4 : 0;
-  return two ? launch_clusters(distill_loss_kernel<T, 2>, grid, C, kThreads, smem, st, a, slice)
-             : launch_clusters(distill_loss_kernel<T, 1>, grid, C, kThreads, smem, st, a, slice);
+  // few threads where rows are short, so that many blocks hide one another's reductions (65,536 rows of 8,192: 256
+  // threads 1,093 us, 128 658; 131,072 of 2,048: 1,598, 811 and with 64 752)
+  if (row_bytes <= 8448) return distill_n<T, 64>(a, C, slice, st);
+  if (row_bytes <= 33024) return distill_n<T, 128>(a, C, slice, st);
+  return distill_n<T, 256>(a, C, slice, st);
 }
 
 }  // namespace

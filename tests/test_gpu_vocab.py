@@ -4,7 +4,8 @@ vocabularies and strides, rows that a mask empties, infinities and NaN, empty an
 entries that are missing or repeated, tokens that occur thousands of times.
 
 Tolerances are bounds on rounding: u = 2^-24 per float32 operation, h = 2^-8 for one rounding to bfloat16 (twice the
-half step, so that a float32 error on a rounding boundary is covered)."""
+half step, so that a float32 error on a rounding boundary is covered); two values that are each rounded can be a whole
+step, 2 h, apart."""
 import math
 
 import numpy as np
@@ -327,6 +328,7 @@ PERR = 100 * U
                                                  (200, 311, 16, 3.0, 0.3, True, True), (2, 32768, 100, 2.0, 0.5, True, False),
                                                  (3, 50021, 512, 1.0, 0.9, True, True), (1, 131073, 33, 1.5, 0.5, True, True),
                                                  (2, 262144, 4, 1.0, 0.0, True, False), (600, 517, 20, 2.0, 0.6, True, True),
+                                                 (150, 9001, 30, 2.0, 0.5, True, False), (600, 24007, 7, 1.7, 0.5, True, True),
                                                  (593, 1024, 128, 1.0, 1.0, False, False), (601, 2053, 129, 0.8, 0.5, True, False)])
 def test_distill(cuda_ok, dt, N, V, k, T, a, hard, tail):
     g = gen(V + k)
@@ -354,15 +356,16 @@ def test_distill(cuda_ok, dt, N, V, k, T, a, hard, tail):
     loss, grad = S.distill_loss_and_grad(x, ids, tl, tg, T, a, w, lse, grad_scale=0.5)
     only = S.distill_loss(x, ids, tl, tg, T, a, w, lse, reduction="none")
     assert grad.dtype == dt and grad.shape == x.shape
+    xs, tls, grads = np64(x), np64(tl), np64(grad)
     for i in range(N):
         if float(w[i]) == 0:
             assert loss[i] == 0 and only[i] == 0 and torch.count_nonzero(grad[i]) == 0
             continue
-        wl, wg, lm, mag = distill64(np64(x)[i], ids[i].tolist(), np64(tl)[i], int(tg[i]) if hard else -1, float(w[i]),
+        wl, wg, lm, mag = distill64(xs[i], ids[i].tolist(), tls[i], int(tg[i]) if hard else -1, float(w[i]),
                                     T, a, None if lse is None else float(lse[i]))
         assert abs(float(loss[i]) - wl) <= PERR * lm + 1e-30, (i, float(loss[i]), wl)
         assert abs(float(only[i]) - wl) <= PERR * lm + 1e-30, (i, float(only[i]), wl)  # the loss without a gradient
-        got = np64(grad)[i]
+        got = grads[i]
         tol = 0.5 * PERR * mag + (H * np.abs(0.5 * wg) if dt == BF16 else 0) + 1e-37
         assert (np.abs(got - 0.5 * wg) <= tol).all(), (i, np.abs(got - 0.5 * wg).max())
     z = x.clone()
@@ -373,8 +376,8 @@ def test_distill(cuda_ok, dt, N, V, k, T, a, hard, tail):
 @pytest.mark.parametrize("dt", [F32, BF16])
 def test_distill_many_rows(cuda_ok, dt):
     """Rows enough that every block has many, and half of them without weight, so that one half of a block runs ahead
-    of the other: the same as the rows in calls of their own (other kernels, so up to rounding)."""
-    N, V, k = 4000, 700, 9
+    of the other: every row against torch in 64 bits."""
+    N, V, k, a = 3000, 22000 if dt == BF16 else 11000, 9, 0.5  # 44 KB a row
     g = gen(77)
     x = (3 * torch.randn(N, V, generator=g, device=DEV)).to(dt)
     ids = torch.randint(-1, V, (N, k), generator=g, device=DEV, dtype=torch.int32)
@@ -383,12 +386,27 @@ def test_distill_many_rows(cuda_ok, dt):
     w = (torch.rand(N, generator=g, device=DEV) > 0.5).float()
     w[::5] = 0.0
     for T in (1.0, 2.0):
-        loss, grad = S.distill_loss_and_grad(x, ids, tl, tg, T, 0.5, w)
-        for lo in range(0, N, 500):
-            part = slice(lo, lo + 500)
-            l2, g2 = S.distill_loss_and_grad(x[part], ids[part], tl[part], tg[part], T, 0.5, w[part])
-            assert torch.allclose(loss[part], l2, rtol=PERR, atol=PERR)
-            assert torch.allclose(grad[part].float(), g2.float(), rtol=H if dt == BF16 else PERR, atol=PERR)
+        loss, grad = S.distill_loss_and_grad(x, ids, tl, tg, T, a, w)
+        xd, wd = x.double(), w.double()
+        lq, l1 = torch.log_softmax(xd / T, 1), torch.log_softmax(xd, 1)
+        ok, some = ids >= 0, (ids >= 0).any(1)
+        lp = torch.log_softmax((tl.double() / T).masked_fill(~ok, -math.inf), 1)
+        p = torch.where(ok, lp.exp(), 0.0).nan_to_num()
+        at = ids.clamp(min=0).long()
+        lqa = lq.gather(1, at)
+        soft = torch.where(ok, p * (lp - lqa), 0.0).sum(1)
+        mag = torch.where(ok, p * (lp.abs() + lqa.abs() + 1), 0.0).sum(1) * a * T * T
+        G, M = lq.exp() * some[:, None], lq.exp() * some[:, None]
+        G, M = G.scatter_add(1, at, -p) * a * T, M.scatter_add(1, at, p) * a * T
+        hit, t = tg >= 0, tg.clamp(min=0).long()[:, None]
+        one = (1 - a) * hit[:, None].double()
+        lt = l1.gather(1, t)[:, 0]
+        want = wd * (a * T * T * soft - (1 - a) * torch.where(hit, lt, 0.0))
+        mag = mag + (1 - a) * torch.where(hit, lt.abs() + 1, 0.0)
+        G = wd[:, None] * (G + one * l1.exp()).scatter_add(1, t, -one)
+        M = wd[:, None] * (M + one * l1.exp()).scatter_add(1, t, one)
+        assert ((loss - want).abs() <= PERR * mag + 1e-30).all()
+        assert ((grad.double() - G).abs() <= PERR * M + (H * G.abs() if dt == BF16 else 0) + 1e-37).all()
 
 
 def test_distill_strides_and_values(cuda_ok):
@@ -404,7 +422,7 @@ def test_distill_strides_and_values(cuda_ok):
         l1, g1 = S.distill_loss_and_grad(x, ids, tl, temperature=2.0, out=out[:, 3:3 + V])
         assert out[:, :3].abs().sum() == 0 and out[:, 3 + V:].abs().sum() == 0
         # an odd start puts other elements into a thread's share: sums differ by their order only
-        assert torch.allclose(g0.float(), g1.float(), rtol=H, atol=PERR)
+        assert torch.allclose(g0.float(), g1.float(), rtol=2 * H, atol=PERR)
         assert torch.allclose(l0, l1, rtol=PERR, atol=PERR)
     # a student that excludes a token the teacher wants: infinite loss, the gradient pulls the token up
     x = torch.randn(2, 40, generator=g, device=DEV)
@@ -562,7 +580,7 @@ def test_offsets_beyond_32_bits(cuda_ok):
     l0 = S.distill_loss(x, ids, tl, temperature=1.5, reduction="none")[last]
     l1, g1 = S.distill_loss_and_grad(x, ids, tl, temperature=1.5, out=x)
     assert torch.allclose(l0, l2, rtol=PERR) and torch.allclose(l1[last], l2, rtol=PERR)
-    assert torch.allclose(g1[last].float(), g2.float(), rtol=H, atol=PERR)
+    assert torch.allclose(g1[last].float(), g2.float(), rtol=2 * H, atol=PERR)
     del x, g1
     d = 768
     N = 2 ** 31 // d + 40
