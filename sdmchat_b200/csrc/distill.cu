@@ -37,6 +37,17 @@ __device__ __forceinline__ float ex2(float t) {
   return e;
 }
 
+// How many exponentials a logit takes.  kOne: the one at T serves, as T = 1 or no hard target is given.  kTwo: one at T and
+// one at 1.  kSquare, kFourth: T = 2 or 4, so that the one at 1 is the other's square or fourth power (c and B are then
+// exactly half or a quarter of those at 1, and it leaves float32's range at the same logit).  16,384 rows of 32,768
+// bfloat16 logits with their gradient: 373 us, 554, 395, 421.
+enum Exps { kOne, kTwo, kSquare, kFourth };
+template <Exps X>
+__device__ __forceinline__ float power(float e) {
+  const float sq = e * e;
+  return X == kFourth ? sq * sq : sq;
+}
+
 // Two floats in one 64-bit register, for the paired instructions.
 typedef unsigned long long pair_t;
 __device__ __forceinline__ pair_t pair(float a, float b) {
@@ -236,8 +247,8 @@ struct Chunks {
   }
 };
 
-// Loss and gradient.  NEXP 2: the exponentials at T and at 1 differ and both are wanted; 1: one serves.
-template <typename T, int NEXP, int NT>
+// Loss and gradient.
+template <typename T, Exps X, int NT>
 __global__ void __launch_bounds__(NT, 768 / NT) distill_grad_kernel(DistillArgs a, int slice) {
   pdl_enter();
   constexpr int E = Chunk<T>::E;
@@ -323,7 +334,7 @@ __global__ void __launch_bounds__(NT, 768 / NT) distill_grad_kernel(DistillArgs 
   // Four exponentials per bfloat16 logit would take the exponential unit longer than memory takes for the logit and
   // its gradient: half of those at T = 1 go to the FMA pipe here, and a quarter below (16,384 rows of 32,768: 558 us; all
   // of these here and none below 590).
-  constexpr bool kMix = NEXP == 2 && sizeof(T) == 2;
+  constexpr bool kMix = X == kTwo && sizeof(T) == 2;
   pair_t s1p = pair(0.f, 0.f);
 #pragma unroll 2
   for (int c = ch.c0 + tid; c < ch.c1; c += NT) {
@@ -331,8 +342,10 @@ __global__ void __launch_bounds__(NT, 768 / NT) distill_grad_kernel(DistillArgs 
     Chunk<T>::unpack(buf4[c], f);
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      st += ex2(fmaf(f[e], ct, nBt));
-      if (NEXP == 2 && !kMix) s1 += ex2(fmaf(f[e], c1, nB1));
+      const float t = ex2(fmaf(f[e], ct, nBt));
+      st += t;
+      if (X == kTwo && !kMix) s1 += ex2(fmaf(f[e], c1, nB1));
+      if (X > kTwo) s1 += power<X>(t);
     }
     if (kMix) {
 #pragma unroll
@@ -350,13 +363,13 @@ __global__ void __launch_bounds__(NT, 768 / NT) distill_grad_kernel(DistillArgs 
   if (edge >= 0) {
     const float f = to_f32(buf[edge]);
     st += ex2(fmaf(f, ct, nBt));
-    if (NEXP == 2) s1 += ex2(fmaf(f, c1, nB1));
+    if (X != kOne) s1 += ex2(fmaf(f, c1, nB1));
   }
   for (int j = tid; j < k; j += NT) {
     const int i = s.id[j] - v0;
     if (s.id[j] < 0 || i < lo || i >= hi || !is_first(s, j)) continue;
     listed += ex2(fmaf(s.val[j], ct, nBt));
-    if (NEXP == 2) s1 += ex2(fmaf(s.val[j], c1, nB1));
+    if (X != kOne) s1 += ex2(fmaf(s.val[j], c1, nB1));
   }
   block_sum3<NT>(s, st, s1, listed);
   if (C > 1) {
@@ -375,7 +388,7 @@ __global__ void __launch_bounds__(NT, 768 / NT) distill_grad_kernel(DistillArgs 
   }
   const float rest = st;
   st += listed;
-  if (NEXP == 1 || st != st) s1 = st;  // a NaN or an infinity shows in st
+  if (X == kOne || st != st) s1 = st;  // a NaN or an infinity shows in st
   const float P = s.p_sum;
   const bool soft = P != -1.f;
   const float pr = soft && a.t_lse ? fmaxf(0.f, 1.f - P) : 0.f;
@@ -386,11 +399,13 @@ __global__ void __launch_bounds__(NT, 768 / NT) distill_grad_kernel(DistillArgs 
   const float qt = soft ? ks * (P + pr) / st : 0.f;          // listed
   const float qr = pr > 0.f ? qt - ks * pr / rest : qt;      // not listed
   const float q1 = q.hard ? kh / s1 : 0.f;
-  const float qm = NEXP == 1 ? qr + q1 : qr;
+  const float qm = X == kOne ? qr + q1 : qr;
   auto value = [&](float f) {
-    float r = qm * ex2(fmaf(f, ct, nBt));
-    if (NEXP == 2) r = fmaf(q1, ex2(fmaf(f, c1, nB1)), r);
-    return r;
+    const float t = ex2(fmaf(f, ct, nBt));
+    if (X == kTwo) return fmaf(q1, ex2(fmaf(f, c1, nB1)), qm * t);
+    if (X == kSquare) return t * fmaf(q1, t, qm);
+    if (X == kFourth) return fmaf(q1, power<X>(t), qm * t);
+    return qm * t;
   };
   if (vec_out) {
 #pragma unroll 2
@@ -461,7 +476,7 @@ struct TeamTeacher {
   int repeated, tgt;
 };
 
-template <typename T, int NEXP>
+template <typename T, Exps X>
 __global__ void __launch_bounds__(kRowsThreads, 1) distill_rows_kernel(DistillArgs a, int slice) {
   pdl_enter();
   constexpr int E = Chunk<T>::E;
@@ -592,7 +607,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) distill_rows_kernel(DistillAr
     team_sync();
     const float nBt = -(mx * ct), nB1 = -(mx * c1);
     float st = 0.f, s1 = 0.f, listed = 0.f;
-    constexpr bool kMix = NEXP == 2 && sizeof(T) == 2;
+    constexpr bool kMix = X == kTwo && sizeof(T) == 2;
     pair_t s1p = pair(0.f, 0.f);
 #pragma unroll 4
     for (int c = ch.c0 + tid; c < ch.c1; c += kTeam) {
@@ -600,8 +615,10 @@ __global__ void __launch_bounds__(kRowsThreads, 1) distill_rows_kernel(DistillAr
       Chunk<T>::unpack(buf4[c], f);
 #pragma unroll
       for (int e = 0; e < E; ++e) {
-        st += ex2(fmaf(f[e], ct, nBt));
-        if (NEXP == 2 && !kMix) s1 += ex2(fmaf(f[e], c1, nB1));
+        const float t = ex2(fmaf(f[e], ct, nBt));
+        st += t;
+        if (X == kTwo && !kMix) s1 += ex2(fmaf(f[e], c1, nB1));
+        if (X > kTwo) s1 += power<X>(t);
       }
       if (kMix) {
 #pragma unroll
@@ -613,12 +630,12 @@ __global__ void __launch_bounds__(kRowsThreads, 1) distill_rows_kernel(DistillAr
     if (edge >= 0) {
       const float f = to_f32(buf[edge]);
       st += ex2(fmaf(f, ct, nBt));
-      if (NEXP == 2) s1 += ex2(fmaf(f, c1, nB1));
+      if (X != kOne) s1 += ex2(fmaf(f, c1, nB1));
     }
     const bool own = mine >= 0 && is_first(s, tid);
     if (own) {
       listed = ex2(fmaf(s.val[tid], ct, nBt));
-      if (NEXP == 2) s1 += ex2(fmaf(s.val[tid], c1, nB1));
+      if (X != kOne) s1 += ex2(fmaf(s.val[tid], c1, nB1));
     }
     st = warp_sum(st);
     s1 = warp_sum(s1);
@@ -638,7 +655,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) distill_rows_kernel(DistillAr
     }
     const float rest = st;
     st += listed;
-    if (NEXP == 1 || st != st) s1 = st;
+    if (X == kOne || st != st) s1 = st;
     const float P = s.p_sum;
     const bool soft = P != -1.f;
     const float pr = soft && a.t_lse ? fmaxf(0.f, 1.f - P) : 0.f;
@@ -647,11 +664,13 @@ __global__ void __launch_bounds__(kRowsThreads, 1) distill_rows_kernel(DistillAr
     const float qt = soft ? ks * (P + pr) / st : 0.f;
     const float qr = pr > 0.f ? qt - ks * pr / rest : qt;
     const float q1 = q.hard ? kh / s1 : 0.f;
-    const float qm = NEXP == 1 ? qr + q1 : qr;
+    const float qm = X == kOne ? qr + q1 : qr;
     auto value = [&](float f) {
-      float r = qm * ex2(fmaf(f, ct, nBt));
-      if (NEXP == 2) r = fmaf(q1, ex2(fmaf(f, c1, nB1)), r);
-      return r;
+      const float t = ex2(fmaf(f, ct, nBt));
+      if (X == kTwo) return fmaf(q1, ex2(fmaf(f, c1, nB1)), qm * t);
+      if (X == kSquare) return t * fmaf(q1, t, qm);
+    if (X == kFourth) return fmaf(q1, power<X>(t), qm * t);
+      return qm * t;
     };
     if (vec_out) {
 #pragma unroll 4
@@ -697,7 +716,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) distill_rows_kernel(DistillAr
 
 // The loss alone: the row streams through registers, each thread keeping the largest logit it has seen and its sums
 // relative to that.  Where the teacher's remaining mass counts, a bit per token tells which are listed.
-template <typename T, int NEXP, int NT>
+template <typename T, Exps X, int NT>
 __global__ void __launch_bounds__(NT, 1536 / NT) distill_loss_kernel(DistillArgs a, int slice) {
   pdl_enter();
   constexpr int E = Chunk<T>::E, U = 4;
@@ -715,10 +734,18 @@ __global__ void __launch_bounds__(NT, 1536 / NT) distill_loss_kernel(DistillArgs
     return;
   }
   const bool tail = a.t_lse != nullptr;
-  load_teacher<NT>(a, q, x, s);
+  const Chunks ch(q, E);
+  // the row is on its way to L2 while its teacher is fetched (8,192 rows of 50,021: 139 us without,
+  // 132 with; 65,536 of 8,192: 340 and 311)
+  if (tid == 0 && ch.c1 > ch.c0)
+    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(x + v0 + ch.c0 * E), "r"((ch.c1 - ch.c0) * 16)
+                 : "memory");
   if (tail) {
     for (int i = tid; i < (slice + 31) / 32; i += NT) is_listed[i] = 0;
     if (tid == 0) s.repeated = 0;
+  }
+  load_teacher<NT>(a, q, x, s);
+  if (tail) {
     __syncthreads();
     for (int j = tid; j < k; j += NT) {
       const int i = s.id[j] - v0;
@@ -729,14 +756,13 @@ __global__ void __launch_bounds__(NT, 1536 / NT) distill_loss_kernel(DistillArgs
     __syncthreads();
   }
   const float ct = q.inv_t * kLog2e, c1 = kLog2e;
-  const Chunks ch(q, E);
   float mt = -CUDART_INF_F, nBt = 0.f, nB1 = 0.f, st = 0.f, s1 = 0.f;
   auto raise = [&](float cm) {  // the largest logit so far
     if (cm > mt) {
       const float nt = -__fmul_rn(cm, ct), n1 = -__fmul_rn(cm, c1);
       if (mt > -CUDART_INF_F) {
         st *= ex2(nt - nBt);
-        if (NEXP == 2) s1 *= ex2(n1 - nB1);
+        if (X != kOne) s1 *= ex2(n1 - nB1);
       }
       mt = cm;
       nBt = nt;
@@ -746,11 +772,7 @@ __global__ void __launch_bounds__(NT, 1536 / NT) distill_loss_kernel(DistillArgs
   auto add = [&](uint4 u, int c) {
     float f[E];
     Chunk<T>::unpack(u, f);
-    if (NEXP == 2) {
-#pragma unroll
-      for (int e = 0; e < E; ++e) s1 += ex2(fmaf(f[e], c1, nB1));
-    }
-    if (tail) {
+    if (tail) {  // a listed token's term is added once, below
       const uint32_t bits = (is_listed[c * E >> 5] >> (c * E & 31)) & ((1u << E) - 1);
       if (bits) {
 #pragma unroll
@@ -759,7 +781,12 @@ __global__ void __launch_bounds__(NT, 1536 / NT) distill_loss_kernel(DistillArgs
       }
     }
 #pragma unroll
-    for (int e = 0; e < E; ++e) st += ex2(fmaf(f[e], ct, nBt));
+    for (int e = 0; e < E; ++e) {
+      const float t = ex2(fmaf(f[e], ct, nBt));
+      st += t;
+      if (X == kTwo) s1 += ex2(fmaf(f[e], c1, nB1));
+      if (X > kTwo) s1 += power<X>(t);
+    }
   };
   const uint4* x4 = reinterpret_cast<const uint4*>(x + v0);  // chunk c, for c in [c0, c1)
   int c = ch.c0 + tid;
@@ -783,8 +810,10 @@ __global__ void __launch_bounds__(NT, 1536 / NT) distill_loss_kernel(DistillArgs
   if (edge >= 0) {
     const float f = to_f32(x[v0 + edge]);
     raise(f);
-    if (NEXP == 2) s1 += ex2(fmaf(f, c1, nB1));
-    if (!(tail && ((is_listed[edge >> 5] >> (edge & 31)) & 1))) st += ex2(fmaf(f, ct, nBt));
+    if (!(tail && ((is_listed[edge >> 5] >> (edge & 31)) & 1))) {
+      st += ex2(fmaf(f, ct, nBt));
+      if (X != kOne) s1 += ex2(fmaf(f, c1, nB1));
+    }
   }
   float mx = warp_max(mt);
   if ((tid & 31) == 0) s.warp[0][tid >> 5] = mx;
@@ -807,7 +836,9 @@ __global__ void __launch_bounds__(NT, 1536 / NT) distill_loss_kernel(DistillArgs
   if (tail)
     for (int j = tid; j < k; j += NT) {
       const int i = s.id[j] - v0;
-      if (s.id[j] >= 0 && i >= lo && i < hi && is_first(s, j)) listed += ex2(fmaf(s.val[j], ct, -Mt));
+      if (s.id[j] < 0 || i < lo || i >= hi || !is_first(s, j)) continue;
+      listed += ex2(fmaf(s.val[j], ct, -Mt));
+      if (X != kOne) s1 += ex2(fmaf(s.val[j], c1, -M1));
     }
   block_sum3<NT>(s, st, s1, listed);
   if (C > 1) {
@@ -826,7 +857,7 @@ __global__ void __launch_bounds__(NT, 1536 / NT) distill_loss_kernel(DistillArgs
   }
   const float rest = st;
   st += listed;
-  if (NEXP == 1) s1 = st;
+  if (X == kOne) s1 = st;
   if (q.rank == 0 && tid < 32) {
     const float loss = row_loss(a, q, s, ct, Mt, M1, st, s1, rest);
     if (tid == 0) a.loss[q.row] = loss;
@@ -859,23 +890,18 @@ __global__ void __launch_bounds__(256) scale_rows_kernel(T* __restrict__ x, int6
   }
 }
 
-template <typename T, int NT>
+template <typename T, Exps X, int NT>
 cudaError_t distill_n(const DistillArgs& a, int C, int slice, cudaStream_t st) {
   const unsigned grid = (unsigned)(a.N * C);
-  const bool two = a.targets && a.temperature != 1.f;
   LaunchScope scope_(a.dlogits ? "distill_grad" : "distill_loss", st);
-  if (a.dlogits) {
-    const size_t smem = (size_t)slice * sizeof(T);
-    return two ? launch_clusters(distill_grad_kernel<T, 2, NT>, grid, C, NT, smem, st, a, slice)
-               : launch_clusters(distill_grad_kernel<T, 1, NT>, grid, C, NT, smem, st, a, slice);
-  }
+  if (a.dlogits)
+    return launch_clusters(distill_grad_kernel<T, X, NT>, grid, C, NT, (size_t)slice * sizeof(T), st, a, slice);
   const size_t smem = a.t_lse ? (size_t)(slice / 32) * 4 : 0;
-  return two ? launch_clusters(distill_loss_kernel<T, 2, NT>, grid, C, NT, smem, st, a, slice)
-             : launch_clusters(distill_loss_kernel<T, 1, NT>, grid, C, NT, smem, st, a, slice);
+  return launch_clusters(distill_loss_kernel<T, X, NT>, grid, C, NT, smem, st, a, slice);
 }
 
-template <typename T>
-cudaError_t distill_t(const DistillArgs& a, cudaStream_t st) {
+template <typename T, Exps X>
+cudaError_t distill_x(const DistillArgs& a, cudaStream_t st) {
   constexpr int E = Chunk<T>::E;
   auto slice_of = [&](int n) { return (int)(ceil_div(ceil_div((int64_t)a.V + E - 1, n), 32) * 32); };
   // one block per row, more where rows are too few to fill the SMs, or a block's copy of the row is too large for two
@@ -886,12 +912,12 @@ cudaError_t distill_t(const DistillArgs& a, cudaStream_t st) {
   if (a.N * C > 0x7fffffff) return cudaErrorInvalidValue;
   const int slice = slice_of(C);
   // Rows of which three fit a block's shared memory but not many more, enough of them that every SM gets several: 16,384
-  // rows of 32,768 bfloat16 take 545 us on persistent blocks and 558 on a block per row (373 and 440 at T = 1); 32,768 rows
-  // of 16,384 take 698 and 563.
+  // rows of 32,768 bfloat16 take 395 us on persistent blocks and @@ on a block per row (T = 2; 373 and 440 at T = 1);
+  // 32,768 rows of 16,384 take 559 and 437.
   const size_t row_bytes = (size_t)slice * sizeof(T);
   if (a.dlogits && C == 1 && a.k <= kTeamTeacher && a.N >= 4 * kSMs && row_bytes > 40 * 1024 &&
       kBuffers * row_bytes <= 200 * 1024) {
-    auto kern = a.targets && a.temperature != 1.f ? distill_rows_kernel<T, 2> : distill_rows_kernel<T, 1>;
+    auto kern = distill_rows_kernel<T, X>;
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(kBuffers * row_bytes));
     if (e != cudaSuccess) return e;
     LaunchScope scope_("distill_rows", st);
@@ -899,9 +925,17 @@ cudaError_t distill_t(const DistillArgs& a, cudaStream_t st) {
   }
   // few threads where rows are short, so that many blocks hide one another's reductions (65,536 rows of 8,192: 256
   // threads 1,093 us, 128 658; 131,072 of 2,048: 1,598, 811 and with 64 752)
-  if (row_bytes <= 8448) return distill_n<T, 64>(a, C, slice, st);
-  if (row_bytes <= 33024) return distill_n<T, 128>(a, C, slice, st);
-  return distill_n<T, 256>(a, C, slice, st);
+  if (row_bytes <= 8448) return distill_n<T, X, 64>(a, C, slice, st);
+  if (row_bytes <= 33024) return distill_n<T, X, 128>(a, C, slice, st);
+  return distill_n<T, X, 256>(a, C, slice, st);
+}
+
+template <typename T>
+cudaError_t distill_t(const DistillArgs& a, cudaStream_t st) {
+  if (!a.targets || a.temperature == 1.f) return distill_x<T, kOne>(a, st);
+  if (a.temperature == 2.f) return distill_x<T, kSquare>(a, st);
+  if (a.temperature == 4.f) return distill_x<T, kFourth>(a, st);
+  return distill_x<T, kTwo>(a, st);
 }
 
 }  // namespace

@@ -374,6 +374,41 @@ def test_distill(cuda_ok, dt, N, V, k, T, a, hard, tail):
 
 
 @pytest.mark.parametrize("dt", [F32, BF16])
+@pytest.mark.parametrize("N,V,k,T,a,hard,tail", [(3, 17, 5, 4.0, 0.5, True, True), (200, 2053, 16, 4.0, 0.3, True, False),
+                                                 (150, 9001, 30, 4.0, 0.5, True, True), (2, 50021, 300, 4.0, 0.5, True, True),
+                                                 (600, 24007, 7, 2.0, 0.5, True, False), (600, 22001, 7, 4.0, 0.5, True, True),
+                                                 (300, 24007, 7, 2.0, 0.5, True, True)])
+def test_distill_powers(cuda_ok, dt, N, V, k, T, a, hard, tail):
+    """At T = 2 and 4 the exponential at 1 is a power of the one at T: its error, 4 u for the exponential, grows by the
+    same power (16 u, and 2 u for the squarings), which PERR's 16 u beyond the 80 u of the difference's roundings hold
+    with that of the sum."""
+    test_distill(cuda_ok, dt, N, V, k, T, a, hard, tail)
+
+
+def test_distill_powers_of_excluded_tokens(cuda_ok):
+    """Logits of -infinity and far below the largest, where the exponential at 1 is 0 and the one at T is not."""
+    for T in (2.0, 4.0):
+        for V in (40, 24000):
+            x = torch.zeros(600, V, device=DEV)
+            x[:, 3], x[:, 4], x[:, 5] = -math.inf, -200.0, torch.finfo(F32).min
+            ids = torch.full((600, 1), 0, device=DEV, dtype=torch.int32)
+            tl, tg = torch.zeros(600, 1, device=DEV), torch.full((600,), 1, device=DEV, dtype=torch.int32)
+            for dt in (F32, BF16):
+                loss, grad = S.distill_loss_and_grad(x.to(dt), ids, tl, tg, T, 0.5)
+                only = S.distill_loss(x.to(dt), ids, tl, tg, T, 0.5, reduction="none")
+                far = math.exp(-200.0 / T)
+                q, q1 = 1 / (V - 3 + far), 1 / (V - 3)
+                want = 0.5 * T * T * math.log(1 / q) + 0.5 * math.log(1 / q1)
+                mag = 0.5 * T * T * (math.log(1 / q) + 1) + 0.5 * (math.log(1 / q1) + 1)
+                assert (loss.double() - want).abs().max() <= PERR * mag and (only.double() - want).abs().max() <= PERR * mag
+                assert (grad[:, 3] == 0).all() and (grad[:, 5] == 0).all()
+                g4, g6 = 0.5 * T * q * far, 0.5 * T * q + 0.5 * q1
+                h = H if dt == BF16 else 0
+                assert ((grad[:, 4].double() - g4).abs() <= (4 * PERR + h) * g4 + 1e-37).all()  # |d| up to 100 there
+                assert ((grad[:, 6].double() - g6).abs() <= (PERR + h) * g6).all()
+
+
+@pytest.mark.parametrize("dt", [F32, BF16])
 def test_distill_many_rows(cuda_ok, dt):
     """Rows enough that every block has many, and half of them without weight, so that one half of a block runs ahead
     of the other: every row against torch in 64 bits."""
