@@ -40,7 +40,7 @@ __device__ __forceinline__ float ex2(float t) {
 // How many exponentials a logit takes.  kOne: the one at T serves, as T = 1 or no hard target is given.  kTwo: one at T and
 // one at 1.  kSquare, kFourth: T = 2 or 4, so that the one at 1 is the other's square or fourth power (c and B are then
 // exactly half or a quarter of those at 1, and it leaves float32's range at the same logit).  16,384 rows of 32,768
-// bfloat16 logits with their gradient: 373 us, 554, 395, 421.
+// bfloat16 logits with their gradient: 373 us, 529, 395, 421.
 enum Exps { kOne, kTwo, kSquare, kFourth };
 template <Exps X>
 __device__ __forceinline__ float power(float e) {
@@ -607,8 +607,6 @@ __global__ void __launch_bounds__(kRowsThreads, 1) distill_rows_kernel(DistillAr
     team_sync();
     const float nBt = -(mx * ct), nB1 = -(mx * c1);
     float st = 0.f, s1 = 0.f, listed = 0.f;
-    constexpr bool kMix = X == kTwo && sizeof(T) == 2;
-    pair_t s1p = pair(0.f, 0.f);
 #pragma unroll 4
     for (int c = ch.c0 + tid; c < ch.c1; c += kTeam) {
       float f[E];
@@ -617,16 +615,9 @@ __global__ void __launch_bounds__(kRowsThreads, 1) distill_rows_kernel(DistillAr
       for (int e = 0; e < E; ++e) {
         const float t = ex2(fmaf(f[e], ct, nBt));
         st += t;
-        if (X == kTwo && !kMix) s1 += ex2(fmaf(f[e], c1, nB1));
-        if (X > kTwo) s1 += power<X>(t);
-      }
-      if (kMix) {
-#pragma unroll
-        for (int e = 0; e < E; e += 2)
-          s1p = add_pair(s1p, exp2_pair(fma_pair(pair(f[e], f[e + 1]), pair(c1, c1), pair(nB1, nB1))));
+        if (X != kOne) s1 += power<X>(t);
       }
     }
-    if (kMix) s1 = both(s1p).x + both(s1p).y;
     if (edge >= 0) {
       const float f = to_f32(buf[edge]);
       st += ex2(fmaf(f, ct, nBt));
@@ -667,7 +658,6 @@ __global__ void __launch_bounds__(kRowsThreads, 1) distill_rows_kernel(DistillAr
     const float qm = X == kOne ? qr + q1 : qr;
     auto value = [&](float f) {
       const float t = ex2(fmaf(f, ct, nBt));
-      if (X == kTwo) return fmaf(q1, ex2(fmaf(f, c1, nB1)), qm * t);
       if (X == kSquare) return t * fmaf(q1, t, qm);
     if (X == kFourth) return fmaf(q1, power<X>(t), qm * t);
       return qm * t;
@@ -911,17 +901,19 @@ cudaError_t distill_x(const DistillArgs& a, cudaStream_t st) {
   while (C < kMaxCluster && (a.N * C < kSMs || slice_of(C) * (int64_t)sizeof(T) > most)) C *= 2;
   if (a.N * C > 0x7fffffff) return cudaErrorInvalidValue;
   const int slice = slice_of(C);
-  // Rows of which three fit a block's shared memory but not many more, enough of them that every SM gets several: 16,384
-  // rows of 32,768 bfloat16 take 395 us on persistent blocks and @@ on a block per row (T = 2; 373 and 440 at T = 1);
-  // 32,768 rows of 16,384 take 559 and 437.
+  // Rows of which three fit a block's shared memory, but of which the SM does not hold four for the other kernel, enough
+  // of them that every SM gets several.  16,384 rows of 32,768 bfloat16 take 395 us on persistent blocks and 414 on a block
+  // per row, of 26,000 348 and 375, but of 24,000 367 and 308; and with two exponentials of 32,768 552 and 529.
   const size_t row_bytes = (size_t)slice * sizeof(T);
-  if (a.dlogits && C == 1 && a.k <= kTeamTeacher && a.N >= 4 * kSMs && row_bytes > 40 * 1024 &&
-      kBuffers * row_bytes <= 200 * 1024) {
-    auto kern = distill_rows_kernel<T, X>;
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(kBuffers * row_bytes));
-    if (e != cudaSuccess) return e;
-    LaunchScope scope_("distill_rows", st);
-    return launch_k(kern, dim3(kSMs), dim3(kRowsThreads), kBuffers * row_bytes, st, a, slice);
+  if constexpr (X != kTwo) {
+    if (a.dlogits && C == 1 && a.k <= kTeamTeacher && a.N >= 4 * kSMs && row_bytes > 50 * 1024 &&
+        kBuffers * row_bytes <= 200 * 1024) {
+      auto kern = distill_rows_kernel<T, X>;
+      cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(kBuffers * row_bytes));
+      if (e != cudaSuccess) return e;
+      LaunchScope scope_("distill_rows", st);
+      return launch_k(kern, dim3(kSMs), dim3(kRowsThreads), kBuffers * row_bytes, st, a, slice);
+    }
   }
   // few threads where rows are short, so that many blocks hide one another's reductions (65,536 rows of 8,192: 256
   // threads 1,093 us, 128 658; 131,072 of 2,048: 1,598, 811 and with 64 752)
