@@ -224,6 +224,7 @@ constexpr int kMaxWarps = 32;      // a block has NT = 512 or 1,024 threads
 constexpr int kBins = 512;         // at most one per thread when they are scanned
 constexpr int kSplit = 256;        // parts of a key range
 constexpr int kList = 1024;        // candidates that one block ranks
+constexpr int kRank = 128;         // more candidates of one bin are thinned out before they are ranked
 constexpr int kListK = 256;        // a top_k up to this, all blocks of a row together, is found among candidates
 
 // float -> unsigned in the same order; -0 and +0 are one value (NaN has been made -infinity).
@@ -299,7 +300,8 @@ struct ChooseShared {
   uint32_t ties[kMaxCluster], listed[kMaxCluster];
   int first[kMaxCluster];
   union {
-    // this block's histogram: tokens, and masses in three limbs of 14 bits (a slice's tokens, under 2^16, cannot overflow one)
+    // this block's histogram: tokens, and masses in three limbs of 14 bits (a slice's tokens, under 2^16, cannot overflow one;
+    // 64-bit shared atomics: 43.8 us for 33 rows of 50,021 where these took 35.5)
     struct {
       uint32_t count[kBins], limb[3][kBins];
     };
@@ -412,29 +414,14 @@ __device__ __forceinline__ int gap_bin(float v, float m, float scale) {
   return v == m ? 0 : min(kBins - 1, (int)((m - v) * scale));
 }
 
-// Lists this block's tokens for which `take` holds, and tells the cluster how many they are.  Returns the cluster's
-// number (lists are cut at kList, and the number is then above it).
-template <int NT, typename Cluster, typename F>
-__device__ uint32_t list_tokens(Cluster& cluster, ChooseShared& s, const float* y, int lo, int hi, int v0, F take) {
+// This block's list of tokens: emptied, filled, and its length told to the cluster, whose number of tokens is returned
+// (lists are cut at kList, and the number is then above it).
+__device__ __forceinline__ void begin_list(ChooseShared& s) {
   if (threadIdx.x == 0) s.list_n = 0;
   __syncthreads();
-#pragma unroll 2
-  for (int i0 = threadIdx.x * 4; i0 < hi; i0 += NT * 4) {
-    const float4 q = *reinterpret_cast<const float4*>(y + i0);
-    const float v[4] = {q.x, q.y, q.z, q.w};
-    uint32_t in = 0;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) in |= (uint32_t)take(v[e]) << e;
-    if (!in) continue;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int i = i0 + e;
-      if (((in >> e) & 1) && i >= lo && i < hi) {
-        const uint32_t at = atomicAdd(&s.list_n, 1u);
-        if (at < kList) s.list[at] = (u64)order_key(v[e]) << 32 | (0xffffffffu - (uint32_t)(v0 + i));
-      }
-    }
-  }
+}
+template <typename Cluster>
+__device__ __forceinline__ uint32_t end_list(Cluster& cluster, ChooseShared& s) {
   __syncthreads();
   if (threadIdx.x < cluster.num_blocks()) *cluster.map_shared_rank(&s.listed[cluster.block_rank()], threadIdx.x) = s.list_n;
   cluster.sync();
@@ -442,11 +429,27 @@ __device__ uint32_t list_tokens(Cluster& cluster, ChooseShared& s, const float* 
   for (unsigned r = 0; r < cluster.num_blocks(); ++r) n += s.listed[r];
   return n;
 }
+// Of the four positions from i on, those in [lo, hi) for which `take` holds.
+template <typename F>
+__device__ __forceinline__ void list_four(ChooseShared& s, const float* y, int i, int lo, int hi, int v0, F take) {
+  const float4 q = *reinterpret_cast<const float4*>(y + i);
+  const float v[4] = {q.x, q.y, q.z, q.w};
+  uint32_t in = 0;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) in |= (uint32_t)take(v[e]) << e;
+  if (!in) return;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    if (((in >> e) & 1) && i + e >= lo && i + e < hi) {
+      const uint32_t at = atomicAdd(&s.list_n, 1u);
+      if (at < kList) s.list[at] = (u64)order_key(v[e]) << 32 | (0xffffffffu - (uint32_t)(v0 + i + e));
+    }
+  }
+}
 
-// Block 0: brings the cluster's lists (n tokens, n <= kList) together in s.sorted, largest first.  All keys differ,
-// so the order does not depend on how the lists were filled.
+// Block 0: brings the cluster's lists (n tokens, n <= kList) together in s.list.
 template <int NT, typename Cluster>
-__device__ void sort_lists(Cluster& cluster, ChooseShared& s, uint32_t n) {
+__device__ void join_lists(Cluster& cluster, ChooseShared& s) {
   uint32_t at = s.listed[0];
   for (unsigned r = 1; r < cluster.num_blocks(); ++r) {
     const uint32_t k = s.listed[r];
@@ -455,6 +458,11 @@ __device__ void sort_lists(Cluster& cluster, ChooseShared& s, uint32_t n) {
     at += k;
   }
   __syncthreads();
+}
+
+// Block 0: s.list in s.sorted, largest first.  All keys differ, so the order does not depend on how the list was filled.
+template <int NT>
+__device__ void sort_list(ChooseShared& s, uint32_t n) {
   // a token's rank is the number of larger ones, counted by four lanes
   for (uint32_t i0 = 0; i0 < n; i0 += NT / 4) {
     const uint32_t i = i0 + threadIdx.x / 4;
@@ -466,6 +474,46 @@ __device__ void sort_lists(Cluster& cluster, ChooseShared& s, uint32_t n) {
     rank += __shfl_xor_sync(0xffffffffu, rank, 2);
     if (i < n && (threadIdx.x & 3) == 0) s.sorted[rank] = mine;
   }
+  __syncthreads();
+}
+
+// Block 0, many tokens of one bin in s.list (n <= kList): keeps those of the one of kSplit equal parts of the bin in which
+// the cut lies, and adds what lies above it.  Ranking is quadratic (33 rows of 50,021: 34.9 us without this, 32.3
+// with).
+template <int NT>
+__device__ void keep_part(ChooseShared& s, const Masses& M, float scale, int B, bool by_count, bool masses, u64 target,
+                          uint32_t& n, uint32_t& above, u64& above_mass) {
+  constexpr int U = kList / NT;
+  u64 mine[U];
+  int part[U];
+  clear_bins<NT, kSplit>(s);
+  __syncthreads();
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const uint32_t i = u * NT + threadIdx.x;
+    part[u] = -1;
+    if (i < n) {
+      mine[u] = s.list[i];
+      const float v = key_value((uint32_t)(mine[u] >> 32));
+      const float gap = v == M.m ? 0.f : (M.m - v) * scale - (float)B;  // from 0 to 1, more in the last bin
+      part[u] = (int)fminf(gap * kSplit, (float)(kSplit - 1));
+      atomicAdd(&s.count[part[u]], 1u);
+      if (masses) add_mass(s, part[u], M(v));
+    }
+  }
+  if (threadIdx.x == 0) s.list_n = 0;
+  __syncthreads();
+  const int b = threadIdx.x;
+  u64 m = 0;
+  if (b < kSplit && masses) m = (u64)s.limb[0][b] + ((u64)s.limb[1][b] << 14) + ((u64)s.limb[2][b] << 28);
+  scan_bins<kSplit>(s, b < kSplit ? s.count[b] : 0u, m, s.split_mass, s.split_count);
+  const int P = find_bin<kSplit>(s, s.split_mass, s.split_count, by_count, target - (by_count ? above : above_mass));
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+    if (part[u] == P) s.list[atomicAdd(&s.list_n, 1u)] = mine[u];
+  n = s.split_count[P + 1] - s.split_count[P];
+  above += s.split_count[P];
+  above_mass += s.split_mass[P];
   __syncthreads();
 }
 
@@ -500,8 +548,11 @@ __device__ Cut search(Cluster& cluster, ChooseShared& s, const float* y, int lo,
   const int B = find_bin<kBins>(s, s.mass_before, s.count_before, by_count, target);
   u64 above_mass = s.mass_before[B];
   uint32_t above = s.count_before[B];
-  const uint32_t n = list_tokens<NT>(cluster, s, y, lo, hi, v0,
-                                 [&](float v) { return gap_bin(v, M.m, scale) == B && v > -CUDART_INF_F; });
+  begin_list(s);
+#pragma unroll 2
+  for (int i = threadIdx.x * 4; i < hi; i += NT * 4)
+    list_four(s, y, i, lo, hi, v0, [&](float v) { return gap_bin(v, M.m, scale) == B && v > -CUDART_INF_F; });
+  uint32_t n = end_list(cluster, s);
   // -infinity is not listed: where the count runs into it, all that is listed is kept
   const bool short_ = by_count && target - above > n;
   if (short_) {
@@ -510,7 +561,9 @@ __device__ Cut search(Cluster& cluster, ChooseShared& s, const float* y, int lo,
   }
   if (n <= kList) {
     if (cluster.block_rank() == 0) {
-      sort_lists<NT>(cluster, s, n);
+      join_lists<NT>(cluster, s);
+      if (n > kRank) keep_part<NT>(s, M, scale, B, by_count, masses, target, n, above, above_mass);
+      sort_list<NT>(s, n);
       u64 w0, w1, all;
       u64 before = above_mass + scan_sorted<NT>(s, M, masses ? n : 0, w0, w1, all);
 #pragma unroll
@@ -716,15 +769,23 @@ __global__ void __launch_bounds__(NT, 1024 / NT) choose_kernel(sdm_logit_rules r
     // below every logit of the bins 0 .. last (the last bin has all that are smaller still)
     const float least = scale > 0.f && last < kBins - 1 ? m - ((float)last + 1.01f) / scale : -CUDART_INF_F;
     cluster.barrier_wait(std::move(started));
-    const uint32_t n = list_tokens<NT>(cluster, s, y, lo, hi, v0,
-                                   [&](float v) { return v >= least && v > -CUDART_INF_F; });
+    begin_list(s);
+    if (top >= least && top > -CUDART_INF_F) {  // few threads hold one
+      for (int i0 = tid * E; i0 < hi; i0 += NT * E) {
+#pragma unroll
+        for (int e = 0; e < E; e += 4)
+          list_four(s, y, i0 + e, lo, hi, v0, [&](float v) { return v >= least && v > -CUDART_INF_F; });
+      }
+    }
+    const uint32_t n = end_list(cluster, s);
     if (n <= kList) {
       if (rank == 0 && n == 0 && tid == 0) {  // nothing is allowed
         ids[row] = -1;
         if (logprob) logprob[row] = -CUDART_INF_F;
       }
       if (rank == 0 && n > 0) {
-        sort_lists<NT>(cluster, s, n);
+        join_lists<NT>(cluster, s);
+        sort_list<NT>(s, n);
         const float most = key_value((uint32_t)(s.sorted[0] >> 32));
         const Masses M(most, Tr);
         const uint32_t kept = min(n, (uint32_t)top_k);
@@ -949,7 +1010,8 @@ cudaError_t choose_t(const sdm_logit_rules& r, const sdm_choice_params& c, const
   int C = 1;
   auto slice_of = [&](int n) { return (int)(ceil_div(ceil_div((int64_t)V + E - 1, n), 1024) * 1024); };
   // More blocks per row while all of them can be on the GPU together (two per SM, and a cluster within a GPC), or while
-  // a slice does not fit a block's shared memory.  256 rows of 32,768: 38 us in whole rows, 40 in halves, 68 in quarters.
+  // a slice does not fit a block's shared memory.  A block's time is mostly that of its phases, whatever
+  // its slice: 256 rows of 32,768 take 34 us as whole rows, 57 in halves, 64 in quarters.
   while (C < kMaxCluster && (S * C * 2 <= 256 || slice_of(C) * 4 > 144 * 1024)) C *= 2;
   if (S * C > 0x7fffffff) return cudaErrorInvalidValue;
   const int slice = slice_of(C);

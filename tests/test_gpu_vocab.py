@@ -183,6 +183,36 @@ def test_sample_logits(cuda_ok, dt, rows, V, k, share, T):
     assert np.allclose(np64(got), want_lp, rtol=16 * U, atol=16 * U)
 
 
+@pytest.mark.parametrize("crowd,far", [(100, 0), (700, 0), (1024, 0), (1025, 0), (100, 800), (30, 1100)])
+@pytest.mark.parametrize("k,share", [(300, 1.0), (0, 0.6), (500, 0.45), (0, 0.95)])
+@pytest.mark.parametrize("rows", [2, 200])
+def test_sample_crowded_cut(cuda_ok, crowd, far, k, share, rows):
+    """The cut among many tokens whose logits are close or tied, and among tokens whose masses are 0."""
+    V, g = 3000, gen(crowd + far)
+    x = torch.full((rows, V), -math.inf, device=DEV)
+    for i in range(rows):
+        at = torch.randperm(V, generator=g, device=DEV)
+        steps = torch.randint(0, 64, (crowd,), generator=g, device=DEV)
+        x[i, at[:crowd]] = -5.02 - steps / 1024.0  # ties among them
+        x[i, at[crowd:crowd + far]] = -40.0 - torch.rand(far, generator=g, device=DEV)
+        x[i, at[crowd + far]] = 0.0
+    rng = np.random.default_rng(crowd)
+    xs = np64(x)
+    p = [1.0 if share >= 1 else clear_p(xs[i], 1.0, k, share) for i in range(rows)]
+    u, want, lp = [], [], []
+    for i in range(rows):
+        keep, w = kept64(xs[i], 1.0, k, p[i])
+        c = np.cumsum(w)
+        j = int(rng.choice(np.flatnonzero(w > 1e-4 * c[-1])))
+        u.append((c[j] - 0.5 * w[j]) / c[-1])
+        want.append(int(keep[j]))
+        lp.append(math.log(w[j] / c[-1]))
+    d = lambda v: torch.tensor(v, device=DEV, dtype=F32)  # noqa: E731
+    ids, got = S.sample_logits(x, u=d(u), top_k=k, top_p=d(p) if share < 1 else 1.0)
+    assert ids.tolist() == want
+    assert (np.abs(np64(got) - lp) <= 16 * U * (1 + np.abs(lp))).all()
+
+
 def test_sample_ties_and_ends(cuda_ok):
     V = 3000
     x = torch.zeros(4, V, device=DEV)
