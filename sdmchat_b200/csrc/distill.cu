@@ -17,7 +17,7 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kMaxWarps = 8;  // a block has NT = 64, 128 or 256 threads
+constexpr int kMaxWarps = 8;  // a block has NT = 32, 64, 128 or 256 threads
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 struct DistillShared {
@@ -332,8 +332,8 @@ __global__ void __launch_bounds__(NT, 768 / NT) distill_grad_kernel(DistillArgs 
   const float ct = q.inv_t * kLog2e, c1 = kLog2e, nBt = -(mx * ct), nB1 = -(mx * c1);
   float st = 0.f, s1 = 0.f, listed = 0.f;
   // Four exponentials per bfloat16 logit would take the exponential unit longer than memory takes for the logit and
-  // its gradient: half of those at T = 1 go to the FMA pipe here, and a quarter below (16,384 rows of 32,768: 558 us; all
-  // of these here and none below 590).
+  // its gradient: half of those at T = 1 go to the FMA pipe here, and a quarter below (16,384 rows of 32,768: 558 us when this
+  // was measured; all of these here and none below 590).
   constexpr bool kMix = X == kTwo && sizeof(T) == 2;
   pair_t s1p = pair(0.f, 0.f);
 #pragma unroll 2
@@ -915,9 +915,12 @@ cudaError_t distill_x(const DistillArgs& a, cudaStream_t st) {
       return launch_k(kern, dim3(kSMs), dim3(kRowsThreads), kBuffers * row_bytes, st, a, slice);
     }
   }
-  // few threads where rows are short, so that many blocks hide one another's reductions (65,536 rows of 8,192: 256
-  // threads 1,093 us, 128 658; 131,072 of 2,048: 1,598, 811 and with 64 752)
-  if (row_bytes <= 8448) return distill_n<T, X, 64>(a, C, slice, st);
+  // few threads where rows are short, so that many blocks hide one another's reductions.  131,072 rows of 2,048 bfloat16
+  // logits with their gradient take 420 us with 32 threads and 446 with 64 (of 1,000 334 and 424), 65,536 of 4,096 331 and
+  // 297; the loss alone of 65,536 rows of 8,192 209 with 64 and 261 with 128, of 32,768 rows of 16,384 222 and 191, of
+  // 16,384 rows of 32,768 204 with 128 and 185 with 256.
+  if (row_bytes <= 6 * 1024) return distill_n<T, X, 32>(a, C, slice, st);
+  if (row_bytes <= 16896) return distill_n<T, X, 64>(a, C, slice, st);
   if (row_bytes <= 33024) return distill_n<T, X, 128>(a, C, slice, st);
   return distill_n<T, X, 256>(a, C, slice, st);
 }
