@@ -17,7 +17,8 @@ namespace {
 constexpr int kPiece = 16;       // positions summed by one warp (with its two neighbours at most 32)
 constexpr int kFewMax = 1024;    // positions that one launch compares with one another: 16 to 24 us over a table of
                                  // 32,768 x 768, against 31 by sorting; at 2,048 it takes 40, and sorting 32
-constexpr int kLong = 16;        // a group that goes on over so many more pieces is joined by blocks
+constexpr int kLong = 6;         // a group that goes on over so many more pieces is joined by blocks (65,536 x 768 by a
+                                 // Zipf law 63 us, with 16 66; 5,000 x 330 24.7 and 26.9)
 constexpr int kSortThreads = 1024, kSortWarps = kSortThreads / 32;
 constexpr int kSortCluster = 16; // blocks of the sorting cluster (more than the portable 8)
 constexpr int kSortEach = 4096;  // positions of one of them
@@ -412,7 +413,7 @@ __device__ __forceinline__ void store_grad(G* at, const float* v, float scale, i
 // stead, the same sums took longer.
 template <typename T, typename G, int VEC, int NQ>
 __global__ void __launch_bounds__(kSumThreads, 2) sum_kernel(const T* __restrict__ dout,
-                                                              int64_t ld, int d,
+                                                              int64_t ld, int N, int d,
                                                               int col_blocks, int64_t items, float scale,
                                                               int accumulate, GroupWs w, G* __restrict__ grad) {
   pdl_enter();
@@ -424,16 +425,20 @@ __global__ void __launch_bounds__(kSumThreads, 2) sum_kernel(const T* __restrict
   const int lane = threadIdx.x & 31;
   const int piece = (int)(col_blocks == 1 ? item : item / col_blocks);
   const int c = (int)(item - (int64_t)piece * col_blocks) * (32 * VEC * NQ) + VEC * lane;
-  const int total = *w.total, j0 = piece * kPiece, n = min(kPiece, total - j0);
+  const int j0 = piece * kPiece;
+  // lane l: the position before the piece (l = 0), the piece's (1 .. n), and the one after it (n + 1); fetched before
+  // `total` is known, and used below it
+  const int j = j0 - 1 + lane;
+  const bool inside = lane <= kPiece + 1 && j >= 0 && j < N;
+  int pos = inside ? w.order[j] : -1, id = inside ? w.token[j] : -1;
+  int later = j0 + kLong * kPiece < N ? w.token[j0 + kLong * kPiece] : -1;
+  const int total = *w.total, n = min(kPiece, total - j0);
   if (n <= 0) {
     if (c == 0) w.crossing[piece] = -1;
     return;
   }
-  // lane l: the position before the piece (l = 0), the piece's (1 .. n), and the one after it (n + 1)
-  const int j = j0 - 1 + lane;
-  const bool there = lane <= n + 1 && j >= 0 && j < total;
-  const int pos = there ? w.order[j] : -1, id = there ? w.token[j] : -1;
-  const int later = j0 + kLong * kPiece < total ? w.token[j0 + kLong * kPiece] : -1;
+  if (lane > n + 1 || j >= total) pos = id = -1;
+  if (j0 + kLong * kPiece >= total) later = -1;
   const int before = __shfl_sync(0xffffffffu, id, 0), after = __shfl_sync(0xffffffffu, id, n + 1);
   const uint32_t ends = __ballot_sync(0xffffffffu, id != __shfl_down_sync(0xffffffffu, id, 1) || lane == n) >> 1;
   float acc[NQ][VEC];
@@ -594,11 +599,13 @@ __global__ void __launch_bounds__(32 * kJoinWarps, 2) join_kernel(int d, int pie
     const int m = ((int)blockIdx.x - hot_blocks * cols) * kJoinWarps + warp;
     if (m >= pieces) return;
     const int v = w.crossing[m];
+    // the tokens at the starts of this piece and the later ones (beyond `total` there is anything, and it is not used)
+    const int k = min(m + lane, pieces - 1), t = w.token[k * kPiece];
     if (v < 0) return;
-    const int at = (m + 1 + lane) * kPiece;  // the first position of a later piece
-    const uint32_t in = __ballot_sync(0xffffffffu, lane < kLong && at < total && w.token[min(at, total - 1)] == v);
-    const int more = __ffs(~in) - 1;
-    const float* first = w.partial + (2 * (int64_t)m + (w.token[m * kPiece] != v ? 1 : 0)) * w.ldp;
+    const int t0 = __shfl_sync(0xffffffffu, t, 0);
+    const uint32_t in = __ballot_sync(0xffffffffu, lane > 0 && lane <= kLong && k == m + lane && k * kPiece < total && t == v);
+    const int more = __ffs(~(in >> 1)) - 1;
+    const float* first = w.partial + (2 * (int64_t)m + (t0 != v ? 1 : 0)) * w.ldp;
     const float* rest = w.partial + 2 * (int64_t)(m + 1) * w.ldp;
     constexpr int NC = 6;  // 768 columns in flight
     for (int c0 = lane * 4; c0 < d; c0 += 128 * NC) {
@@ -717,8 +724,8 @@ cudaError_t launch_sum_q(const T* dout, int64_t ld, int64_t N, int d, float scal
   const int64_t items = ceil_div(N, kPiece) * col_blocks, blocks = ceil_div(items, kSumWarps);
   if (blocks > 0x7fffffff) return cudaErrorInvalidValue;
   LaunchScope scope_("embed_grad_sum", st);
-  return launch_next(sum_kernel<T, G, VEC, NQ>, (unsigned)blocks, kSumThreads, st, dout, ld, d, col_blocks, items, scale,
-                     accumulate, w, grad);
+  return launch_next(sum_kernel<T, G, VEC, NQ>, (unsigned)blocks, kSumThreads, st, dout, ld, (int)N, d, col_blocks, items,
+                     scale, accumulate, w, grad);
 }
 template <typename T, typename G, int VEC>
 cudaError_t launch_sum(const T* dout, int64_t ld, int64_t N, int d, float scale, int accumulate,
@@ -795,7 +802,7 @@ cudaError_t grad_t(const int32_t* ids, const T* dout, int64_t ld, int64_t N, int
   }
   if (e != cudaSuccess) return e;
   const int pieces = (int)ceil_div(N, kPiece), cols = (int)ceil_div(d, 128);
-  const int hot_blocks = std::min(pieces / kLong + 1, 64);
+  const int hot_blocks = std::min(pieces / kLong + 1, kSMs);
   const int64_t blocks = (int64_t)hot_blocks * cols + ceil_div(pieces, kJoinWarps);
   if (blocks > 0x7fffffff) return cudaErrorInvalidValue;
   LaunchScope scope_("embed_grad_join", st);
