@@ -247,6 +247,22 @@ struct Chunks {
   }
 };
 
+// Whether a row's largest logit, times c, leaves float32's range (a row that is all at the type's lowest value): its
+// logits are then taken relative to the largest first, where any two that differ do so by far more than exp spans.
+__device__ __forceinline__ bool is_far(float mx, float ct, float c1) {
+  return fabsf(mx) < CUDART_INF_F && !(fabsf(mx) * fmaxf(ct, c1) < CUDART_INF_F);
+}
+template <typename T, int NT>
+__device__ __forceinline__ void lower_row(T* buf, int c0, int c1, int edge, int tid, float mx) {
+  constexpr int E = Chunk<T>::E;
+#pragma unroll 1
+  for (int c = c0 + tid; c < c1; c += NT) {
+#pragma unroll 1
+    for (int i = c * E; i < c * E + E; ++i) buf[i] = from_f32<T>(to_f32(buf[i]) - mx);
+  }
+  if (edge >= 0) buf[edge] = from_f32<T>(to_f32(buf[edge]) - mx);
+}
+
 // Loss and gradient.
 template <typename T, Exps X, int NT>
 __global__ void __launch_bounds__(NT, 768 / NT) distill_grad_kernel(DistillArgs a, int slice) {
@@ -329,7 +345,14 @@ __global__ void __launch_bounds__(NT, 768 / NT) distill_grad_kernel(DistillArgs 
   }
 
   // sums of exp over the row, at T and at 1
-  const float ct = q.inv_t * kLog2e, c1 = kLog2e, nBt = -(mx * ct), nB1 = -(mx * c1);
+  const float ct = q.inv_t * kLog2e, c1 = kLog2e;
+  if (is_far(mx, ct, c1)) {
+    lower_row<T, NT>(buf, ch.c0, ch.c1, edge, tid, mx);
+    for (int j = tid; j < k; j += NT) s.val[j] -= mx;
+    if (tid == 0) s.target_val -= mx;
+    mx = 0.f;
+  }
+  const float nBt = -(mx * ct), nB1 = -(mx * c1);
   float st = 0.f, s1 = 0.f, listed = 0.f;
   // Four exponentials per bfloat16 logit would take the exponential unit longer than memory takes for the logit and
   // its gradient: half of those at T = 1 go to the FMA pipe here, and a quarter below (16,384 rows of 32,768: 558 us when this
@@ -605,6 +628,12 @@ __global__ void __launch_bounds__(kRowsThreads, 1) distill_rows_kernel(DistillAr
       buf[mine] = from_f32<T>(-CUDART_INF_F);
     }
     team_sync();
+    if (is_far(mx, ct, c1)) {
+      lower_row<T, kTeam>(buf, ch.c0, ch.c1, edge, tid, mx);
+      if (tid < k) s.val[tid] -= mx;
+      if (tid == 0) s.target_val -= mx;
+      mx = 0.f;
+    }
     const float nBt = -(mx * ct), nB1 = -(mx * c1);
     float st = 0.f, s1 = 0.f, listed = 0.f;
 #pragma unroll 4
@@ -817,9 +846,22 @@ __global__ void __launch_bounds__(NT, 1536 / NT) distill_loss_kernel(DistillArgs
     for (int r = 0; r < C; ++r) mx = fmaxf(mx, s.part[0][r]);
   }
   // all sums relative to the row's largest logit
+  const bool far = is_far(mx, ct, c1);
+  if (far) {  // sums of their own
+    st = s1 = 0.f;
+    for (int i = lo + tid; i < hi; i += NT) {
+      const float f = to_f32(x[v0 + i]) - mx;
+      if (tail && ((is_listed[i >> 5] >> (i & 31)) & 1)) continue;
+      st += ex2(f * ct);
+      if (X != kOne) s1 += ex2(f * c1);
+    }
+    for (int j = tid; j < k; j += NT) s.val[j] -= mx;
+    if (tid == NT - 1) s.target_val -= mx;
+    mx = 0.f;
+  }
   const float Mt = __fmul_rn(mx, ct), M1 = __fmul_rn(mx, c1);
   float listed = 0.f;
-  if (mt > -CUDART_INF_F) {  // else they are 0, or NaN
+  if (mt > -CUDART_INF_F && !far) {  // else they are 0, or NaN
     st *= ex2(-nBt - Mt);
     s1 *= ex2(-nB1 - M1);
   }
@@ -918,8 +960,9 @@ cudaError_t distill_x(const DistillArgs& a, cudaStream_t st) {
   // few threads where rows are short, so that many blocks hide one another's reductions.  131,072 rows of 2,048 bfloat16
   // logits with their gradient take 420 us with 32 threads and 446 with 64 (of 1,000 334 and 424), 65,536 of 4,096 331 and
   // 297; the loss alone of 65,536 rows of 8,192 209 with 64 and 261 with 128, of 32,768 rows of 16,384 222 and 191, of
-  // 16,384 rows of 32,768 204 with 128 and 185 with 256.
-  if (row_bytes <= 6 * 1024) return distill_n<T, X, 32>(a, C, slice, st);
+  // 16,384 rows of 32,768 204 with 128 and 185 with 256.  A cluster's blocks keep 64: 48 rows of 1,000 float32 logits take
+  // 6.9 us, and 7.6 with 32.
+  if (C == 1 && row_bytes <= 6 * 1024) return distill_n<T, X, 32>(a, C, slice, st);
   if (row_bytes <= 16896) return distill_n<T, X, 64>(a, C, slice, st);
   if (row_bytes <= 33024) return distill_n<T, X, 128>(a, C, slice, st);
   return distill_n<T, X, 256>(a, C, slice, st);

@@ -416,6 +416,42 @@ def test_distill_powers(cuda_ok, dt, N, V, k, T, a, hard, tail):
     test_distill(cuda_ok, dt, N, V, k, T, a, hard, tail)
 
 
+@pytest.mark.parametrize("dt", [F32, BF16])
+@pytest.mark.parametrize("N,V", [(3, 40), (600, 24003), (600, 28001), (2, 50021)])
+@pytest.mark.parametrize("T", [1.0, 2.0, 0.5, 3.0])
+def test_distill_rows_at_the_ends_of_the_range(cuda_ok, dt, N, V, T):
+    """A row all at the type's lowest value is level; a row with one token at its highest has all mass there."""
+    if dt == F32 and V > 20000:
+        V //= 2
+    x = torch.full((N, V), torch.finfo(dt).min, device=DEV, dtype=dt)
+    x[1] = 0.0
+    x[1, 7] = torch.finfo(dt).max
+    ids = torch.tensor([[3, 7]] * N, device=DEV, dtype=torch.int32)
+    tl, tg = torch.zeros(N, 2, device=DEV), torch.full((N,), 7, device=DEV, dtype=torch.int32)
+    ids[1], tl[1] = torch.tensor([7, -1], device=DEV), 0.0
+    lse = torch.full((N,), math.log(4.0), device=DEV)  # half the teacher's mass on the two
+    for tail in (None, lse):
+        loss, grad = S.distill_loss_and_grad(x, ids, tl, tg, T, 0.5, None, tail)
+        only = S.distill_loss(x, ids, tl, tg, T, 0.5, None, tail, reduction="none")
+        for i in {0, N - 1} - {1}:
+            soft = math.log(V) - math.log(2) if tail is None else \
+                0.5 * (math.log(V) - math.log(4)) + 0.5 * (math.log(0.5) - math.log((V - 2) / V))
+            want = 0.5 * T * T * soft + 0.5 * math.log(V)
+            mag = 0.5 * T * T * (2 * math.log(V) + 4) + 0.5 * (math.log(V) + 1)
+            assert abs(float(loss[i]) - want) <= PERR * mag and abs(float(only[i]) - want) <= PERR * mag
+            p, rest = (0.5, 1 / V) if tail is None else (0.25, 1 / V - 0.5 / (V - 2))
+            g = grad[i].double().cpu().numpy()
+            h = H if dt == BF16 else 0
+            want7, want3 = 0.5 * T * (1 / V - p) + 0.5 * (1 / V - 1), 0.5 * T * (1 / V - p) + 0.5 / V
+            want0 = 0.5 * T * rest + 0.5 / V
+            m0 = 0.5 * T * (1 / V + 0.5 / V) + 0.5 / V
+            assert abs(g[7] - want7) <= PERR * (T + 1) + h * abs(want7) and abs(g[3] - want3) <= PERR * T + h * abs(want3)
+            others = np.delete(g, [3, 7])
+            assert (np.abs(others - want0) <= PERR * 2 * m0 + h * abs(want0)).all()
+        if tail is None:
+            assert abs(float(loss[1])) <= PERR and abs(float(only[1])) <= PERR and grad[1].abs().max() <= PERR
+
+
 def test_distill_powers_of_excluded_tokens(cuda_ok):
     """Logits of -infinity and far below the largest, where the exponential at 1 is 0 and the one at T is not."""
     for T in (2.0, 4.0):
