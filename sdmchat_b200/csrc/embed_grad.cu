@@ -2,9 +2,8 @@
 //
 // Gradient.  Up to kFewMax positions are done in one launch (few_kernel): blocks clear the rows that no id names, and the
 // first position of each token adds up its others.  For more, the positions are sorted by token while the gradient is
-// cleared: up to kSortMax positions by one cluster's
-// radix sort in shared memory (sort_kernel; the other blocks clear), more by a counting sort over all SMs
-// (group_kernel).  sum_kernel cuts the sorted order into pieces of kPiece positions, a warp each: a group inside a
+// cleared: up to kSortMax positions by one cluster's radix sort in shared memory (sort_kernel; the other blocks clear),
+// more by a counting sort over all SMs (group_kernel).  sum_kernel cuts the sorted order into pieces of kPiece positions, a warp each: a group inside a
 // piece is added up and written, a group that crosses a cut leaves a partial sum on each side.  join_kernel adds the
 // partial sums in order.  No float atomics, and every addition has its place: the result is a function of the inputs
 // alone.
@@ -16,7 +15,7 @@ namespace {
 
 constexpr int kPiece = 16;       // positions summed by one warp (with its two neighbours at most 32)
 constexpr int kFewMax = 1024;    // positions that one launch compares with one another: 16 to 24 us over a table of
-                                 // 32,768 x 768, against 31 by sorting; at 2,048 it takes 40, and sorting 32
+                                 // 32,768 x 768, against 30 by sorting; at 2,048 it takes 40, and sorting 31
 constexpr int kLong = 6;         // a group that goes on over so many more pieces is joined by blocks (65,536 x 768 by a
                                  // Zipf law 63 us, with 16 66; 5,000 x 330 24.7 and 26.9)
 constexpr int kSortThreads = 1024, kSortWarps = kSortThreads / 32;
