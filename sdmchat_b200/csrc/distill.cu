@@ -30,7 +30,9 @@ struct DistillShared {
 };
 
 // Exponentials are 2^(v c - B), c = log2(e) / T and B = c max rounded to float32: the one rounding of B cancels in
-// every quotient and logarithm, which take the same B.
+// every quotient and logarithm, which take the same B.  It has to be small beside float32's exponents, though: below
+// |c max| = kFar it is at most 2^-5.
+constexpr float kFar = 1048576.f;
 __device__ __forceinline__ float ex2(float t) {
   float e;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
@@ -247,10 +249,13 @@ struct Chunks {
   }
 };
 
-// Whether a row's largest logit, times c, leaves float32's range (a row that is all at the type's lowest value): its
-// logits are then taken relative to the largest first, where any two that differ do so by far more than exp spans.
+// Whether a row's largest logit, times the larger c that is used, is at or beyond kFar (a row that is all at a mask's lowest
+// value).  Its logits are then taken relative to the largest first: such differences are exact where a logit is within a factor of
+// two of the largest, and any other is 2^19 / c or more below.  (At that c: the rounding of such a difference to
+// bfloat16, 2^-9 of it, counts only where T is above 5,000 and a hard target asks for T = 1 besides.)
+template <Exps X>
 __device__ __forceinline__ bool is_far(float mx, float ct, float c1) {
-  return fabsf(mx) < CUDART_INF_F && !(fabsf(mx) * fmaxf(ct, c1) < CUDART_INF_F);
+  return fabsf(mx) < CUDART_INF_F && !(fabsf(mx) * (X == kOne ? ct : fmaxf(ct, c1)) < kFar);
 }
 template <typename T, int NT>
 __device__ __forceinline__ void lower_row(T* buf, int c0, int c1, int edge, int tid, float mx) {
@@ -346,7 +351,7 @@ __global__ void __launch_bounds__(NT, 768 / NT) distill_grad_kernel(DistillArgs 
 
   // sums of exp over the row, at T and at 1
   const float ct = q.inv_t * kLog2e, c1 = kLog2e;
-  if (is_far(mx, ct, c1)) {
+  if (is_far<X>(mx, ct, c1)) {
     lower_row<T, NT>(buf, ch.c0, ch.c1, edge, tid, mx);
     for (int j = tid; j < k; j += NT) s.val[j] -= mx;
     if (tid == 0) s.target_val -= mx;
@@ -628,7 +633,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) distill_rows_kernel(DistillAr
       buf[mine] = from_f32<T>(-CUDART_INF_F);
     }
     team_sync();
-    if (is_far(mx, ct, c1)) {
+    if (is_far<X>(mx, ct, c1)) {
       lower_row<T, kTeam>(buf, ch.c0, ch.c1, edge, tid, mx);
       if (tid < k) s.val[tid] -= mx;
       if (tid == 0) s.target_val -= mx;
@@ -846,7 +851,7 @@ __global__ void __launch_bounds__(NT, 1536 / NT) distill_loss_kernel(DistillArgs
     for (int r = 0; r < C; ++r) mx = fmaxf(mx, s.part[0][r]);
   }
   // all sums relative to the row's largest logit
-  const bool far = is_far(mx, ct, c1);
+  const bool far = is_far<X>(mx, ct, c1);
   if (far) {  // sums of their own
     st = s1 = 0.f;
     for (int i = lo + tid; i < hi; i += NT) {

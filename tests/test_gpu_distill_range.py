@@ -1,0 +1,114 @@
+"""Distillation where logits leave the range that one base can serve: rows partly masked with finite lowest values,
+rows that lie far from zero as a whole, and students whose listed tokens lead all others by more than an exponential
+spans.  The loss alone, the loss with its gradient and 64 bits have to agree, in every kernel (blocks and clusters of
+blocks per row, persistent blocks, the loss alone).
+
+Tolerances are those of the operator's other tests: a probability is off by 100 u of its own value (|d| * 2 u for the
+roundings of an exponent d of magnitude up to 40, 4 u for the exponential, the rest for sums and quotients), a
+logarithm by 100 u of its magnitude, one rounding to bfloat16 by 2^-8 of the value."""
+import math
+
+import pytest
+import torch
+
+import sdmchat_b200 as S
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+U, H = 2.0 ** -24, 2.0 ** -8
+PERR = 100 * U
+F32, BF16 = torch.float32, torch.bfloat16
+
+
+def gen(seed):
+    return torch.Generator(device=DEV).manual_seed(seed)
+
+
+def reference(x, ids, tl, tg, T, a, lse):
+    """(loss, gradient, their magnitudes for the rounding bounds) of all rows in 64 bits; distinct entries per row."""
+    x, tl = x.double(), tl.double()
+    N, V = x.shape
+    ok, at = ids >= 0, ids.clamp(min=0).long()
+    some = ok.any(1)
+    zt = (tl / T).masked_fill(~ok, -math.inf)
+    norm = torch.logsumexp(zt, 1) if lse is None else lse.double()
+    lp = torch.where(ok, zt - torch.where(some, norm, 0.0)[:, None], 0.0)
+    p = torch.where(ok, lp.exp(), 0.0)
+    P = p.sum(1)
+    lq = torch.log_softmax(x / T, 1)
+    lqa = lq.gather(1, at)
+    part = torch.where(ok, p * (lp - lqa), 0.0).sum(1)
+    lm = torch.where(ok, p * (lp.abs() + lqa.abs() + 1), 0.0).sum(1)
+    pr = torch.zeros_like(P)
+    q = lq.exp() * some[:, None]
+    listed = torch.zeros(N, V + 1, dtype=torch.bool, device=x.device)
+    listed.scatter_(1, torch.where(ok, at, V), True)
+    listed = listed[:, :V]
+    G = torch.zeros_like(x)
+    M = torch.zeros_like(x)
+    if lse is not None:
+        pr = torch.where(some, (1 - P).clamp(min=0), 0.0)
+        lr = torch.logsumexp(lq.masked_fill(listed, -math.inf), 1)  # log of the student's mass that is not listed
+        part = part + torch.where(pr > 0, pr * (pr.clamp(min=1e-300).log() - lr), 0.0)
+        lm = lm + torch.where(pr > 0, (P + 1) * (pr.clamp(min=1e-300).log().abs() + lr.abs() + 1), 0.0)
+        share = torch.softmax((x / T).masked_fill(listed, -math.inf), 1) * (pr > 0)[:, None]
+        G, M = G - pr[:, None] * share, M + (pr + 1)[:, None] * share
+    mass = (P + pr)[:, None]
+    G, M = G + mass * q, M + mass * q
+    G, M = G.scatter_add(1, at, -p), M.scatter_add(1, at, p)
+    loss, lm, G, M = a * T * T * part, a * T * T * lm, a * T * G, a * T * M
+    if tg is not None:
+        hit, t = tg >= 0, tg.clamp(min=0).long()[:, None]
+        l1 = torch.log_softmax(x, 1)
+        lt = torch.where(hit, l1.gather(1, t)[:, 0], 0.0)
+        one = (1 - a) * hit[:, None].double()
+        loss, lm = loss - (1 - a) * lt, lm + (1 - a) * hit * (lt.abs() + 1)
+        G, M = G + one * l1.exp(), M + one * l1.exp()
+        G, M = G.scatter_add(1, t, -one), M.scatter_add(1, t, one)
+    return loss, G, lm, M
+
+
+def check(x, ids, tl, tg, T, a, lse, with_loss=True):
+    loss, grad = S.distill_loss_and_grad(x, ids, tl, tg, T, a, None, lse)
+    only = S.distill_loss(x, ids, tl, tg, T, a, None, lse, reduction="none")
+    want, G, lm, M = reference(x, ids, tl, tg, T, a, lse)
+    bad = ~((only - want).abs() <= PERR * lm + 1e-30) & with_loss
+    assert not bad.any(), ("loss alone", bad.nonzero()[:5].tolist(), only[bad][:5], want[bad][:5])
+    bad = ~((loss - want).abs() <= PERR * lm + 1e-30) & with_loss
+    assert not bad.any(), ("loss", bad.nonzero()[:5].tolist(), loss[bad][:5], want[bad][:5])
+    tol = PERR * M + (H * G.abs() if x.dtype == BF16 else 0) + 1e-37
+    bad = ~((grad.double() - G).abs() <= tol)
+    assert not bad.any(), ("gradient", bad.nonzero()[:5].tolist(), grad[bad][:5], G[bad][:5])
+
+
+# rows and vocabularies: a cluster of eight blocks per row, of two to four, a block per row, persistent blocks
+SHAPES = [(12, 1000), (12, 50021), (48, 2053), (240, 2053), (624, 517), (624, 14003), (624, 28001)]
+
+
+@pytest.mark.parametrize("dt", [F32, BF16])
+@pytest.mark.parametrize("N,V", SHAPES)
+@pytest.mark.parametrize("T", [0.5, 1.0, 1.5, 2.0, 4.0])
+def test_rows_far_from_zero(cuda_ok, dt, N, V, T):
+    """Whole rows at or around one value of every magnitude."""
+    g = gen(N + V + 1)
+    k = 5
+    base = torch.tensor([-1e30, -1e10, -1e20, 1e10, -3e9, 3e5, -6e5, 8e5, -1e6, 3e6, -1e7, 1e30], device=DEV)
+    at = base[torch.arange(N, device=DEV) % 12][:, None]
+    spread = torch.where(at.abs() < 2e7, torch.randn(N, V, generator=g, device=DEV) * 2, 0.0)
+    x = (at + spread).to(dt)
+    x[::5, 3] *= 1 + 2.0 ** -6  # one token of some rows apart
+    ids = torch.stack([torch.randperm(V, generator=g, device=DEV)[:k] for _ in range(N)]).to(torch.int32)
+    hot = x.argmax(1).to(torch.int32)
+    lead = x.max(1).values > x.min(1).values  # rows that are not level: the teacher lists tokens near the largest
+    near = (x >= x.max(1, keepdim=True).values - 20).float()
+    ids = torch.where(lead[:, None], torch.multinomial(near, 1).to(torch.int32), ids)
+    ids[lead, 1:] = -1
+    tg = torch.where(lead, hot, ids[:, 0])
+    tl = torch.randn(N, k, generator=g, device=DEV)
+    for hard in (False, True):
+        check(x, ids, tl, tg if hard else None, T, 0.6, None)
+    # the rest of the teacher's mass, where a token that is not listed shares it with the largest
+    level = ~lead
+    lse = torch.logsumexp((tl / T).masked_fill(ids < 0, -math.inf), 1) + 0.3
+    for hard in (False, True):
+        check(x[level], ids[level], tl[level], tg[level] if hard else None, T, 0.6, lse[level])
