@@ -7,6 +7,7 @@
 //
 // With the gradient, a row (64 KB at 32,768 bfloat16 logits) is read from memory once, into the shared memory of a
 // block, or of a cluster of blocks that exchange their maxima and sums; the gradient is formed from that copy.
+#include <float.h>
 #include <math_constants.h>
 #include <type_traits>
 #include "tma.cuh"
@@ -738,10 +739,91 @@ __global__ void __launch_bounds__(kRowsThreads, 1) distill_rows_kernel(DistillAr
   }
 }
 
-// The loss alone: the row streams through registers, each thread keeping the largest logit it has seen and its sums
-// relative to that.  Where the teacher's remaining mass counts, a bit per token tells which are listed.
+// The largest value of a row, and the sums of three, over its blocks.
+template <int NT, typename Cluster>
+__device__ __forceinline__ float row_max(Cluster& cluster, DistillShared& s, const Row& q, float m) {
+  const int tid = threadIdx.x;
+  m = warp_max(m);
+  if ((tid & 31) == 0) s.warp[0][tid >> 5] = m;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < (NT / 32); ++w) m = fmaxf(m, s.warp[0][w]);
+  if (q.C > 1) {
+    if (tid < q.C) *cluster.map_shared_rank(&s.part[0][q.rank], tid) = m;
+    cluster.sync();
+    for (int r = 0; r < q.C; ++r) m = fmaxf(m, s.part[0][r]);
+  }
+  return m;
+}
+template <int NT, typename Cluster>
+__device__ __forceinline__ void row_sum3(Cluster& cluster, DistillShared& s, const Row& q, float& a, float& b, float& c) {
+  const int tid = threadIdx.x;
+  block_sum3<NT>(s, a, b, c);
+  if (q.C > 1) {
+    if (tid < q.C) {
+      *cluster.map_shared_rank(&s.part[1][q.rank], tid) = a;
+      *cluster.map_shared_rank(&s.part[2][q.rank], tid) = b;
+      *cluster.map_shared_rank(&s.part[3][q.rank], tid) = c;
+    }
+    cluster.sync();
+    a = b = c = 0.f;
+    for (int r = 0; r < q.C; ++r) {
+      a += s.part[1][r];
+      b += s.part[2][r];
+      c += s.part[3][r];
+    }
+  }
+}
+
+// The loss alone of a far row, from the row once more: its largest logit (all of them may lie below where the threads began),
+// and the sums over differences to it.  Out of line: inlined, it took registers from the loop over ordinary rows.
 template <typename T, Exps X, int NT>
-__global__ void __launch_bounds__(NT, 1536 / NT) distill_loss_kernel(DistillArgs a, int slice) {
+__device__ __noinline__ void far_loss(const DistillArgs& a, int slice, DistillShared& s, const uint32_t* is_listed) {
+  auto cluster = cg::this_cluster();
+  const int C = (int)cluster.num_blocks();
+  const T* x;
+  Row q = row_of<T>(a, slice, C, (int)cluster.block_rank(), blockIdx.x / C, x);
+  load_terms(a, q);
+  const int tid = threadIdx.x;
+  const float ct = q.inv_t * kLog2e, c1 = kLog2e;
+  const bool tail = a.t_lse != nullptr;
+  auto apart = [&](int i) { return tail && ((is_listed[i >> 5] >> (i & 31)) & 1); };
+  float mx = -CUDART_INF_F;
+#pragma unroll 1
+  for (int i = q.lo + tid; i < q.hi; i += NT) mx = fmaxf(mx, to_f32(x[q.v0 + i]));
+  mx = row_max<NT>(cluster, s, q, mx);
+  float st = 0.f, s1 = 0.f, listed = 0.f;
+#pragma unroll 1
+  for (int i = q.lo + tid; i < q.hi; i += NT) {
+    const float f = to_f32(x[q.v0 + i]) - mx;
+    if (apart(i)) continue;
+    st += ex2(f * ct);
+    if (X != kOne) s1 += ex2(f * c1);
+  }
+  for (int j = tid; j < q.k; j += NT) {
+    const int i = s.id[j] - q.v0;
+    s.val[j] -= mx;
+    if (!tail || s.id[j] < 0 || i < q.lo || i >= q.hi || !is_first(s, j)) continue;
+    listed += ex2(s.val[j] * ct);
+    if (X != kOne) s1 += ex2(s.val[j] * c1);
+  }
+  if (tid == 0) s.target_val -= mx;
+  row_sum3<NT>(cluster, s, q, st, s1, listed);
+  const float rest = st;
+  st += listed;
+  if (X == kOne) s1 = st;
+  if (q.rank == 0 && tid < 32) {
+    const float loss = row_loss(a, q, s, ct, 0.f, 0.f, st, s1, rest);
+    if (tid == 0) a.loss[q.row] = loss;
+  }
+}
+
+// The loss alone: the row streams through registers, each thread keeping the largest logit it has seen and its sums
+// relative to that, or to a value below all rows that are not far (kFar) while it has seen none above: tokens at a mask's
+// lowest value count for nothing beside a row's others, and their product with c may be beyond float32.  Where the
+// teacher's remaining mass counts, a bit per token tells which are listed.
+template <typename T, Exps X, int NT>
+__global__ void __launch_bounds__(NT, 1536 / NT) distill_loss_kernel(const __grid_constant__ DistillArgs a, int slice) {
   pdl_enter();
   constexpr int E = Chunk<T>::E, U = 4;
   extern __shared__ uint32_t is_listed[];
@@ -780,11 +862,12 @@ __global__ void __launch_bounds__(NT, 1536 / NT) distill_loss_kernel(DistillArgs
     __syncthreads();
   }
   const float ct = q.inv_t * kLog2e, c1 = kLog2e;
-  float mt = -CUDART_INF_F, nBt = 0.f, nB1 = 0.f, st = 0.f, s1 = 0.f;
+  float mt = fmaxf(-2.f * kFar * kLn2 * (X == kOne ? a.temperature : fminf(a.temperature, 1.f)), -FLT_MAX);
+  float nBt = -__fmul_rn(mt, ct), nB1 = -__fmul_rn(mt, c1), st = 0.f, s1 = 0.f;
   auto raise = [&](float cm) {  // the largest logit so far
     if (cm > mt) {
       const float nt = -__fmul_rn(cm, ct), n1 = -__fmul_rn(cm, c1);
-      if (mt > -CUDART_INF_F) {
+      if ((X == kOne ? st : st + s1) != 0.f) {
         st *= ex2(nt - nBt);
         if (X != kOne) s1 *= ex2(n1 - nB1);
       }
@@ -839,37 +922,14 @@ __global__ void __launch_bounds__(NT, 1536 / NT) distill_loss_kernel(DistillArgs
       if (X != kOne) s1 += ex2(fmaf(f, c1, nB1));
     }
   }
-  float mx = warp_max(mt);
-  if ((tid & 31) == 0) s.warp[0][tid >> 5] = mx;
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < (NT / 32); ++w) mx = fmaxf(mx, s.warp[0][w]);
+  const float mx = row_max<NT>(cluster, s, q, mt);
   if (tid >= NT - 32) teacher_softmax(a, q, s);
-  if (C > 1) {
-    if (tid < C) *cluster.map_shared_rank(&s.part[0][q.rank], tid) = mx;
-    cluster.sync();
-    for (int r = 0; r < C; ++r) mx = fmaxf(mx, s.part[0][r]);
-  }
-  // all sums relative to the row's largest logit
   const bool far = is_far<X>(mx, ct, c1);
-  if (far) {  // sums of their own
-    st = s1 = 0.f;
-    for (int i = lo + tid; i < hi; i += NT) {
-      const float f = to_f32(x[v0 + i]) - mx;
-      if (tail && ((is_listed[i >> 5] >> (i & 31)) & 1)) continue;
-      st += ex2(f * ct);
-      if (X != kOne) s1 += ex2(f * c1);
-    }
-    for (int j = tid; j < k; j += NT) s.val[j] -= mx;
-    if (tid == NT - 1) s.target_val -= mx;
-    mx = 0.f;
-  }
+  // all sums relative to the row's largest logit
   const float Mt = __fmul_rn(mx, ct), M1 = __fmul_rn(mx, c1);
   float listed = 0.f;
-  if (mt > -CUDART_INF_F && !far) {  // else they are 0, or NaN
-    st *= ex2(-nBt - Mt);
-    s1 *= ex2(-nB1 - M1);
-  }
+  st *= ex2(-nBt - Mt);
+  s1 *= ex2(-nB1 - M1);
   if (tail)
     for (int j = tid; j < k; j += NT) {
       const int i = s.id[j] - v0;
@@ -877,25 +937,13 @@ __global__ void __launch_bounds__(NT, 1536 / NT) distill_loss_kernel(DistillArgs
       listed += ex2(fmaf(s.val[j], ct, -Mt));
       if (X != kOne) s1 += ex2(fmaf(s.val[j], c1, -M1));
     }
-  block_sum3<NT>(s, st, s1, listed);
-  if (C > 1) {
-    if (tid < C) {
-      *cluster.map_shared_rank(&s.part[1][q.rank], tid) = st;
-      *cluster.map_shared_rank(&s.part[2][q.rank], tid) = s1;
-      *cluster.map_shared_rank(&s.part[3][q.rank], tid) = listed;
-    }
-    cluster.sync();
-    st = s1 = listed = 0.f;
-    for (int r = 0; r < C; ++r) {
-      st += s.part[1][r];
-      s1 += s.part[2][r];
-      listed += s.part[3][r];
-    }
-  }
+  row_sum3<NT>(cluster, s, q, st, s1, listed);
   const float rest = st;
   st += listed;
   if (X == kOne) s1 = st;
-  if (q.rank == 0 && tid < 32) {
+  if (__builtin_expect(far, 0)) {  // the same in all blocks of the row
+    far_loss<T, X, NT>(a, slice, s, is_listed);
+  } else if (q.rank == 0 && tid < 32) {
     const float loss = row_loss(a, q, s, ct, Mt, M1, st, s1, rest);
     if (tid == 0) a.loss[q.row] = loss;
   }

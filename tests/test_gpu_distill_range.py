@@ -112,3 +112,42 @@ def test_rows_far_from_zero(cuda_ok, dt, N, V, T):
     lse = torch.logsumexp((tl / T).masked_fill(ids < 0, -math.inf), 1) + 0.3
     for hard in (False, True):
         check(x[level], ids[level], tl[level], tg[level] if hard else None, T, 0.6, lse[level])
+
+
+@pytest.mark.parametrize("dt", [F32, BF16])
+@pytest.mark.parametrize("N,V", SHAPES)
+@pytest.mark.parametrize("T", [0.5, 1.0, 1.5, 2.0, 4.0])
+def test_partly_masked_rows(cuda_ok, dt, N, V, T):
+    """1, 8, 64 and most of a row's tokens are ordinary, at its beginning, its end, side by side inside or anywhere;
+    the others hold a mask's finite lowest value."""
+    g = gen(N + V)
+    k = 5
+    x = torch.empty(N, V, device=DEV)
+    ids = torch.full((N, k), -1, device=DEV, dtype=torch.int32)
+    tg = torch.empty(N, device=DEV, dtype=torch.int32)
+    one = torch.zeros(N, device=DEV, dtype=torch.bool)
+    lowest = [torch.finfo(dt).min, -1e30, -1e20, -1e10]
+    order = torch.randperm(48 * (1 + N // 48), generator=g, device=DEV).tolist()
+    for i in range(N):
+        c = order[i] % 48
+        n = (1, 8, 64, V - 100)[c % 4]
+        start = {0: 0, 1: V - n, 2: (V - n) // 2 // 8 * 8}.get(c // 4 % 3, 0)
+        at = torch.arange(start, start + n, device=DEV)
+        if c % 7 == 3:
+            at = torch.randperm(V, generator=g, device=DEV)[:n]
+        x[i] = lowest[c // 12]
+        x[i, at] = 2 * torch.randn(n, generator=g, device=DEV)
+        some = at[torch.randperm(n, generator=g, device=DEV)[:k]]
+        m = min(k, n)
+        ids[i, :m] = some[:m].to(torch.int32)
+        tg[i] = at[n // 2]
+        one[i] = n == 1
+    x = x.to(dt)
+    tl = torch.randn(N, k, generator=g, device=DEV)
+    for hard in (False, True):
+        for tail in (False, True):
+            e = ids.masked_fill(one[:, None], -1) if tail else ids  # the rest of the mass needs a token to go to
+            lse = None
+            if tail:
+                lse = torch.logsumexp((tl / T).masked_fill(e < 0, -math.inf), 1).nan_to_num(neginf=0.0) + 0.3
+            check(x, e, tl, tg if hard else None, T, 0.6, lse)
