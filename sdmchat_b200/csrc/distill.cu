@@ -209,10 +209,16 @@ __device__ __forceinline__ bool is_first(const S& s, int j) {
   return true;
 }
 
-// The row's loss from its sums (one warp): st, s1 over all tokens at T and at 1, rest over the unlisted ones at T.
+// The student's mass on the unlisted tokens is a sum of its own, relative to the row's largest logit like the others
+// until it falls below kApart: terms under 2^-126 are 0, and 2^18 of those may have counted.  From there on (listed
+// tokens that lead by 55 T and more) it is taken again, relative to the largest unlisted logit.
+constexpr float kApart = 8.271806125530277e-25f;  // 2^-80
+
+// The row's loss from its sums (one warp): st, s1 over all tokens at T and at 1, lrest the logarithm of the sum over the
+// unlisted ones at T.
 template <typename S>
 __device__ __forceinline__ float row_loss(const DistillArgs& a, const Row& q, const S& s, float ct,
-                                          float Bt, float B1, float st, float s1, float rest) {
+                                          float Bt, float B1, float st, float s1, float lrest) {
   const int lane = threadIdx.x & 31;
   float loss = 0.f;
   if (s.p_sum != -1.f) {
@@ -225,7 +231,7 @@ __device__ __forceinline__ float row_loss(const DistillArgs& a, const Row& q, co
     }
     sum = warp_sum(sum);
     const float pr = a.t_lse ? fmaxf(0.f, 1.f - s.p_sum) : 0.f;
-    if (pr > 0.f) sum += pr * (logf(pr) - kLn2 * (log2f(rest) - lst));
+    if (pr > 0.f) sum += pr * (logf(pr) - kLn2 * (lrest - lst));
     loss = a.alpha * sum * (a.temperature * a.temperature);
   }
   if (q.hard) loss += (1.f - a.alpha) * kLn2 * (log2f(s1) - fmaf(s.target_val, kLog2e, -B1));
@@ -250,10 +256,10 @@ struct Chunks {
   }
 };
 
-// Whether a row's largest logit, times the larger c that is used, is at or beyond kFar (a row that is all at a mask's lowest
-// value).  Its logits are then taken relative to the largest first: such differences are exact where a logit is within a factor of
-// two of the largest, and any other is 2^19 / c or more below.  (At that c: the rounding of such a difference to
-// bfloat16, 2^-9 of it, counts only where T is above 5,000 and a hard target asks for T = 1 besides.)
+// Whether a row's largest logit, times the larger c that is used, is at or beyond kFar (a row that is all at a mask's
+// lowest value).  Its logits are then taken relative to the largest first: such differences are exact where a logit is
+// within a factor of two of the largest, and any other is 2^19 / c or more below.  (At that c: the rounding of such a
+// difference to bfloat16, 2^-9 of it, counts only where T is above 5,000 and a hard target asks for T = 1 besides.)
 template <Exps X>
 __device__ __forceinline__ bool is_far(float mx, float ct, float c1) {
   return fabsf(mx) < CUDART_INF_F && !(fabsf(mx) * (X == kOne ? ct : fmaxf(ct, c1)) < kFar);
@@ -269,9 +275,77 @@ __device__ __forceinline__ void lower_row(T* buf, int c0, int c1, int edge, int 
   if (edge >= 0) buf[edge] = from_f32<T>(to_f32(buf[edge]) - mx);
 }
 
-// Loss and gradient.
-template <typename T, Exps X, int NT>
-__global__ void __launch_bounds__(NT, 768 / NT) distill_grad_kernel(DistillArgs a, int slice) {
+// Largest value and sum over a row's threads: a block's, and its cluster's; or a team's of the kernel of persistent blocks.
+template <int NT>
+struct BlockReduce {
+  DistillShared& s;
+  int C, rank;
+  __device__ float max(float m) const {
+    m = warp_max(m);
+    if ((threadIdx.x & 31) == 0) s.warp[0][threadIdx.x >> 5] = m;
+    __syncthreads();
+    for (int w = 0; w < (NT / 32); ++w) m = fmaxf(m, s.warp[0][w]);
+    return across(0, m, true);
+  }
+  __device__ float sum(float v) const {
+    float none = 0.f, none_ = 0.f;
+    block_sum3<NT>(s, v, none, none_);
+    return across(1, v, false);
+  }
+  __device__ float across(int part, float v, bool largest) const {
+    if (C == 1) return v;
+    auto cluster = cg::this_cluster();
+    if ((int)threadIdx.x < C) *cluster.map_shared_rank(&s.part[part][rank], threadIdx.x) = v;
+    cluster.sync();
+    v = s.part[part][0];
+    for (int r = 1; r < C; ++r) v = largest ? fmaxf(v, s.part[part][r]) : v + s.part[part][r];
+    return v;
+  }
+};
+
+// The gradient of a row's unlisted tokens where the listed ones lead by so much (kApart), from its copy in `buf`, where
+// the listed ones are at -infinity: T (q - p_r q / q_r) without the first term, which is below 2^-56 of the second, and the hard
+// target's.  nBt, nB1: the row's base; kr: the factor of q / q_r.  Returns the logarithm of their sum, for row_loss.
+// Out of line, so that ordinary rows keep their registers (16,384 x 32,768: 391 us, 401 with this inlined).
+template <typename T, int NT, typename Reduce>
+__device__ __noinline__ float apart_gradient(DistillArgs a, int slice, int64_t row, int C, int rank, int tid, const T* buf,
+                                             Reduce over, float nBt, float nB1, float kr, float q1, float kh) {
+  constexpr int E = Chunk<T>::E;
+  const T* x;
+  Row q = row_of<T>(a, slice, C, rank, row, x);
+  load_terms(a, q);
+  T* g = static_cast<T*>(a.dlogits) + row * a.ld_grad;
+  const Chunks ch(q, E);
+  const int edge = ch.edge(tid);
+  const float ct = q.inv_t * kLog2e, c1 = kLog2e;
+  auto each = [&](auto f) {
+#pragma unroll 1
+    for (int i = ch.c0 * E + tid; i < ch.c1 * E; i += NT) f(i, to_f32(buf[i]));
+    if (edge >= 0) f(edge, to_f32(buf[edge]));
+  };
+  float mr = -CUDART_INF_F, sum = 0.f;
+  each([&](int, float v) { mr = fmaxf(mr, v); });
+  mr = over.max(mr);
+  const bool none = mr == -CUDART_INF_F;  // no unlisted token is possible, and none has a gradient
+  if (none) mr = 0.f;
+  each([&](int, float v) { sum += ex2((v - mr) * ct); });
+  sum = over.sum(sum);
+  kr = none ? 0.f : kr / sum;
+  each([&](int i, float v) {
+    const float y = q1 * ex2(fmaf(v, c1, nB1)) - kr * ex2((v - mr) * ct);
+    g[q.v0 + i] = from_f32<T>(q.hard && q.v0 + i == q.tgt ? y - kh : y);
+  });
+  return log2f(sum) + fmaf(mr, ct, nBt);
+}
+
+// Threads of an SM, by the registers (64, 72 and 80) that the loops over an ordinary row take, where the call in the kernel
+// would have them take more.
+template <typename T, Exps X>
+constexpr int kGradThreads = sizeof(T) == 4 ? 768 : X == kTwo ? 896 : 1024;
+
+// Loss and gradient.  kTail: the teacher's remaining mass counts (teacher_lse is given).
+template <typename T, Exps X, int NT, bool kTail>
+__global__ void __launch_bounds__(NT, (kTail ? kGradThreads<T, X> : 768) / NT) distill_grad_kernel(DistillArgs a, int slice) {
   pdl_enter();
   constexpr int E = Chunk<T>::E;
   typedef typename std::conditional<sizeof(T) == 2, uint16_t, uint32_t>::type Tag;
@@ -420,7 +494,7 @@ __global__ void __launch_bounds__(NT, 768 / NT) distill_grad_kernel(DistillArgs 
   if (X == kOne || st != st) s1 = st;  // a NaN or an infinity shows in st
   const float P = s.p_sum;
   const bool soft = P != -1.f;
-  const float pr = soft && a.t_lse ? fmaxf(0.f, 1.f - P) : 0.f;
+  const float pr = kTail && soft ? fmaxf(0.f, 1.f - P) : 0.f;
 
   // the gradient: a token that is not listed has qr exp(logit / T) + q1 exp(logit), each over its sum
   const float scale = q.w * a.grad_scale;
@@ -436,7 +510,12 @@ __global__ void __launch_bounds__(NT, 768 / NT) distill_grad_kernel(DistillArgs 
     if (X == kFourth) return fmaf(q1, power<X>(t), qm * t);
     return qm * t;
   };
-  if (vec_out) {
+  const bool apart = kTail && pr > 0.f && rest < kApart;  // the same in all blocks of the row
+  float lrest = 0.f;
+  if (kTail && apart) {
+    lrest = apart_gradient<T, NT>(a, slice, q.row, C, q.rank, tid, buf, BlockReduce<NT>{s, C, q.rank}, nBt, nB1, ks * pr,
+                                  q1, kh);
+  } else if (vec_out) {
 #pragma unroll 2
     for (int c = ch.c0 + tid; c < ch.c1; c += NT) {
       float f[E];
@@ -460,9 +539,9 @@ __global__ void __launch_bounds__(NT, 768 / NT) distill_grad_kernel(DistillArgs 
   } else {
     for (int i = ch.c0 * E + tid; i < ch.c1 * E; i += NT) g[v0 + i] = from_f32<T>(value(to_f32(buf[i])));
   }
-  if (edge >= 0) g[v0 + edge] = from_f32<T>(value(to_f32(buf[edge])));
+  if (edge >= 0 && !apart) g[v0 + edge] = from_f32<T>(value(to_f32(buf[edge])));
   if (q.rank == 0 && tid >= NT - 32) {
-    const float loss = row_loss(a, q, s, ct, -nBt, -nB1, st, s1, rest);
+    const float loss = row_loss(a, q, s, ct, -nBt, -nB1, st, s1, apart ? lrest : log2f(rest));
     if (tid == NT - 1) a.loss[q.row] = loss;
   }
   __syncthreads();  // the tokens with a term of their own are written over the pass above
@@ -483,7 +562,7 @@ __global__ void __launch_bounds__(NT, 768 / NT) distill_grad_kernel(DistillArgs 
   if (q.hard && tid < 32 && q.tgt - v0 >= lo && q.tgt - v0 < hi) {
     bool listed_too = false;
     for (int j = tid; j < k; j += 32) listed_too |= s.id[j] == q.tgt;
-    if (!__any_sync(0xffffffffu, listed_too) && tid == 0)
+    if (!__any_sync(0xffffffffu, listed_too) && tid == 0 && !apart)
       g[q.tgt] = from_f32<T>(qr * ex2(fmaf(s.target_val, ct, nBt)) + q1 * ex2(fmaf(s.target_val, c1, nB1)) - kh);
   }
 }
@@ -505,7 +584,28 @@ struct TeamTeacher {
   int repeated, tgt;
 };
 
-template <typename T, Exps X>
+struct TeamReduce {
+  float (*red)[kTeamWarps];
+  int barrier;
+  __device__ void sync() const { asm volatile("bar.sync %0, %1;" ::"r"(barrier), "n"(kTeam) : "memory"); }
+  __device__ float max(float m) const {
+    m = warp_max(m);
+    if ((threadIdx.x & 31) == 0) red[0][threadIdx.x % kTeam / 32] = m;
+    sync();
+    for (int w = 0; w < kTeamWarps; ++w) m = fmaxf(m, red[0][w]);
+    return m;
+  }
+  __device__ float sum(float v) const {
+    v = warp_sum(v);
+    if ((threadIdx.x & 31) == 0) red[1][threadIdx.x % kTeam / 32] = v;
+    sync();
+    v = 0.f;
+    for (int w = 0; w < kTeamWarps; ++w) v += red[1][w];
+    return v;
+  }
+};
+
+template <typename T, Exps X, bool kTail>
 __global__ void __launch_bounds__(kRowsThreads, 1) distill_rows_kernel(DistillArgs a, int slice) {
   pdl_enter();
   constexpr int E = Chunk<T>::E;
@@ -684,7 +784,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) distill_rows_kernel(DistillAr
     if (X == kOne || st != st) s1 = st;
     const float P = s.p_sum;
     const bool soft = P != -1.f;
-    const float pr = soft && a.t_lse ? fmaxf(0.f, 1.f - P) : 0.f;
+    const float pr = kTail && soft ? fmaxf(0.f, 1.f - P) : 0.f;
     const float scale = q.w * a.grad_scale;
     const float ks = soft ? scale * a.alpha * a.temperature : 0.f, kh = q.hard ? scale * (1.f - a.alpha) : 0.f;
     const float qt = soft ? ks * (P + pr) / st : 0.f;
@@ -694,10 +794,15 @@ __global__ void __launch_bounds__(kRowsThreads, 1) distill_rows_kernel(DistillAr
     auto value = [&](float f) {
       const float t = ex2(fmaf(f, ct, nBt));
       if (X == kSquare) return t * fmaf(q1, t, qm);
-    if (X == kFourth) return fmaf(q1, power<X>(t), qm * t);
+      if (X == kFourth) return fmaf(q1, power<X>(t), qm * t);
       return qm * t;
     };
-    if (vec_out) {
+    const bool apart = kTail && pr > 0.f && rest < kApart;
+    float lrest = 0.f;
+    if (kTail && apart) {
+      lrest = apart_gradient<T, kTeam>(a, slice, row, 1, 0, tid, buf, TeamReduce{red[team], team + 1}, nBt, nB1, ks * pr,
+                                       q1, kh);
+    } else if (vec_out) {
 #pragma unroll 4
       for (int c = ch.c0 + tid; c < ch.c1; c += kTeam) {
         float f[E];
@@ -709,7 +814,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) distill_rows_kernel(DistillAr
     } else {
       for (int p = ch.c0 * E + tid; p < ch.c1 * E; p += kTeam) g[v0 + p] = from_f32<T>(value(to_f32(buf[p])));
     }
-    if (edge >= 0) g[v0 + edge] = from_f32<T>(value(to_f32(buf[edge])));
+    if (edge >= 0 && !apart) g[v0 + edge] = from_f32<T>(value(to_f32(buf[edge])));
     team_sync();
     if (own) {
       const int id = s.id[tid];
@@ -725,12 +830,12 @@ __global__ void __launch_bounds__(kRowsThreads, 1) distill_rows_kernel(DistillAr
       g[id] = from_f32<T>(r);
     }
     if (warp == kTeamWarps - 1) {
-      const float loss = row_loss(a, q, s, ct, -nBt, -nB1, st, s1, rest);
+      const float loss = row_loss(a, q, s, ct, -nBt, -nB1, st, s1, apart ? lrest : log2f(rest));
       if (lane == 0) a.loss[row] = loss;
       if (q.hard) {
         bool listed_too = false;
         for (int j = lane; j < k; j += 32) listed_too |= s.id[j] == q.tgt;
-        if (!__any_sync(0xffffffffu, listed_too) && lane == 0)
+        if (!__any_sync(0xffffffffu, listed_too) && lane == 0 && !apart)
           g[q.tgt] = from_f32<T>(qr * ex2(fmaf(s.target_val, ct, nBt)) + q1 * ex2(fmaf(s.target_val, c1, nB1)) - kh);
       }
     }
@@ -775,10 +880,13 @@ __device__ __forceinline__ void row_sum3(Cluster& cluster, DistillShared& s, con
   }
 }
 
-// The loss alone of a far row, from the row once more: its largest logit (all of them may lie below where the threads began),
-// and the sums over differences to it.  Out of line: inlined, it took registers from the loop over ordinary rows.
-template <typename T, Exps X, int NT>
-__device__ __noinline__ void far_loss(const DistillArgs& a, int slice, DistillShared& s, const uint32_t* is_listed) {
+// The loss alone of a far row, or of one whose listed tokens lead by so much (kApart), from the row once more: its largest
+// logit (all of them may lie below where the threads began), the sums over differences to it, and the unlisted
+// tokens' over differences to the largest of those.  Out of line: inlined, it took registers from the loop over
+// ordinary rows.
+template <typename T, int NT, bool kTail>
+__device__ __noinline__ void careful_loss(const DistillArgs& a, int slice, DistillShared& s, const uint32_t* is_listed,
+                                          bool two) {
   auto cluster = cg::this_cluster();
   const int C = (int)cluster.num_blocks();
   const T* x;
@@ -786,7 +894,7 @@ __device__ __noinline__ void far_loss(const DistillArgs& a, int slice, DistillSh
   load_terms(a, q);
   const int tid = threadIdx.x;
   const float ct = q.inv_t * kLog2e, c1 = kLog2e;
-  const bool tail = a.t_lse != nullptr;
+  constexpr bool tail = kTail;
   auto apart = [&](int i) { return tail && ((is_listed[i >> 5] >> (i & 31)) & 1); };
   float mx = -CUDART_INF_F;
 #pragma unroll 1
@@ -798,22 +906,38 @@ __device__ __noinline__ void far_loss(const DistillArgs& a, int slice, DistillSh
     const float f = to_f32(x[q.v0 + i]) - mx;
     if (apart(i)) continue;
     st += ex2(f * ct);
-    if (X != kOne) s1 += ex2(f * c1);
+    if (two) s1 += ex2(f * c1);
   }
   for (int j = tid; j < q.k; j += NT) {
     const int i = s.id[j] - q.v0;
     s.val[j] -= mx;
     if (!tail || s.id[j] < 0 || i < q.lo || i >= q.hi || !is_first(s, j)) continue;
     listed += ex2(s.val[j] * ct);
-    if (X != kOne) s1 += ex2(s.val[j] * c1);
+    if (two) s1 += ex2(s.val[j] * c1);
   }
   if (tid == 0) s.target_val -= mx;
   row_sum3<NT>(cluster, s, q, st, s1, listed);
-  const float rest = st;
+  float lrest = log2f(st);
   st += listed;
-  if (X == kOne) s1 = st;
+  if (!two) s1 = st;
+  if (tail) {
+    float mr = -CUDART_INF_F, sum = 0.f, none = 0.f, none_ = 0.f;
+#pragma unroll 1
+    for (int i = q.lo + tid; i < q.hi; i += NT)
+      if (!apart(i)) mr = fmaxf(mr, to_f32(x[q.v0 + i]));
+    mr = row_max<NT>(cluster, s, q, mr);
+    if (mr == -CUDART_INF_F) {
+      lrest = mr;
+    } else {
+#pragma unroll 1
+      for (int i = q.lo + tid; i < q.hi; i += NT)
+        if (!apart(i)) sum += ex2((to_f32(x[q.v0 + i]) - mr) * ct);
+      row_sum3<NT>(cluster, s, q, sum, none, none_);
+      lrest = log2f(sum) + (mr - mx) * ct;
+    }
+  }
   if (q.rank == 0 && tid < 32) {
-    const float loss = row_loss(a, q, s, ct, 0.f, 0.f, st, s1, rest);
+    const float loss = row_loss(a, q, s, ct, 0.f, 0.f, st, s1, lrest);
     if (tid == 0) a.loss[q.row] = loss;
   }
 }
@@ -822,7 +946,7 @@ __device__ __noinline__ void far_loss(const DistillArgs& a, int slice, DistillSh
 // relative to that, or to a value below all rows that are not far (kFar) while it has seen none above: tokens at a mask's
 // lowest value count for nothing beside a row's others, and their product with c may be beyond float32.  Where the
 // teacher's remaining mass counts, a bit per token tells which are listed.
-template <typename T, Exps X, int NT>
+template <typename T, Exps X, int NT, bool kTail>
 __global__ void __launch_bounds__(NT, 1536 / NT) distill_loss_kernel(const __grid_constant__ DistillArgs a, int slice) {
   pdl_enter();
   constexpr int E = Chunk<T>::E, U = 4;
@@ -839,7 +963,7 @@ __global__ void __launch_bounds__(NT, 1536 / NT) distill_loss_kernel(const __gri
     if (q.rank == 0 && tid == 0) a.loss[q.row] = 0.f;
     return;
   }
-  const bool tail = a.t_lse != nullptr;
+  constexpr bool tail = kTail;
   const Chunks ch(q, E);
   // the row is on its way to L2 while its teacher is fetched (8,192 rows of 50,021: 139 us without,
   // 132 with; 65,536 of 8,192: 340 and 311)
@@ -924,7 +1048,6 @@ __global__ void __launch_bounds__(NT, 1536 / NT) distill_loss_kernel(const __gri
   }
   const float mx = row_max<NT>(cluster, s, q, mt);
   if (tid >= NT - 32) teacher_softmax(a, q, s);
-  const bool far = is_far<X>(mx, ct, c1);
   // all sums relative to the row's largest logit
   const float Mt = __fmul_rn(mx, ct), M1 = __fmul_rn(mx, c1);
   float listed = 0.f;
@@ -941,11 +1064,13 @@ __global__ void __launch_bounds__(NT, 1536 / NT) distill_loss_kernel(const __gri
   const float rest = st;
   st += listed;
   if (X == kOne) s1 = st;
-  if (__builtin_expect(far, 0)) {  // the same in all blocks of the row
-    far_loss<T, X, NT>(a, slice, s, is_listed);
-  } else if (q.rank == 0 && tid < 32) {
-    const float loss = row_loss(a, q, s, ct, Mt, M1, st, s1, rest);
+  if (q.rank == 0 && tid < 32) {
+    const float loss = row_loss(a, q, s, ct, Mt, M1, st, s1, log2f(rest));
     if (tid == 0) a.loss[q.row] = loss;
+  }
+  if (is_far<X>(mx, ct, c1) || (tail && rest < kApart)) {  // the same in all blocks of the row
+    __syncthreads();
+    careful_loss<T, NT, kTail>(a, slice, s, is_listed, X != kOne);
   }
 }
 
@@ -980,9 +1105,11 @@ cudaError_t distill_n(const DistillArgs& a, int C, int slice, cudaStream_t st) {
   const unsigned grid = (unsigned)(a.N * C);
   LaunchScope scope_(a.dlogits ? "distill_grad" : "distill_loss", st);
   if (a.dlogits)
-    return launch_clusters(distill_grad_kernel<T, X, NT>, grid, C, NT, (size_t)slice * sizeof(T), st, a, slice);
+    return launch_clusters(a.t_lse ? distill_grad_kernel<T, X, NT, true> : distill_grad_kernel<T, X, NT, false>, grid, C, NT,
+                           (size_t)slice * sizeof(T), st, a, slice);
   const size_t smem = a.t_lse ? (size_t)(slice / 32) * 4 : 0;
-  return launch_clusters(distill_loss_kernel<T, X, NT>, grid, C, NT, smem, st, a, slice);
+  return launch_clusters(a.t_lse ? distill_loss_kernel<T, X, NT, true> : distill_loss_kernel<T, X, NT, false>, grid, C, NT,
+                         smem, st, a, slice);
 }
 
 template <typename T, Exps X>
@@ -1003,7 +1130,7 @@ cudaError_t distill_x(const DistillArgs& a, cudaStream_t st) {
   if constexpr (X != kTwo) {
     if (a.dlogits && C == 1 && a.k <= kTeamTeacher && a.N >= 4 * kSMs && row_bytes > 50 * 1024 &&
         kBuffers * row_bytes <= 200 * 1024) {
-      auto kern = distill_rows_kernel<T, X>;
+      auto kern = a.t_lse ? distill_rows_kernel<T, X, true> : distill_rows_kernel<T, X, false>;
       cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(kBuffers * row_bytes));
       if (e != cudaSuccess) return e;
       LaunchScope scope_("distill_rows", st);

@@ -151,3 +151,39 @@ def test_partly_masked_rows(cuda_ok, dt, N, V, T):
             if tail:
                 lse = torch.logsumexp((tl / T).masked_fill(e < 0, -math.inf), 1).nan_to_num(neginf=0.0) + 0.3
             check(x, e, tl, tg if hard else None, T, 0.6, lse)
+
+
+@pytest.mark.parametrize("dt", [F32, BF16])
+@pytest.mark.parametrize("N,V", SHAPES)
+@pytest.mark.parametrize("T", [0.7, 1.0, 1.5, 2.0, 4.0])
+def test_listed_tokens_lead(cuda_ok, dt, N, V, T):
+    """The teacher's remaining mass where the student gives the tokens that are not listed next to nothing."""
+    g = gen(N + V + 2)
+    k = 5
+    x = torch.randn(N, V, generator=g, device=DEV)
+    ids = torch.stack([torch.randperm(V, generator=g, device=DEV)[:k] for _ in range(N)]).to(torch.int32)
+    gap = torch.tensor([0.0, 20.0, 50.0, 61.0, 86.0, 100.0, 150.0, 300.0, 600.0, 1e4], device=DEV)
+    gap = gap[torch.arange(N, device=DEV) % 10]
+    far = torch.tensor([0.0, -1e6, 0.0], device=DEV)[torch.arange(N, device=DEV) % 3]  # rows far from zero among them
+    x.scatter_(1, ids[:, :3].long(), gap[:, None] + torch.randn(N, 3, generator=g, device=DEV))
+    x = (x + far[:, None]).to(dt)
+    tl = torch.randn(N, k, generator=g, device=DEV)
+    tg = torch.randint(0, V, (N,), generator=g, device=DEV, dtype=torch.int32)
+    tg = torch.where(torch.arange(N, device=DEV) % 2 == 0, ids[:, 0], tg)
+    lse = torch.logsumexp(tl / T, 1) + 0.3
+    for hard in (False, True):
+        check(x, ids, tl, tg if hard else None, T, 0.6, lse)
+    # the others at a mask's finite lowest value (finfo.min times 1 / T and log2(e) is beyond float32: the loss is infinite)
+    others = torch.ones(N, V, device=DEV, dtype=torch.bool).scatter_(1, ids.long(), False)
+    for low in (-1e10, -1e20, torch.finfo(dt).min):
+        y = torch.randn(N, V, generator=g, device=DEV).masked_fill(others, low).to(dt)
+        tg = torch.where(torch.arange(N, device=DEV) % 2 == 0, ids[:, 0], -1)
+        for hard in (False, True):
+            check(y, ids, tl, tg if hard else None, T, 0.6, lse, with_loss=low > -1e30)
+    # nothing but listed tokens is possible: the loss is infinite, and the others, at -infinity, have no gradient
+    listed = torch.zeros(N, V, device=DEV, dtype=torch.bool).scatter_(1, ids.long(), True)
+    y = x.masked_fill(~listed, -math.inf)
+    loss, grad = S.distill_loss_and_grad(y, ids, tl, None, T, 0.6, None, lse)
+    only = S.distill_loss(y, ids, tl, None, T, 0.6, None, lse, reduction="none")
+    assert torch.isposinf(loss).all() and torch.isposinf(only).all()
+    assert torch.isfinite(grad).all() and (grad[~listed] == 0).all()
