@@ -580,7 +580,7 @@ constexpr int kRing = kTeams * kBuffers;
 struct TeamTeacher {
   int id[kTeamTeacher];
   float logp[kTeamTeacher], val[kTeamTeacher];
-  float target_val, p_sum, w;
+  float target_val, p_sum;
   int repeated, tgt;
 };
 
@@ -624,9 +624,10 @@ __global__ void __launch_bounds__(kRowsThreads, 1) distill_rows_kernel(DistillAr
     tma::mbar_init_fence();
   }
   __syncthreads();
-  // row i of the block goes to team i mod 2 and buffer i mod 3; a wait that gives up waits once more for the copy that
-  // may be under way, and leaves
-  auto give_up = [&](int i) { tma::mbar_wait(&full[i % kRing], (i / kRing) & 1); };
+  // Row i of the block goes to team i mod 2 and buffer i mod 3.  Where a wait gives up, those who meet at a barrier leave
+  // together: a team finds out at its first barrier of a row whether all of its threads saw the row arrive, and a warp that
+  // runs ahead waits by one lane.  The block's shared memory is kept until the copies into it have landed, by the warps
+  // that issued them.
   if (threadIdx.x >= kTeams * kTeam) {  // the warps that run ahead
     int i = ((int)threadIdx.x - kTeams * kTeam) / 32;
     for (int64_t row = blockIdx.x + (int64_t)i * gridDim.x; row < a.N; row += (int64_t)kTeams * gridDim.x, i += kTeams) {
@@ -649,7 +650,11 @@ __global__ void __launch_bounds__(kRowsThreads, 1) distill_rows_kernel(DistillAr
       }
       const float target_val = q.hard ? to_f32(x[q.tgt]) : 0.f;
       const int last = i - kBuffers;  // the row that had the buffer
-      if (last >= 0 && !tma::mbar_wait(&empty[last % kRing], (last / kRing) & 1)) return give_up(last);
+      if (last >= 0) {
+        const int free_ = lane == 0 ? tma::mbar_wait(&empty[last % kRing], (last / kRing) & 1) : 0;
+        __syncwarp();
+        if (!__shfl_sync(0xffffffffu, free_, 0)) break;
+      }
       const Chunks ch(q, E);
       TeamTeacher& s = teachers[b];
       if (lane == 0) {
@@ -658,7 +663,6 @@ __global__ void __launch_bounds__(kRowsThreads, 1) distill_rows_kernel(DistillAr
         if (bytes) tma::load_1d(buffers + b * words + ch.c0, x + q.v0 + ch.c0 * E, bytes, &full[i % kRing]);
         s.target_val = target_val;
         s.repeated = 0;
-        s.w = q.w;
         s.tgt = q.tgt;
       }
 #pragma unroll
@@ -675,14 +679,35 @@ __global__ void __launch_bounds__(kRowsThreads, 1) distill_rows_kernel(DistillAr
       __syncwarp();
       if (lane == 0) tma::mbar_arrive(&full[i % kRing]);
     }
+    if (lane == 0) {  // its last rows, one for each barrier it uses: no older copy can be in flight
+      for (int u = 1; u <= kRing / kTeams; ++u)
+        if (i - u * kTeams >= 0) tma::mbar_land(&full[(i - u * kTeams) % kRing], ((i - u * kTeams) / kRing) & 1);
+    }
     return;
   }
 
   const int team = (int)threadIdx.x / kTeam;
   const int tid = (int)threadIdx.x % kTeam, warp = tid >> 5;
   auto team_sync = [&]() { asm volatile("bar.sync %0, %1;" ::"r"(team + 1), "n"(kTeam) : "memory"); };
+  // a barrier of the team: whether `ok` holds for all of it
+  auto team_all = [&](bool ok) {
+    uint32_t all;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.u32 p, %1, 0;\n\t"
+        "bar.red.and.pred q, %2, %3, p;\n\t"
+        "selp.u32 %0, 1, 0, q;\n\t}"
+        : "=r"(all)
+        : "r"((uint32_t)ok), "r"(team + 1), "n"(kTeam)
+        : "memory");
+    return all != 0;
+  };
+  // weights come from memory, a row ahead: whether a row counts is the same for all of the team, whatever its waits saw
+  auto weight = [&](int64_t row) { return row < a.N && a.row_weight ? a.row_weight[row] : 1.f; };
   const float ct = (1.f / a.temperature) * kLog2e, c1 = kLog2e;
+  bool here = true;  // no wait of this thread has given up
   int i = team;
+  float w_next = weight(blockIdx.x + (int64_t)team * gridDim.x);
   for (int64_t row = blockIdx.x + (int64_t)team * gridDim.x; row < a.N; row += (int64_t)kTeams * gridDim.x, i += kTeams) {
     const int b = i % kBuffers;
     const T* x;
@@ -699,11 +724,9 @@ __global__ void __launch_bounds__(kRowsThreads, 1) distill_rows_kernel(DistillAr
       edge_val = to_f32(x[v0 + edge]);
       mx = edge_val == edge_val ? edge_val : -CUDART_INF_F;
     }
-    if (!tma::mbar_wait(&full[i % kRing], (i / kRing) & 1)) return give_up(i);
-    q.w = s.w;
-    q.tgt = s.tgt;
-    q.hard = q.tgt >= 0 && q.tgt < q.V;
-    if (edge >= 0) buf[edge] = from_f32<T>(edge_val);
+    q.w = w_next;
+    w_next = weight(row + (int64_t)kTeams * gridDim.x);
+    here = here && tma::mbar_wait(&full[i % kRing], (i / kRing) & 1);
     if (q.w == 0.f) {
       if (tid == 0) a.loss[row] = 0.f;
       for (int c = ch.c0 + tid; c < ch.c1; c += kTeam) {
@@ -714,14 +737,19 @@ __global__ void __launch_bounds__(kRowsThreads, 1) distill_rows_kernel(DistillAr
         }
       }
       if (edge >= 0) g[v0 + edge] = from_f32<T>(0.f);
-      tma::fence_proxy_async();
-      tma::mbar_arrive(&empty[i % kRing]);
+      if (here) {
+        tma::fence_proxy_async();
+        tma::mbar_arrive(&empty[i % kRing]);
+      }
       continue;
     }
+    if (here && edge >= 0) buf[edge] = from_f32<T>(edge_val);
     for (int c = ch.c0 + tid; c < ch.c1; c += kTeam) mx = fmaxf(mx, chunk_max<T>(buf4[c]));
     mx = warp_max(mx);
     if (lane == 0) red[team][0][warp] = mx;
-    team_sync();
+    if (!team_all(here)) return;
+    q.tgt = s.tgt;
+    q.hard = q.tgt >= 0 && q.tgt < q.V;
     // the listed tokens leave the sums, as in the kernel of a block per row
     Tag* tag = reinterpret_cast<Tag*>(buf);
     const int mine = tid < k && s.id[tid] >= 0 ? s.id[tid] - v0 : -1;  // k <= kTeamTeacher < kTeam

@@ -58,6 +58,17 @@ static __device__ __noinline__ bool mbar_wait(uint64_t* bar, uint32_t parity) {
     }
   }
 }
+// Waits until a copy of the block's own has landed, before its shared memory is given up: for the default limit, whatever
+// set_wait_limit has set.
+static __device__ __noinline__ void mbar_land(uint64_t* bar, uint32_t parity) {
+  const uint64_t t0 = global_ns();
+  while (!mbar_try_wait(bar, parity)) {
+    if (global_ns() - t0 > kDefaultWaitLimitNs) {
+      atomicExch(&g_wait_timeout, 1);
+      return;
+    }
+  }
+}
 
 // Orders this thread's earlier generic-proxy accesses of shared memory before its later async-proxy (TMA) ones.
 __device__ __forceinline__ void fence_proxy_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
