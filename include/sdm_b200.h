@@ -58,8 +58,8 @@ sdm_status sdm_profile_begin(void);
 int sdm_profile_end(void);
 sdm_status sdm_profile_group(int i, char* kernel, char* tag, int name_len, int* launches, double* total_ms);
 /* Synchronises `stream`, then reports SDM_ERR_TIMEOUT if any bounded device-side wait (the tensor-core GEMM's
- * mbarrier waits, the scan's chunk-copy waits and the distillation's row waits give up after about 4 s) gave up since the previous call, and
- * clears the flags. */
+ * mbarrier waits, the scan's chunk-copy waits and the distillation's row waits give up after about 4 s) gave up since
+ * the previous call, and clears the flags. */
 sdm_status sdm_device_status(void* stream);
 /* Failure-handling checks (no counterpart in the reference, which has no device-side waits).
  * sdm_set_wait_limit_ns sets, on the current device, how long every bounded device-side wait polls before it gives
@@ -303,7 +303,8 @@ sdm_status sdm_logits_choose(const sdm_logit_rules* rules, const sdm_choice_para
  *   loss = row_weight (alpha soft + (1 - alpha) hard)    (row_weight (N) float32 or NULL = 1)
  * loss (N) float32.  dlogits (N, V) in dtype, row stride ld_grad, or NULL: grad_scale * d loss / d logits, rounded
  * once; may be logits itself (same stride), and may not overlap it otherwise.  A row whose weight is 0 is not read:
- * its loss and gradient are 0.  An id listed twice counts twice in p and once in q.  1 <= k <= 512, V <= 2^18. */
+ * its loss and gradient are 0.  An id listed twice counts twice in p and once in q.  1 <= k <= 512, V <= 2^18.  Should
+ * a wait of the kernel give up (sdm_device_status), the rows that it did not finish have a NaN loss. */
 sdm_status sdm_distill(const void* logits, int64_t ld, int64_t N, int V, int dtype, const int32_t* teacher_ids,
                        const float* teacher_logits, int k, const float* teacher_lse, const int32_t* targets,
                        const float* row_weight, float temperature, float alpha, float grad_scale, float* loss,

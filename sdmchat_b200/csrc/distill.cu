@@ -747,7 +747,10 @@ __global__ void __launch_bounds__(kRowsThreads, 1) distill_rows_kernel(DistillAr
     for (int c = ch.c0 + tid; c < ch.c1; c += kTeam) mx = fmaxf(mx, chunk_max<T>(buf4[c]));
     mx = warp_max(mx);
     if (lane == 0) red[team][0][warp] = mx;
-    if (!team_all(here)) return;
+    if (!team_all(here)) {  // the rows that are left: no loss that could be taken for one
+      for (; tid == 0 && row < a.N; row += (int64_t)kTeams * gridDim.x) a.loss[row] = CUDART_NAN_F;
+      return;
+    }
     q.tgt = s.tgt;
     q.hard = q.tgt >= 0 && q.tgt < q.V;
     // the listed tokens leave the sums, as in the kernel of a block per row

@@ -3,7 +3,8 @@ distillation loss and the token table's lookup with their gradients (training).
 
 Tensors are on a CUDA device, in float32 or bfloat16 (ids int32; other integer types are converted); every call runs
 on the current stream of its tensors' device.  `distill_loss` and `embed_tokens` record autograd; the other functions
-are forward only.  There is no CPU or PyTorch fallback.
+are forward only.  There is no CPU or PyTorch fallback.  Distillation's device-side waits are bounded: rows left over
+by one that gave up have a NaN loss, and sdm_device_status reports it.
 """
 import contextlib
 import dataclasses

@@ -1,6 +1,6 @@
 """The persistent distillation kernel under a wait limit of a nanosecond: waits that do not find their row or buffer at
-once give up.  The kernel has to end, sdm_device_status to tell whether a wait gave up, and the next call under the
-default limit to be right."""
+once give up.  The kernel has to end, sdm_device_status to tell whether a wait gave up, rows that were not finished to
+have a NaN loss, and the next call under the default limit to be right."""
 import pytest
 import torch
 
@@ -33,7 +33,9 @@ def test_waits_that_give_up(cuda_ok, dt, V, tail):
     finally:
         _lib.check(lib.sdm_set_wait_limit_ns(0), "sdm_set_wait_limit_ns")
     assert status in (SDM_OK, SDM_ERR_TIMEOUT) and lib.sdm_device_status(st) == SDM_OK
-    if status == SDM_OK:
-        assert torch.equal(loss, want) and torch.equal(grad, dwant)
+    done = ~torch.isnan(loss)
+    assert torch.equal(loss[done], want[done]) and torch.equal(grad[done], dwant[done])
+    assert done.all() or status == SDM_ERR_TIMEOUT
+    print(int(done.sum()), "of", N, "rows finished, status", status)
     loss, grad = S.distill_loss_and_grad(x, ids, tl, tg, 2.0, 0.5, w, lse)
     assert torch.equal(loss, want) and torch.equal(grad, dwant) and lib.sdm_device_status(st) == SDM_OK
