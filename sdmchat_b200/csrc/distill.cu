@@ -364,13 +364,7 @@ __global__ void __launch_bounds__(NT, (kTail ? kGradThreads<T, X> : 768) / NT) d
   const Chunks ch(q, E);
   const int edge = ch.edge(tid);  // at most one token of the ragged chunks per thread
 
-  // the row into shared memory, all of it on its way at once
-  for (int c = ch.c0 + tid; c < ch.c1; c += NT)
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(buf4 + c)),
-                 "l"(x + v0 + c * E)
-                 : "memory");
   if (q.w == 0.f) {
-    asm volatile("cp.async.wait_all;" ::: "memory");
     if (q.rank == 0 && tid == 0) a.loss[q.row] = 0.f;
     const uint4 zero = make_uint4(0, 0, 0, 0);
     for (int c = ch.c0 + tid; c < ch.c1; c += NT) {
@@ -384,6 +378,11 @@ __global__ void __launch_bounds__(NT, (kTail ? kGradThreads<T, X> : 768) / NT) d
     return;
   }
 
+  // the row into shared memory, all of it on its way at once
+  for (int c = ch.c0 + tid; c < ch.c1; c += NT)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(buf4 + c)),
+                 "l"(x + v0 + c * E)
+                 : "memory");
   load_teacher<NT>(a, q, x, s);
   float mx = -CUDART_INF_F;
   if (edge >= 0) {
@@ -640,7 +639,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) distill_rows_kernel(DistillAr
 #pragma unroll
       for (int u = 0; u < kTeamTeacher / 32; ++u) {
         const int j = lane + 32 * u;
-        id[u] = j < k ? a.t_ids[row * k + j] : -1;
+        id[u] = j < k && q.w != 0.f ? a.t_ids[row * k + j] : -1;
         t[u] = j < k ? a.t_logits[row * k + j] : 0.f;
       }
 #pragma unroll
@@ -648,7 +647,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) distill_rows_kernel(DistillAr
         if (id[u] < 0 || id[u] >= q.V || t[u] == -CUDART_INF_F) id[u] = -1;
         val[u] = id[u] >= 0 ? to_f32(x[id[u]]) : 0.f;
       }
-      const float target_val = q.hard ? to_f32(x[q.tgt]) : 0.f;
+      const float target_val = q.hard && q.w != 0.f ? to_f32(x[q.tgt]) : 0.f;
       const int last = i - kBuffers;  // the row that had the buffer
       if (last >= 0) {
         const int free_ = lane == 0 ? tma::mbar_wait(&empty[last % kRing], (last / kRing) & 1) : 0;
@@ -658,7 +657,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) distill_rows_kernel(DistillAr
       const Chunks ch(q, E);
       TeamTeacher& s = teachers[b];
       if (lane == 0) {
-        const uint32_t bytes = (uint32_t)(ch.c1 - ch.c0) * 16;
+        const uint32_t bytes = q.w != 0.f ? (uint32_t)(ch.c1 - ch.c0) * 16 : 0;
         tma::mbar_arrive_expect_tx(&full[i % kRing], bytes);
         if (bytes) tma::load_1d(buffers + b * words + ch.c0, x + q.v0 + ch.c0 * E, bytes, &full[i % kRing]);
         s.target_val = target_val;
@@ -720,11 +719,11 @@ __global__ void __launch_bounds__(kRowsThreads, 1) distill_rows_kernel(DistillAr
     T* buf = reinterpret_cast<T*>(buf4);
     TeamTeacher& s = teachers[b];
     float mx = -CUDART_INF_F, edge_val = 0.f;
-    if (edge >= 0) {
+    q.w = w_next;
+    if (edge >= 0 && q.w != 0.f) {
       edge_val = to_f32(x[v0 + edge]);
       mx = edge_val == edge_val ? edge_val : -CUDART_INF_F;
     }
-    q.w = w_next;
     w_next = weight(row + (int64_t)kTeams * gridDim.x);
     here = here && tma::mbar_wait(&full[i % kRing], (i / kRing) & 1);
     if (q.w == 0.f) {

@@ -187,3 +187,30 @@ def test_listed_tokens_lead(cuda_ok, dt, N, V, T):
     only = S.distill_loss(y, ids, tl, None, T, 0.6, None, lse, reduction="none")
     assert torch.isposinf(loss).all() and torch.isposinf(only).all()
     assert torch.isfinite(grad).all() and (grad[~listed] == 0).all()
+
+
+@pytest.mark.parametrize("dt,V,T", [(BF16, 32768, 2.0), (BF16, 20000, 2.0), (F32, 8192, 1.5)])
+def test_rows_without_weight_are_not_read(cuda_ok, dt, V, T):
+    """Of rows without weight only the gradient's zeros move: half the bytes of a copy of the logits, which takes the
+    memory 8,192 rows of 40 KB and more long enough to be measured."""
+    N = 8192 * 32768 // V
+    x = torch.zeros(N, V, device=DEV, dtype=dt)
+    ids, tl = torch.zeros(N, 4, device=DEV, dtype=torch.int32), torch.zeros(N, 4, device=DEV)
+    w, out = torch.zeros(N, device=DEV), torch.ones_like(x)
+
+    def best(f):
+        t = []
+        for _ in range(8):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            f()
+            b.record()
+            b.synchronize()
+            t.append(a.elapsed_time(b))
+        return min(t)
+
+    tg = torch.zeros(N, device=DEV, dtype=torch.int32)
+    mine = best(lambda: S.distill_loss_and_grad(x, ids, tl, tg, T, 0.5, w, out=out))
+    assert torch.count_nonzero(out) == 0
+    copy = best(lambda: out.copy_(x))
+    assert mine < 0.85 * copy, (mine, copy)
