@@ -277,7 +277,8 @@ sdm_status sdm_logits_process(const sdm_logit_rules* rules, const void* logits, 
  * below max(1, ceil(top_p * kept mass)) (top_p >= 1: all); the token is the first one in index order whose running
  * kept mass exceeds min(floor(u * K), K - 1), K the kept mass.  ids (S) int32, logprob (S) float32 or NULL:
  * t - log(K / 2^40), the log-probability under the distribution drawn from.  T = 0 takes the largest y (lowest index)
- * with its logprob at T = 1 over all tokens; a negative or NaN T is taken as 0.  A row with no y above -infinity gets id -1 and logprob -infinity.
+ * with its logprob at T = 1 over all tokens; a negative or NaN T is taken as 0, an infinite one as the largest number
+ * (all allowed tokens alike).  A row with no y above -infinity gets id -1 and logprob -infinity.
  * temperature, top_p, u (S) float32 and top_k (S) int32, per row where the pointer is given, else the value beside
  * it; u (in [0, 1)) may be NULL only where temperature is NULL and temperature_all is 0.  V at most 2^18. */
 typedef struct {

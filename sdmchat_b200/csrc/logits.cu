@@ -3,6 +3,7 @@
 // Both kernels split a row over blocks, each block owning a slice of the vocabulary.  A block marks, in one shared
 // word per token of its slice, what the row's history and biases say about the token; then it reads its logits once,
 // 16 bytes per thread, and applies the rules where a word is set.
+#include <float.h>
 #include <math_constants.h>
 #include "vocab.cuh"
 
@@ -691,7 +692,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) choose_kernel(sdm_logit_rules r
   const RowRules q = row_rules(r, row, V);
   const float T0 = c.temperature ? c.temperature[row] : c.temperature_all;
   const bool greedy = !(T0 > 0.f);
-  const float Tr = greedy ? 1.f : T0;
+  const float Tr = greedy ? 1.f : fminf(T0, FLT_MAX);  // infinite: level; a gap of infinity over it would be NaN
   const int top_k = c.top_k ? c.top_k[row] : c.top_k_all;
   const float top_p = c.top_p ? c.top_p[row] : c.top_p_all;
   const float u = c.u ? c.u[row] : 0.f;

@@ -1,0 +1,31 @@
+"""Arguments at the ends of their ranges: the vocabulary-end operators on the GPU against plain computations."""
+import math
+
+import pytest
+import torch
+
+import sdmchat_b200 as S
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+@pytest.mark.parametrize("V", [50, 3000, 40000])
+@pytest.mark.parametrize("rows", [2, 200])
+@pytest.mark.parametrize("T", [3e38, math.inf])
+def test_temperature_without_end(cuda_ok, V, rows, T):
+    """All tokens that are not at -infinity are alike: u picks among the kept ones by their number."""
+    g = torch.Generator(device=DEV).manual_seed(V)
+    x = torch.randn(rows, V, generator=g, device=DEV)
+    x[:, ::3] = -math.inf
+    u = torch.rand(rows, generator=g, device=DEV)
+    n = V - len(range(0, V, 3))
+    for kw in ({}, dict(top_k=5), dict(top_k=n // 2), dict(top_p=0.5), dict(top_k=20, top_p=0.375)):
+        k = kw.get("top_k", n)
+        m = math.ceil(k * kw.get("top_p", 1.0))
+        for temperature in (T, torch.full((rows,), T, device=DEV)):
+            ids, lp = S.sample_logits(x, u=u, temperature=temperature, **kw)
+            assert torch.allclose(lp, torch.full_like(lp, -math.log(m)), atol=16 * 2.0 ** -24 * (1 + math.log(m)))
+            keep = torch.sort(x, dim=1, descending=True, stable=True).indices[:, :m].sort(1).values
+            at = (u.double() * m).long().clamp(max=m - 1)
+            assert torch.equal(ids.long(), keep.gather(1, at[:, None])[:, 0])
