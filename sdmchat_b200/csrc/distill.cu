@@ -1158,10 +1158,10 @@ cudaError_t distill_x(const DistillArgs& a, cudaStream_t st) {
   // per row, of 26,000 348 and 375, but of 24,000 367 and 308; and with two exponentials of 32,768 552 and 529.
   const size_t row_bytes = (size_t)slice * sizeof(T);
   if constexpr (X != kTwo) {
-    if (a.dlogits && C == 1 && a.k <= kTeamTeacher && a.N >= 4 * kSMs && row_bytes > 50 * 1024 &&
-        kBuffers * row_bytes <= 200 * 1024) {
+    constexpr int kMost = 200 * 1024;
+    if (a.dlogits && C == 1 && a.k <= kTeamTeacher && a.N >= 4 * kSMs && row_bytes > 50 * 1024 && kBuffers * row_bytes <= kMost) {
       auto kern = a.t_lse ? distill_rows_kernel<T, X, true> : distill_rows_kernel<T, X, false>;
-      cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(kBuffers * row_bytes));
+      cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost);
       if (e != cudaSuccess) return e;
       LaunchScope scope_("distill_rows", st);
       return launch_k(kern, dim3(kSMs), dim3(kRowsThreads), kBuffers * row_bytes, st, a, slice);

@@ -59,13 +59,18 @@ inline cudaError_t launch_next(void (*kern)(KArgs...), unsigned grid, int block,
   return cudaLaunchKernelEx(&cfg, kern, static_cast<Args&&>(args)...);
 }
 
+// A kernel's limit of dynamic shared memory belongs to the function, not to a launch: it is set to the same number by every
+// call, so that host threads which launch one kernel at several sizes do not lower it under one another.
+constexpr size_t kMaxDynamicSmem = 160 * 1024;
+
 // A cluster launch of kern (blocks of one row share a cluster).  Programmatic dependent launch as in launch_k.  A cluster
 // of one block is launched as a plain block: with the attribute, blocks start at 1.2 per us and SM (distillation of
 // 131,072 rows of 2,048: 685 us with it, 445 without).
 template <typename... KArgs, typename... Args>
 inline cudaError_t launch_clusters(void (*kern)(KArgs...), unsigned grid, int cluster, int block, size_t smem,
                                    cudaStream_t st, Args&&... args) {
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (smem > kMaxDynamicSmem) return cudaErrorInvalidValue;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMaxDynamicSmem);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(grid);

@@ -29,3 +29,32 @@ def test_temperature_without_end(cuda_ok, V, rows, T):
             keep = torch.sort(x, dim=1, descending=True, stable=True).indices[:, :m].sort(1).values
             at = (u.double() * m).long().clamp(max=m - 1)
             assert torch.equal(ids.long(), keep.gather(1, at[:, None])[:, 0])
+
+
+def test_host_threads_at_different_sizes(cuda_ok):
+    """Two host threads launch the same kernel on streams of their own, one over a vocabulary that takes little shared
+    memory and one over one that takes much: no launch may be refused.  The calls are made at the C entry point, so
+    that the threads meet in it."""
+    import threading
+
+    from sdmchat_b200 import _lib
+    lib = _lib.lib()
+    greedy = _lib.ChoiceParams(top_p_all=1.0)
+
+    def work(V, seed, results):
+        x = torch.randn(1, V, generator=torch.Generator(device=DEV).manual_seed(seed), device=DEV)
+        ids = torch.full((1,), -7, device=DEV, dtype=torch.int32)
+        torch.cuda.synchronize()
+        st = torch.cuda.Stream()
+        args = (None, greedy, _lib.ptr(x), V, 1, V, 0, _lib.ptr(ids), None, _lib.c_void_p(st.cuda_stream))
+        refused = sum(lib.sdm_logits_choose(*args) != 0 for _ in range(20000))
+        st.synchronize()
+        results.append((refused, int(ids.item()) == int(x.argmax())))
+
+    results = []
+    threads = [threading.Thread(target=work, args=(V, V, results)) for V in (70000, 200000)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert results == [(0, True), (0, True)], results
