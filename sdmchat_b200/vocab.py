@@ -1,10 +1,11 @@
 """The vocabulary end of a language model on libsdm_b200: rules on logits and the choice of a token (serving), the
 distillation loss and the token table's lookup with their gradients (training).
 
-Tensors are on a CUDA device, in float32 or bfloat16 (ids int32; other integer types are converted); every call runs
-on the current stream of its tensors' device.  `distill_loss` and `embed_tokens` record autograd; the other functions
-are forward only.  There is no CPU or PyTorch fallback.  Distillation's device-side waits are bounded: rows left over
-by one that gave up have a NaN loss, and sdm_device_status reports it.
+Tensors are on a CUDA device, in float32 or bfloat16 (ids int32; other integer types are converted, numbers that int32
+does not hold to ones outside every table); every call runs on the current stream of its tensors' device.
+`distill_loss` and `embed_tokens` record autograd; the other functions are forward only.  There is no CPU or PyTorch
+fallback.  Distillation's device-side waits are bounded: rows left over by one that gave up have a NaN loss, and
+sdm_device_status reports it.
 """
 import contextlib
 import dataclasses
@@ -18,6 +19,8 @@ from ._lib import check, lib, workspace, dtype_code
 
 Per = Union[float, torch.Tensor]  # one value for all rows, or one per row
 I32, F32 = torch.int32, torch.float32
+I32_MAX = 2 ** 31 - 1
+_WIDE = (torch.int64, torch.uint32, torch.uint64)  # integer types with numbers that int32 does not hold
 _NOTHING = contextlib.nullcontext()
 # sdm_logit_rules and sdm_choice_params as C lays them out (a call at one stream is bound by the host: packing a struct
 # this way takes a fifth of setting its fields one by one)
@@ -42,9 +45,18 @@ def _guard(ix):
     return _NOTHING if torch.cuda.current_device() == ix else torch.cuda.device(ix)
 
 
-def _at(t, ix, name, dtype, shape, keep):
+def _narrow(t):
+    """Whole numbers t as contiguous int32.  What int32 does not hold becomes -1 or 2^31 - 1, so that an id outside a
+    table stays outside."""
+    t = t.detach()
+    if t.dtype in _WIDE:
+        t = t.to(torch.int64).clamp(-1, I32_MAX)
+    return t.to(I32).contiguous()
+
+
+def _at(t, ix, name, dtype, shape, keep, bits=False):
     """Pointer of t (None: 0) as a contiguous tensor of dtype on device ix with the given shape (None: any size).  A
-    converted copy goes into `keep`, which lives until the launch."""
+    converted copy goes into `keep`, which lives until the launch.  bits: int32 words whose bits count."""
     if t is None:
         return 0
     if t.dtype is dtype and t.get_device() == ix and t.shape == shape and t.is_contiguous():
@@ -55,7 +67,7 @@ def _at(t, ix, name, dtype, shape, keep):
         raise ValueError(f"{name} has shape {tuple(t.shape)}, wanted {tuple('any' if w is None else w for w in shape)}")
     if dtype is I32 and (t.dtype.is_floating_point or t.dtype.is_complex):
         raise TypeError(f"{name} holds whole numbers, not {t.dtype}")
-    t = t.detach().to(dtype).contiguous()
+    t = _narrow(t) if dtype is I32 and not bits else t.detach().to(dtype).contiguous()
     keep.append(t)
     return t.data_ptr()
 
@@ -72,6 +84,8 @@ def _rows(t, name):
     if t.dim() != 2:
         raise ValueError(f"{name} is 2-D (rows, vocabulary), not {t.dim()}-D")
     N, V = t.shape
+    if V > I32_MAX:
+        raise ValueError(f"{name}: {V} tokens are more than the library counts")
     if t.is_contiguous():
         return t, V
     if V > 1 and t.stride(1) != 1 or N > 1 and t.stride(0) < V:
@@ -140,7 +154,7 @@ class LogitRules:
         mrp = _at(self.mask_row, ix, "mask_row", I32, (S,), keep)
         if mask is not None:
             G = mask.shape[0]
-            mp = _at(mask, ix, "mask", I32, (G, -(-V // 32)), keep)
+            mp = _at(mask, ix, "mask", I32, (G, -(-V // 32)), keep, bits=True)
             if not mrp and G != 1 and G != S:
                 raise ValueError(f"{G} masks for {S} rows need mask_row")
         elif mrp:
@@ -306,7 +320,7 @@ def _ids32(ids):
         return ids
     if ids.dtype.is_floating_point or ids.dtype.is_complex or ids.dtype is torch.bool:
         raise TypeError(f"ids are whole numbers, not {ids.dtype}")
-    return ids.detach().to(I32).contiguous()
+    return _narrow(ids)
 
 
 def embed_grad(ids, dout, num_rows, scale=1.0, padding_id=None, dtype=torch.float32, out=None):
@@ -331,18 +345,22 @@ def embed_grad(ids, dout, num_rows, scale=1.0, padding_id=None, dtype=torch.floa
         if out.shape != (num_rows, d) or not out.is_contiguous() or out.get_device() != ix:
             raise ValueError(f"out is a contiguous ({num_rows}, {d}) tensor on {ids.device}")
         grad = out
+    if not 0 < num_rows <= I32_MAX or d > I32_MAX:
+        raise ValueError(f"a table of {num_rows} x {d} is more than the library counts")
+    skip = padding_id if padding_id is not None and 0 <= padding_id < num_rows else -1
     nbytes = lib().sdm_embed_grad_workspace_size(N, d, num_rows)
     ws = workspace(nbytes, i32.device)
     with _guard(ix):
         check(lib().sdm_embed_grad(i32.data_ptr(), dout.data_ptr(), ld, N, d, num_rows, scale,
-                                   -1 if padding_id is None else padding_id, dtype_code(dout.dtype),
-                                   dtype_code(grad.dtype), int(out is not None), grad.data_ptr(), ws.data_ptr(),
-                                   nbytes, _stream(ix)), "sdm_embed_grad")
+                                   skip, dtype_code(dout.dtype), dtype_code(grad.dtype), int(out is not None),
+                                   grad.data_ptr(), ws.data_ptr(), nbytes, _stream(ix)), "sdm_embed_grad")
     return grad
 
 
 def _embed(i32, table, scale, bad):
     V, d = table.shape
+    if max(V, d) > I32_MAX:
+        raise ValueError(f"a table of {V} x {d} is more than the library counts")
     ix = i32.get_device()
     out = torch.empty(*i32.shape, d, dtype=table.dtype, device=table.device)
     with _guard(ix):

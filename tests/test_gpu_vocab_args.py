@@ -58,3 +58,26 @@ def test_host_threads_at_different_sizes(cuda_ok):
     for t in threads:
         t.join()
     assert results == [(0, True), (0, True)], results
+
+
+def test_ids_beyond_32_bits(cuda_ok):
+    """Ids that a 64-bit tensor holds and 32 bits do not are outside every table."""
+    far = [2 ** 32 + 5, -2 ** 32 + 5, 2 ** 31 + 5]
+    ids = torch.tensor(far + [3], device=DEV)
+    table = torch.randn(10, 4, device=DEV)
+    bad = torch.zeros(1, device=DEV, dtype=torch.int32)
+    out = S.embed_tokens(ids, table, bad=bad)
+    assert bad.item() == 1 and (out[:3] == 0).all() and torch.equal(out[3], table[3])
+    grad = S.embed_grad(ids, torch.ones(4, 4, device=DEV), 10)
+    assert grad.sum() == 4 and (grad[3] == 1).all()
+    for skip in (2 ** 32 + 3, -2 ** 32 + 3, 10, -1):  # no token of the table: nothing is skipped
+        assert torch.equal(S.embed_grad(ids, torch.ones(4, 4, device=DEV), 10, padding_id=skip), grad)
+    x = torch.randn(1, 10, device=DEV)
+    far = torch.tensor([far], device=DEV)
+    assert torch.equal(S.process_logits(x, S.LogitRules(history=far, presence=1.0)), x)
+    assert torch.equal(S.process_logits(x, S.LogitRules(bias_ids=far, bias_values=torch.ones(1, 3, device=DEV))), x)
+    tl = torch.zeros(1, 3, device=DEV)
+    loss, dx = S.distill_loss_and_grad(x, far, tl, targets=far[:, 0], alpha=0.5)
+    assert loss.item() == 0 and (dx == 0).all()
+    ids, _ = S.sample_logits(x, u=torch.tensor([0.999], device=DEV), top_k=torch.tensor([2 ** 32 + 1], device=DEV))
+    assert ids.item() == S.sample_logits(x, u=torch.tensor([0.999], device=DEV))[0].item()
