@@ -337,6 +337,9 @@ class OneSdmLM(nn.Module):
         [0, 1) that pick the tokens, by default torch.rand's.  A stream whose rules allow no token gets -1 from there
         on.  return_logprobs: also the tokens' log-probabilities (S, steps) under the distribution drawn from."""
         sampled = rules is not None or u is not None or torch.is_tensor(temperature) or temperature != 0
+        if u is not None and tuple(u.shape) != (prompt.shape[0], steps):
+            raise ValueError(f"u has shape {tuple(u.shape)}, wanted one number per stream and step: "
+                             f"{(prompt.shape[0], steps)}")
         state = self.init_decode(prompt.shape[0], prompt.device)
         if sampled or return_logprobs:
             return self._generate_sampled(prompt, steps, use_graph, rules or LogitRules(), u, temperature, top_k, top_p,

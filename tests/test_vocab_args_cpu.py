@@ -33,3 +33,12 @@ def test_widths_beyond_32_bits_are_refused():
     wide = torch.zeros(1, 1).expand(1, 2 ** 32 + 8)  # one number in memory
     with pytest.raises(ValueError):
         W._rows(wide, "logits")
+
+
+def test_generate_wants_a_number_per_step():
+    """Steps take their numbers from u by index on the device, where an index beyond it could not be refused."""
+    m = S.build_onesdm("onesdm_allsdm", 64, dict(d=64, layers=1, mlp_f=176, heads=4, n_sub=8, d_a=8, k=4, chunk=16))
+    prompt = torch.zeros(3, 5, dtype=torch.long)
+    for shape in ((3, 7), (3, 9), (2, 8), (8,), (3, 8, 1)):
+        with torch.no_grad(), pytest.raises(ValueError, match="one number per stream and step"):
+            m.generate(prompt, 8, u=torch.rand(shape), temperature=1.0)
