@@ -322,7 +322,7 @@ sdm_status sdm_scale_rows(void* x, int64_t ld, int64_t N, int V, int dtype, cons
  * accumulate is 1), dout (N, d) in dtype with row stride ld, grad in grad_dtype; ids outside [0, V) and padding_id
  * (-1: none) are skipped.  Positions are grouped by id, and each sum runs over them in order (long ones in fixed
  * pieces joined in order) in float32, so the result does not depend on timing.  N at most 2^30, d
- * at most 2^20, V at most 2^24. */
+ * at most 2^20 (of the lookup 2^30), V at most 2^24 (of the lookup any). */
 sdm_status sdm_embed_scaled(const int32_t* ids, const void* emb, int64_t N, int d, int V, float scale, int dtype,
                             void* out, int* bad, void* stream);
 size_t sdm_embed_grad_workspace_size(int64_t N, int d, int V);

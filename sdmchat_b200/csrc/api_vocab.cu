@@ -91,7 +91,7 @@ sdm_status sdm_scale_rows(void* x, int64_t ld, int64_t N, int V, int dtype, cons
 sdm_status sdm_embed_scaled(const int32_t* ids, const void* emb, int64_t N, int d, int V, float scale, int dtype,
                             void* out, int* bad, void* stream) {
   if (!emb || (N != 0 && (!ids || !out)) || !dtype_ok(dtype) || !aligned(emb, dtype) || !aligned(out, dtype)) return SDM_ERR_ARG;
-  if (N < 0 || N > (1 << 30) || d < 1 || V < 1) return SDM_ERR_SHAPE;
+  if (N < 0 || N > (1 << 30) || d < 1 || d > (1 << 30) || V < 1) return SDM_ERR_SHAPE;  // columns are counted in an int
   return to_status(launch_embed_scaled(ids, emb, N, d, V, scale, dtype, out, bad, S(stream)));
 }
 

@@ -42,3 +42,12 @@ def test_generate_wants_a_number_per_step():
     for shape in ((3, 7), (3, 9), (2, 8), (8,), (3, 8, 1)):
         with torch.no_grad(), pytest.raises(ValueError, match="one number per stream and step"):
             m.generate(prompt, 8, u=torch.rand(shape), temperature=1.0)
+
+
+def test_lookup_refuses_rows_whose_columns_an_int_does_not_count():
+    import ctypes
+
+    from sdmchat_b200 import _lib
+    fake = ctypes.c_void_p(0x10000)  # never dereferenced
+    for d in (2 ** 30 + 1, 2 ** 31 - 1):
+        assert _lib.lib().sdm_embed_scaled(fake, fake, 1, d, 1, 1.0, 1, fake, None, None) == 2
