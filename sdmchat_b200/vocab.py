@@ -110,6 +110,12 @@ def _out_rows(out, like, name):
     return out.stride(0) if N > 1 else V
 
 
+def _written(t):
+    """Tells autograd that the library wrote to a tensor of the caller's: what was saved of its old values is stale."""
+    torch.autograd.graph.increment_version(t)
+    return t
+
+
 @dataclasses.dataclass
 class LogitRules:
     """What a serving loop knows about each of S rows of logits (struct sdm_logit_rules; everything is optional).
@@ -173,7 +179,8 @@ def process_logits(logits, rules=None, out=None):
     code = dtype_code(logits.dtype)
     x, ld = _rows(logits, "logits")
     S, V = x.shape
-    if out is None:
+    own = out is None
+    if own:
         out, ld_out = torch.empty(S, V, dtype=x.dtype, device=x.device), V
     else:
         ld_out = _out_rows(out, logits, "out")
@@ -182,7 +189,7 @@ def process_logits(logits, rules=None, out=None):
     with _guard(ix):
         check(lib().sdm_logits_process(r, x.data_ptr(), ld, S, V, code, out.data_ptr(), ld_out, _stream(ix)),
               "sdm_logits_process")
-    return out
+    return out if own else _written(out)
 
 
 def sample_logits(logits, rules=None, u=None, temperature: Per = 1.0, top_k: Union[int, torch.Tensor] = 0,
@@ -237,6 +244,8 @@ def _distill(logits, teacher_ids, teacher_logits, targets, temperature, alpha, r
     with _guard(ix):
         check(lib().sdm_distill(x.data_ptr(), ld, N, V, code, idp, tlp, k, lsep, tgp, wp, temperature, alpha,
                                 grad_scale, loss.data_ptr(), gp, ldg, _stream(ix)), "sdm_distill")
+    if out is not None:
+        _written(out)
     return loss, grad
 
 
@@ -354,7 +363,7 @@ def embed_grad(ids, dout, num_rows, scale=1.0, padding_id=None, dtype=torch.floa
         check(lib().sdm_embed_grad(i32.data_ptr(), dout.data_ptr(), ld, N, d, num_rows, scale,
                                    skip, dtype_code(dout.dtype), dtype_code(grad.dtype), int(out is not None),
                                    grad.data_ptr(), ws.data_ptr(), nbytes, _stream(ix)), "sdm_embed_grad")
-    return grad
+    return grad if out is None else _written(out)
 
 
 def _embed(i32, table, scale, bad):

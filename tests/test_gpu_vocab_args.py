@@ -81,3 +81,20 @@ def test_ids_beyond_32_bits(cuda_ok):
     assert loss.item() == 0 and (dx == 0).all()
     ids, _ = S.sample_logits(x, u=torch.tensor([0.999], device=DEV), top_k=torch.tensor([2 ** 32 + 1], device=DEV))
     assert ids.item() == S.sample_logits(x, u=torch.tensor([0.999], device=DEV))[0].item()
+
+
+def test_outputs_in_place_are_seen_by_autograd(cuda_ok):
+    """A tensor that a graph saved and an operator then wrote over makes the backward pass raise, as torch's own do."""
+    ids = torch.zeros(3, 2, device=DEV, dtype=torch.int32)
+    tl = torch.zeros(3, 2, device=DEV)
+    tok = torch.zeros(4, device=DEV, dtype=torch.int32)
+    for write in (lambda x: S.process_logits(x, out=x), lambda x: S.distill_loss_and_grad(x, ids, tl, out=x),
+                  lambda x: S.embed_grad(tok, torch.ones(4, 8, device=DEV), 3, out=x)):
+        leaf = torch.randn(3, 8, device=DEV, requires_grad=True)
+        x = leaf * 2
+        y = (x * x).sum()  # saves x
+        write(x.detach())
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.backward()
+        with torch.inference_mode():  # whose tensors' versions nobody reads
+            write(torch.randn(3, 8, device=DEV))
