@@ -105,7 +105,11 @@ def _out_rows(out, like, name):
         return t.data_ptr(), t.data_ptr() + ((N - 1) * t.stride(0) + (V - 1) * t.stride(1) + 1) * t.element_size()
 
     (a0, a1), (b0, b1) = span(out), span(like)
-    if a0 < b1 and b0 < a1 and (a0 != b0 or out.stride() != like.stride()) and N * V > 0:
+    apart = False  # side by side in the rows of one buffer
+    if N > 1 and out.stride() == like.stride():
+        ld, width = out.stride(0) * out.element_size(), V * out.element_size()
+        apart = width <= (a0 - b0) % ld <= ld - width
+    if a0 < b1 and b0 < a1 and not apart and (a0 != b0 or out.stride() != like.stride()) and N * V > 0:
         raise ValueError(f"{name} overlaps the logits without being them")
     return out.stride(0) if N > 1 else V
 

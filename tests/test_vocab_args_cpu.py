@@ -51,3 +51,21 @@ def test_lookup_refuses_rows_whose_columns_an_int_does_not_count():
     fake = ctypes.c_void_p(0x10000)  # never dereferenced
     for d in (2 ** 30 + 1, 2 ** 31 - 1):
         assert _lib.lib().sdm_embed_scaled(fake, fake, 1, d, 1, 1.0, 1, fake, None, None) == 2
+
+
+def test_outputs_beside_the_logits_in_one_buffer():
+    buf = torch.zeros(4, 25)
+    for a, b in ((0, 10), (10, 0), (0, 15), (15, 0), (2, 12)):
+        assert W._out_rows(buf[:, a:a + 10], buf[:, b:b + 10], "out") == 25
+    assert W._out_rows(buf[1:, :10], buf[:3, 10:20], "out") == 25
+    assert W._out_rows(buf[:, :10], buf[:, :10], "out") == 25  # the logits themselves
+    for a, b in ((0, 9), (9, 0), (1, 0)):
+        with pytest.raises(ValueError):
+            W._out_rows(buf[:, a:a + 10], buf[:, b:b + 10], "out")
+    for out, like in ((buf[1:, :10], buf[:3, :10]), (buf[:, 12:22], buf[:, 3:13]), (buf[1:, :10], buf[:3, 18:])):
+        if out.shape == like.shape:
+            with pytest.raises(ValueError):
+                W._out_rows(out, like, "out")
+    flat = torch.zeros(100)
+    with pytest.raises(ValueError):  # a row's end and the next one's beginning
+        W._out_rows(flat[5:].as_strided((4, 10), (12, 1), 5), flat.as_strided((4, 10), (12, 1), 0), "out")
