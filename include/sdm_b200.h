@@ -311,7 +311,7 @@ sdm_status sdm_distill(const void* logits, int64_t ld, int64_t N, int V, int dty
                        const float* row_weight, float temperature, float alpha, float grad_scale, float* loss,
                        void* dlogits, int64_t ld_grad, void* stream);
 /* x (N, V) *= g[row] in place (g_stride 1) or *= g[0] (g_stride 0), in dtype, row stride ld: the chain rule's factor
- * on a gradient that sdm_distill wrote.  A row whose factor is 1 is left alone, unread. */
+ * on a gradient that sdm_distill wrote (in bfloat16 rounded again).  A row whose factor is 1 is left alone, unread. */
 sdm_status sdm_scale_rows(void* x, int64_t ld, int64_t N, int V, int dtype, const float* g, int g_stride,
                           void* stream);
 

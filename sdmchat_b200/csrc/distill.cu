@@ -43,7 +43,7 @@ __device__ __forceinline__ float ex2(float t) {
 // How many exponentials a logit takes.  kOne: the one at T serves, as T = 1 or no hard target is given.  kTwo: one at T and
 // one at 1.  kSquare, kFourth: T = 2 or 4, so that the one at 1 is the other's square or fourth power (c and B are then
 // exactly half or a quarter of those at 1, and it leaves float32's range at the same logit).  16,384 rows of 32,768
-// bfloat16 logits with their gradient: 373 us, 529, 395, 421.
+// bfloat16 logits with their gradient: 378 us, 532, 392, 429.
 enum Exps { kOne, kTwo, kSquare, kFourth };
 template <Exps X>
 __device__ __forceinline__ float power(float e) {
@@ -76,8 +76,8 @@ __device__ __forceinline__ pair_t add_pair(pair_t a, pair_t b) {
 
 // 2^t on the FMA pipe, for a kernel that would wait on the exponential unit (16 a clock and SM against 128 FMAs):
 // t = n + f with n = rint(t) (Cody and Waite's reduction), a polynomial in f in [-1/2, 1/2] fitted by Remez's exchange
-// to the least relative error (1.6e-7 with its coefficients in float32, 2.2e-7 evaluated there), and n added to the exponent.
-// Below -126 it stays at 2^-126.
+// to the least relative error (1.6e-7 with its coefficients in float32, 2.2e-7 evaluated there), and n added to the
+// exponent.  Below -126 it stays at 2^-126.
 __device__ __forceinline__ pair_t exp2_pair(pair_t t) {
   float2 v = both(t);
   t = pair(fmaxf(v.x, -126.f), fmaxf(v.y, -126.f));
@@ -996,8 +996,8 @@ __global__ void __launch_bounds__(NT, 1536 / NT) distill_loss_kernel(const __gri
   }
   constexpr bool tail = kTail;
   const Chunks ch(q, E);
-  // the row is on its way to L2 while its teacher is fetched (8,192 rows of 50,021: 139 us without,
-  // 132 with; 65,536 of 8,192: 340 and 311)
+  // the row is on its way to L2 while its teacher is fetched (8,192 rows of 50,021: 150 us without,
+  // 148 with; 65,536 of 8,192: 204 and 192)
   if (tid == 0 && ch.c1 > ch.c0)
     asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(x + v0 + ch.c0 * E), "r"((ch.c1 - ch.c0) * 16)
                  : "memory");
@@ -1155,12 +1155,14 @@ cudaError_t distill_x(const DistillArgs& a, cudaStream_t st) {
   if (a.N * C > 0x7fffffff) return cudaErrorInvalidValue;
   const int slice = slice_of(C);
   // Rows of which three fit a block's shared memory, but of which the SM does not hold four for the other kernel, enough
-  // of them that every SM gets several.  16,384 rows of 32,768 bfloat16 take 395 us on persistent blocks and 414 on a block
-  // per row, of 26,000 348 and 375, but of 24,000 367 and 308; and with two exponentials of 32,768 552 and 529.
+  // of them that every SM gets several.  16,384 rows of 32,768 bfloat16 take 392 us on persistent blocks and 417 on a block
+  // per row, of 26,000 347 and 376, but of 24,000 363 and 309.  (With two exponentials a logit persistent blocks took 552 us
+  // at 32,768 when a block per row took 529.)
   const size_t row_bytes = (size_t)slice * sizeof(T);
   if constexpr (X != kTwo) {
     constexpr int kMost = 200 * 1024;
-    if (a.dlogits && C == 1 && a.k <= kTeamTeacher && a.N >= 4 * kSMs && row_bytes > 50 * 1024 && kBuffers * row_bytes <= kMost) {
+    if (a.dlogits && C == 1 && a.k <= kTeamTeacher && a.N >= 4 * kSMs && row_bytes > 50 * 1024 &&
+        kBuffers * row_bytes <= kMost) {
       auto kern = a.t_lse ? distill_rows_kernel<T, X, true> : distill_rows_kernel<T, X, false>;
       cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost);
       if (e != cudaSuccess) return e;
@@ -1169,10 +1171,10 @@ cudaError_t distill_x(const DistillArgs& a, cudaStream_t st) {
     }
   }
   // few threads where rows are short, so that many blocks hide one another's reductions.  131,072 rows of 2,048 bfloat16
-  // logits with their gradient take 420 us with 32 threads and 446 with 64 (of 1,000 334 and 424), 65,536 of 4,096 331 and
-  // 297; the loss alone of 65,536 rows of 8,192 209 with 64 and 261 with 128, of 32,768 rows of 16,384 222 and 191, of
-  // 16,384 rows of 32,768 204 with 128 and 185 with 256.  A cluster's blocks keep 64: 48 rows of 1,000 float32 logits take
-  // 6.9 us, and 7.6 with 32.
+  // logits with their gradient take 423 us with 32 threads and 449 with 64 (of 1,000 325 and 413), 65,536 of 4,096 337 and
+  // 309; the loss alone (T = 2, hard targets) of 65,536 rows of 8,192 193 with 64 and 240 with 128, of 32,768 rows of
+  // 16,384 218 and 178, of 16,384 rows of 32,768 199 with 128 and 177 with 256.  A cluster's blocks keep 64: 48 rows of
+  // 1,000 float32 logits take 6.8 us, and 7.7 with 32.
   if (C == 1 && row_bytes <= 6 * 1024) return distill_n<T, X, 32>(a, C, slice, st);
   if (row_bytes <= 16896) return distill_n<T, X, 64>(a, C, slice, st);
   if (row_bytes <= 33024) return distill_n<T, X, 128>(a, C, slice, st);

@@ -299,8 +299,9 @@ def distill_loss(logits, teacher_ids, teacher_logits, targets=None, temperature=
     sum over N).
 
     Differentiable by the logits: with autograd recording, the gradient is formed with the loss in the same pass over
-    the logits and kept for the backward pass, which is free for "sum" and "mean" used as the loss itself; it can be
-    run once."""
+    the logits and kept in their dtype for the backward pass, which is free for "sum" and "mean" used as the loss itself;
+    another factor multiplies it there, in bfloat16 with a second rounding.  The backward pass can be run once.
+    Teacher, targets and weights get no gradient."""
     if reduction not in ("none", "sum", "mean"):
         raise ValueError(f"reduction is none, sum or mean, not {reduction!r}")
     args = (teacher_ids, teacher_logits, targets, temperature, alpha, row_weight, teacher_lse)
