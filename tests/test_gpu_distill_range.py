@@ -79,6 +79,17 @@ def check(x, ids, tl, tg, T, a, lse, with_loss=True):
     tol = PERR * M + (H * G.abs() if x.dtype == BF16 else 0) + 1e-37
     bad = ~((grad.double() - G).abs() <= tol)
     assert not bad.any(), ("gradient", bad.nonzero()[:5].tolist(), grad[bad][:5], G[bad][:5])
+    over = x.clone()  # over the logits
+    again = S.distill_loss_and_grad(over, ids, tl, tg, T, a, None, lse, out=over)
+    assert torch.equal(again[0], loss) and torch.equal(over, grad)
+    # rows at every kind of address, the gradient's at another
+    N, V = x.shape
+    wide, out = torch.zeros(N, V + 9, device=DEV, dtype=x.dtype), torch.zeros(N, V + 6, device=DEV, dtype=x.dtype)
+    wide[:, 3:V + 3] = x
+    S.distill_loss_and_grad(wide[:, 3:V + 3], ids, tl, tg, T, a, None, lse, out=out[:, 5:V + 5])
+    bad = ~((out[:, 5:V + 5].double() - G).abs() <= tol)
+    assert not bad.any(), ("gradient off 16 bytes", bad.nonzero()[:5].tolist())
+    assert (out[:, :5] == 0).all() and (out[:, V + 5:] == 0).all()
 
 
 # rows and vocabularies: a cluster of eight blocks per row, of two to four, a block per row, persistent blocks
