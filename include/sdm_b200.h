@@ -304,8 +304,9 @@ sdm_status sdm_logits_choose(const sdm_logit_rules* rules, const sdm_choice_para
  *   loss = row_weight (alpha soft + (1 - alpha) hard)    (row_weight (N) float32 or NULL = 1)
  * loss (N) float32.  dlogits (N, V) in dtype, row stride ld_grad, or NULL: grad_scale * d loss / d logits, rounded
  * once; may be logits itself (same stride), and may not overlap it otherwise.  A row whose weight is 0 is not read:
- * its loss and gradient are 0.  An id listed twice counts twice in p and once in q.  1 <= k <= 512, V <= 2^18.  Should
- * a wait of the kernel give up (sdm_device_status), the rows that it did not finish have a NaN loss. */
+ * its loss and gradient are 0.  An id listed twice counts twice in p and once in q.  1 <= k <= 512, V <= 2^18; 1 / T and
+ * T^2 are finite in float32.  Should a wait of the kernel give up (sdm_device_status), the rows that it did not finish
+ * have a NaN loss. */
 sdm_status sdm_distill(const void* logits, int64_t ld, int64_t N, int V, int dtype, const int32_t* teacher_ids,
                        const float* teacher_logits, int k, const float* teacher_lse, const int32_t* targets,
                        const float* row_weight, float temperature, float alpha, float grad_scale, float* loss,

@@ -70,7 +70,10 @@ sdm_status sdm_distill(const void* logits, int64_t ld, int64_t N, int V, int dty
   if ((N != 0 && (!logits || !teacher_ids || !teacher_logits || !loss)) || !dtype_ok(dtype) ||
       !aligned(logits, dtype) || !aligned(dlogits, dtype))
     return SDM_ERR_ARG;
-  if (!(temperature > 0.f) || isinf(temperature) || !isfinite(alpha) || !isfinite(grad_scale)) return SDM_ERR_ARG;
+  // 1 / T scales every logit, T^2 the loss
+  if (!(temperature > 0.f) || !isfinite(1.f / temperature) || !isfinite(temperature * temperature) || !isfinite(alpha) ||
+      !isfinite(grad_scale))
+    return SDM_ERR_ARG;
   if (N < 0 || N > 0x7fffffff / kMaxCluster || V < 1 || V > kMaxChoiceV || ld < V || (dlogits && ld_grad < V) ||
       k < 1 || k > kMaxTeacher)
     return SDM_ERR_SHAPE;

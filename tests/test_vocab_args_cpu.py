@@ -69,3 +69,13 @@ def test_outputs_beside_the_logits_in_one_buffer():
     flat = torch.zeros(100)
     with pytest.raises(ValueError):  # a row's end and the next one's beginning
         W._out_rows(flat[5:].as_strided((4, 10), (12, 1), 5), flat.as_strided((4, 10), (12, 1), 0), "out")
+
+
+def test_distillation_refuses_temperatures_whose_reciprocal_or_square_is_infinite():
+    import ctypes
+
+    from sdmchat_b200 import _lib
+    fake = ctypes.c_void_p(0x10000)  # never dereferenced
+    for T in (1e-40, 1e-45, 2e19, 3e38):
+        assert _lib.lib().sdm_distill(fake, 100, 3, 100, 0, fake, fake, 4, None, None, None, T, 0.5, 1.0, fake, None, 0,
+                                      None) == 1
